@@ -33,10 +33,12 @@
 extern "C" {
 #endif
 
-#define RECAP_ABI_VERSION 9
+#define RECAP_ABI_VERSION 10
 
 enum { RECAP_OK = 0, RECAP_EINVAL = 1, RECAP_EUNSUPPORTED = 2, RECAP_EHIP = 3 };
-enum { RECAP_F16 = 1, RECAP_BF16 = 2 };
+enum { RECAP_F16 = 1, RECAP_BF16 = 2, RECAP_F32 = 3 };  /* RECAP_F32: residual stream only */
+enum { RECAP_NORM_NONE = 0, RECAP_NORM_RMS = 1, RECAP_NORM_LAYER = 2, RECAP_NORM_RMS_ALL = 3 };
+enum { RECAP_PAIRS_INTERLEAVED = 0, RECAP_PAIRS_HALVES = 1 };
 enum { RECAP_CLOSURE_ROT = 1, RECAP_CLOSURE_CVK = 2, RECAP_CLOSURE_SCATTER = 4 };
 
 int recap_abi_version(void);
@@ -443,6 +445,80 @@ int recap_pager_resize(recap_pager* pager, const int64_t* field_bytes, int32_t n
  * `stream` (hipMemcpyAsync, direction inferred).
  * Replaces the non_blocking copy_ of recap/host_banks.py:99-103. */
 int recap_bank_copy_async(void* dst, const void* src, int64_t bytes, void* stream);
+
+/* Around the attention call ------------------------------------------------------------ */
+
+/* Queries and keys for recap_kv_pack and the attention entry points from their projections:
+ * an optional norm, then the rotation of the video tokens by their position on a
+ * (time, height, width) grid.
+ *  - norm RECAP_NORM_RMS or RECAP_NORM_LAYER over a head's dim channels (weight, bias [dim]),
+ *    RECAP_NORM_RMS_ALL over the heads * dim channels of a token (weight, bias
+ *    [heads * dim], head by head), RECAP_NORM_NONE for none.  Weights and biases may be NULL;
+ *    weight_dtype is the tensors' type or RECAP_F32.
+ *  - axis_tables[i] (fp32 [lengths[i], pairs[i], 2], device memory, 8-byte aligned): the
+ *    (cos, sin) of axis i (time, height, width) at each position; pairs[0] + pairs[1] +
+ *    pairs[2] = dim / 2, and an axis of no pairs may have a NULL table.  Token offset + v with
+ *    0 <= v < lengths[0] * lengths[1] * lengths[2] sits at (v / (H * W), v / W % H, v % W);
+ *    the other tokens (text) are not rotated.  Frequency i rotates channels (2i, 2i + 1)
+ *    (RECAP_PAIRS_INTERLEAVED) or (i, i + dim / 2) (RECAP_PAIRS_HALVES).  axis_tables NULL: no
+ *    rotation.
+ *  - k may be NULL.  An output may be its own input, and overlaps nothing else.
+ * No weights, sums or angles are kept from call to call.  Covers the query/key norm and the rotary embedding
+ * before operator.attend in the model processors, recap/models/hunyuan.py:79-154. */
+int recap_qk_rotary(const void* q, const void* k, int dtype, int64_t batch, int64_t tokens,
+                    int64_t dim, int64_t q_heads, int64_t k_heads, int64_t q_stride_b,
+                    int64_t q_stride_h, int64_t q_stride_n, int64_t k_stride_b,
+                    int64_t k_stride_h, int64_t k_stride_n, const float* const* axis_tables,
+                    const int64_t* lengths, const int64_t* pairs, int64_t offset, int pairing,
+                    int norm, const void* q_weight, const void* q_bias, const void* k_weight,
+                    const void* k_bias, int weight_dtype, float eps, void* q_out,
+                    int64_t qo_stride_b, int64_t qo_stride_h, int64_t qo_stride_n, void* k_out,
+                    int64_t ko_stride_b, int64_t ko_stride_h, int64_t ko_stride_n, void* stream);
+
+/* The residual stream x [batch, tokens, width] around a block, per row:
+ *   recap_norm_modulate        out = norm(x) * (1 + scale) + shift
+ *   recap_gated_residual       residual_out = x + gate * branch_norm(branch)
+ *   recap_gated_residual_norm  residual_out as above, and out = norm(the unrounded sum)
+ *                              * (1 + scale) + shift, in one pass
+ *  - The stream (x, residual_out) is of x_dtype, the branch and out of dtype: RECAP_BF16 or
+ *    RECAP_F16 for both, or an RECAP_F32 stream with any dtype.
+ *  - norm is RECAP_NORM_RMS or RECAP_NORM_LAYER, branch_norm either or RECAP_NORM_NONE, with
+ *    optional weight and bias [width] of weight_dtype (dtype or RECAP_F32).
+ *  - gate, scale and shift are optional, of mod_dtype (dtype or RECAP_F32); a stride of 0 along
+ *    batch or tokens broadcasts them.
+ *  - Strides are in elements, channels have unit stride, and nothing needs more than its
+ *    element's alignment.  residual_out may be x and out may be branch (for
+ *    recap_norm_modulate, x); outputs overlap nothing else.
+ * Statistics and products are fp32; each output is rounded once.  Covers the modulated norms
+ * and gated residuals of the transformer blocks whose processors call operator.attend,
+ * recap/models/hunyuan.py:79-154. */
+int recap_norm_modulate(const void* x, int x_dtype, int64_t batch, int64_t tokens,
+                        int64_t width, int64_t x_stride_b, int64_t x_stride_n,
+                        const void* scale, int64_t scale_stride_b, int64_t scale_stride_n,
+                        const void* shift, int64_t shift_stride_b, int64_t shift_stride_n,
+                        int mod_dtype, const void* weight, const void* bias, int weight_dtype,
+                        int norm, float eps, void* out, int dtype, int64_t out_stride_b,
+                        int64_t out_stride_n, void* stream);
+int recap_gated_residual(const void* x, int x_dtype, int64_t batch, int64_t tokens,
+                         int64_t width, int64_t x_stride_b, int64_t x_stride_n,
+                         const void* branch, int dtype, int64_t branch_stride_b,
+                         int64_t branch_stride_n, const void* gate, int64_t gate_stride_b,
+                         int64_t gate_stride_n, int mod_dtype, const void* branch_weight,
+                         const void* branch_bias, int weight_dtype, int branch_norm, float eps,
+                         void* residual_out, int64_t residual_stride_b,
+                         int64_t residual_stride_n, void* stream);
+int recap_gated_residual_norm(const void* x, int x_dtype, int64_t batch, int64_t tokens,
+                              int64_t width, int64_t x_stride_b, int64_t x_stride_n,
+                              const void* branch, int dtype, int64_t branch_stride_b,
+                              int64_t branch_stride_n, const void* gate, int64_t gate_stride_b,
+                              int64_t gate_stride_n, const void* scale, int64_t scale_stride_b,
+                              int64_t scale_stride_n, const void* shift, int64_t shift_stride_b,
+                              int64_t shift_stride_n, int mod_dtype, const void* branch_weight,
+                              const void* branch_bias, const void* weight, const void* bias,
+                              int weight_dtype, int branch_norm, int norm, float eps,
+                              void* residual_out, int64_t residual_stride_b,
+                              int64_t residual_stride_n, void* out, int64_t out_stride_b,
+                              int64_t out_stride_n, void* stream);
 
 #ifdef __cplusplus
 }

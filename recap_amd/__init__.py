@@ -18,21 +18,24 @@ from __future__ import annotations
 
 from typing import Any, Callable
 
+from .block import AttentionBlock
 from .config import (OperatingPoint, OperatorConfig, RecapConfig, config_from_dict,
                      load_config)
 from .controller import Controller
 from .host_banks import HostBankOperator
 from .layout import Layout, SparseGeometry, hilbert_permutation
 from .operator import EXACT, REFRESH, SPARSE, DetailBank, Operator, SparseAttention
+from .rotary import rotary_axes
 from .session import REUSE, RecapSession
 from .types import AttentionBranch, BlockSummary, ClosureBank
 
 __all__ = [
-    "EXACT", "REFRESH", "REUSE", "SPARSE", "AttentionBranch", "BlockSummary", "ClosureBank",
+    "EXACT", "REFRESH", "REUSE", "SPARSE", "AttentionBlock", "AttentionBranch", "BlockSummary",
+    "ClosureBank",
     "Controller", "DetailBank", "HostBankOperator",
     "Layout", "OperatingPoint", "Operator", "OperatorConfig", "RecapConfig", "RecapSession",
     "SparseAttention", "SparseGeometry", "config_from_dict", "hilbert_permutation", "install",
-    "load_config", "register_builder",
+    "load_config", "register_builder", "rotary_axes",
 ]
 
 # model name -> build_operator(pipe, config) -> (operator, info), the contract of the

@@ -11,16 +11,19 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "librecap_hip.so"
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 RECAP_OK, RECAP_EINVAL, RECAP_EUNSUPPORTED, RECAP_EHIP = 0, 1, 2, 3
-RECAP_F16, RECAP_BF16 = 1, 2
+RECAP_F16, RECAP_BF16, RECAP_F32 = 1, 2, 3
+NORM_NONE, NORM_RMS, NORM_LAYER, NORM_RMS_ALL = 0, 1, 2, 3
+PAIRS_INTERLEAVED, PAIRS_HALVES = 0, 1
 CLOSURE_ROT, CLOSURE_CVK, CLOSURE_SCATTER = 1, 2, 4
 CAPTURE_NOALLOC_MAX_PAIRS = 1 << 19  # RECAP_CAPTURE_NOALLOC_MAX_PAIRS
 PAGER_TIMING = 1  # RECAP_PAGER_TIMING
 
 _P, _I64, _I, _F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
 _STRIDES = [_I64, _I64, _I64]
+_ROWS = [_P, _I64, _I64]  # rows [batch, tokens] of unit-stride channels
 
 # name -> (restype, argtypes), exactly the prototypes of include/recap_hip.h
 SIGNATURES: dict[str, tuple] = {
@@ -96,6 +99,15 @@ SIGNATURES: dict[str, tuple] = {
     "recap_pager_copy_time": (_I, [_P, _P, _P]),
     "recap_pager_resize": (_I, [_P, _P, ctypes.c_int32]),
     "recap_bank_copy_async": (_I, [_P, _P, _I64, _P]),
+    "recap_qk_rotary": (_I, [_P, _P, _I, *([_I64] * 5), *_STRIDES, *_STRIDES, _P, _P, _P, _I64, _I,
+                             _I, _P, _P, _P, _P, _I, _F, _P, *_STRIDES, _P, *_STRIDES, _P]),
+    "recap_norm_modulate": (_I, [_P, _I, _I64, _I64, _I64, _I64, _I64, *_ROWS, *_ROWS, _I, _P, _P,
+                                 _I, _I, _F, _P, _I, _I64, _I64, _P]),
+    "recap_gated_residual": (_I, [_P, _I, _I64, _I64, _I64, _I64, _I64, _P, _I, _I64, _I64, *_ROWS,
+                                  _I, _P, _P, _I, _I, _F, *_ROWS, _P]),
+    "recap_gated_residual_norm": (_I, [_P, _I, _I64, _I64, _I64, _I64, _I64, _P, _I, _I64, _I64,
+                                       *_ROWS, *_ROWS, *_ROWS, _I, _P, _P, _P, _P, _I, _I, _I, _F,
+                                       *_ROWS, *_ROWS, _P]),
 }
 
 _lock = threading.Lock()

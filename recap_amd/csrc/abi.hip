@@ -1062,4 +1062,230 @@ int recap_bank_copy_async(void* dst, const void* src, int64_t bytes, void* strea
                     "hipMemcpyAsync");
 }
 
+// Around the attention call ---------------------------------------------------------------
+
+int recap_qk_rotary(const void* q, const void* k, int dtype, int64_t batch, int64_t tokens,
+                    int64_t dim, int64_t q_heads, int64_t k_heads, int64_t q_stride_b,
+                    int64_t q_stride_h, int64_t q_stride_n, int64_t k_stride_b,
+                    int64_t k_stride_h, int64_t k_stride_n, const float* const* axis_tables,
+                    const int64_t* lengths, const int64_t* pairs, int64_t offset, int pairing,
+                    int norm, const void* q_weight, const void* q_bias, const void* k_weight,
+                    const void* k_bias, int weight_dtype, float eps, void* q_out,
+                    int64_t qo_stride_b, int64_t qo_stride_h, int64_t qo_stride_n, void* k_out,
+                    int64_t ko_stride_b, int64_t ko_stride_h, int64_t ko_stride_n,
+                    void* stream) {
+  CHECK(check_common(dtype, dim));
+  REQUIRE(tokens >= 1 && tokens <= INT32_MAX, "tokens %lld outside 1..2^31-1", (long long)tokens);
+  CHECK(check_qkv("q", q, batch, q_heads, q_stride_b, q_stride_h, q_stride_n));
+  CHECK(check_qkv("q_out", q_out, batch, q_heads, qo_stride_b, qo_stride_h, qo_stride_n));
+  REQUIRE(batch <= INT32_MAX / tokens, "batch * tokens exceeds 2^31-1");
+  REQUIRE(q_heads <= kRotaryMaxHeads, "q_heads %lld exceeds %d", (long long)q_heads,
+          kRotaryMaxHeads);
+  REQUIRE((k == nullptr) == (k_out == nullptr), "k and k_out go together");
+  RotaryArgs a{};
+  a.x[0] = {static_cast<const uint16_t*>(q), q_stride_b, q_stride_h, q_stride_n,
+            static_cast<uint16_t*>(q_out), qo_stride_b, qo_stride_h, qo_stride_n, q_weight,
+            q_bias, (int)q_heads};
+  a.tensors = 1;
+  if (k != nullptr) {
+    CHECK(check_qkv("k", k, batch, k_heads, k_stride_b, k_stride_h, k_stride_n));
+    CHECK(check_qkv("k_out", k_out, batch, k_heads, ko_stride_b, ko_stride_h, ko_stride_n));
+    REQUIRE(k_heads <= kRotaryMaxHeads, "k_heads %lld exceeds %d", (long long)k_heads,
+            kRotaryMaxHeads);
+    a.x[1] = {static_cast<const uint16_t*>(k), k_stride_b, k_stride_h, k_stride_n,
+              static_cast<uint16_t*>(k_out), ko_stride_b, ko_stride_h, ko_stride_n, k_weight,
+              k_bias, (int)k_heads};
+    a.tensors = 2;
+  }
+  REQUIRE(norm >= RECAP_NORM_NONE && norm <= RECAP_NORM_RMS_ALL, "unknown norm %d", norm);
+  REQUIRE(pairing == RECAP_PAIRS_INTERLEAVED || pairing == RECAP_PAIRS_HALVES,
+          "unknown pairing %d", pairing);
+  REQUIRE(norm == RECAP_NORM_NONE || (std::isfinite(eps) && eps > 0.0f),
+          "eps must be positive and finite, got %g", (double)eps);
+  REQUIRE(norm != RECAP_NORM_NONE || !(q_weight || q_bias || k_weight || k_bias),
+          "weights and biases need a norm");
+  REQUIRE(weight_dtype == dtype || weight_dtype == RECAP_F32,
+          "weight_dtype %d is neither the tensors' nor RECAP_F32", weight_dtype);
+  const uintptr_t weight_align = weight_dtype == RECAP_F32 ? 3 : 1;
+  for (const void* w : {q_weight, q_bias, k_weight, k_bias})
+    REQUIRE((reinterpret_cast<uintptr_t>(w) & weight_align) == 0, "a weight is misaligned");
+  if (axis_tables != nullptr) {
+    REQUIRE(lengths && pairs, "lengths and pairs must be non-NULL");
+    int64_t total = 0, video = 1;
+    for (int i = 0; i < 3; ++i) {
+      REQUIRE(lengths[i] >= 1 && lengths[i] <= tokens, "axis %d: length %lld outside 1..tokens", i,
+              (long long)lengths[i]);
+      REQUIRE(pairs[i] >= 0 && pairs[i] <= dim / 2, "axis %d: %lld pairs outside 0..dim/2", i,
+              (long long)pairs[i]);
+      REQUIRE(pairs[i] == 0 || axis_tables[i] != nullptr, "axis %d: table is NULL", i);
+      REQUIRE((reinterpret_cast<uintptr_t>(axis_tables[i]) & 7) == 0,
+              "axis %d: table is not 8-byte aligned", i);
+      total += pairs[i];
+      video *= lengths[i];
+      REQUIRE(video <= tokens, "the grid has more positions than the call has tokens");
+      a.axis[i] = {axis_tables[i], (int)lengths[i], (int)pairs[i]};
+    }
+    REQUIRE(total == dim / 2, "the axes have %lld pairs, dim / 2 is %lld", (long long)total,
+            (long long)(dim / 2));
+    REQUIRE(offset >= 0 && offset <= tokens - video, "offset %lld outside 0..%lld",
+            (long long)offset, (long long)(tokens - video));
+    a.offset = offset;
+    a.video = video;
+  }
+  a.rows = batch * tokens;
+  a.tokens = tokens;
+  a.norm = norm;
+  a.halves = pairing == RECAP_PAIRS_HALVES;
+  a.wide_weight = weight_dtype == RECAP_F32;
+  a.eps = eps;
+  return hip_status(run_rotary(a, dtype, (int)dim, as_stream(stream)), "qk_rotary launch");
+}
+
+namespace {
+
+bool stream_dtype(int t) { return t == RECAP_BF16 || t == RECAP_F16 || t == RECAP_F32; }
+
+// A row view of a call's tensors: alignment of its element type, strides that are
+// non-negative, and for an output rows that do not overlap.
+int check_rows(const char* name, const void* p, int dtype, int64_t batch, int64_t tokens,
+               int64_t width, int64_t sb, int64_t sn, bool output) {
+  const uintptr_t align = dtype == RECAP_F32 ? 3 : 1;
+  REQUIRE((reinterpret_cast<uintptr_t>(p) & align) == 0, "%s is misaligned for its type", name);
+  REQUIRE(sb >= 0 && sn >= 0, "%s strides (%lld, %lld) must be non-negative", name,
+          (long long)sb, (long long)sn);
+  if (!output) return RECAP_OK;
+  const bool by_batch = batch == 1 || sb >= (tokens - 1) * sn + width;
+  const bool by_token = tokens == 1 || sn >= (batch - 1) * sb + width;
+  REQUIRE((tokens == 1 || sn >= width) && (batch == 1 || sb >= width) && (by_batch || by_token),
+          "%s strides (%lld, %lld) let rows overlap", name, (long long)sb, (long long)sn);
+  return RECAP_OK;
+}
+
+// Checks of the three residual-stream entry points, and the launch.
+int residual(ResidualArgs& a, const char* what, int x_dtype, int dtype, int mod_dtype,
+             int weight_dtype, int64_t batch, int64_t tokens, int64_t width, void* stream) {
+  REQUIRE(stream_dtype(x_dtype) && stream_dtype(dtype), "%s: unknown dtype %d or %d", what,
+          x_dtype, dtype);
+  REQUIRE(x_dtype == dtype || x_dtype == RECAP_F32,
+          "%s: the stream is of the branch's type or fp32", what);
+  REQUIRE(mod_dtype == dtype || mod_dtype == RECAP_F32,
+          "%s: gate, scale and shift are of the branch's type or fp32", what);
+  REQUIRE(weight_dtype == dtype || weight_dtype == RECAP_F32,
+          "%s: weights are of the branch's type or fp32", what);
+  REQUIRE(batch >= 1 && tokens >= 1 && width >= 1, "%s: sizes must be positive", what);
+  REQUIRE(width <= (1 << 24), "%s: width %lld exceeds 2^24", what, (long long)width);
+  REQUIRE(tokens <= INT32_MAX && batch <= INT32_MAX / tokens, "%s: batch * tokens exceeds 2^31-1",
+          what);
+  REQUIRE(std::isfinite(a.eps) && a.eps > 0.0f, "%s: eps must be positive and finite, got %g",
+          what, (double)a.eps);
+  const struct { const char* name; const RowView& v; int dtype; bool output; } views[] = {
+      {"x", a.x, x_dtype, false}, {"branch", a.branch, dtype, false},
+      {"gate", a.gate, mod_dtype, false}, {"scale", a.scale, mod_dtype, false},
+      {"shift", a.shift, mod_dtype, false}, {"residual_out", a.r, x_dtype, true},
+      {"out", a.y, dtype, true}};
+  for (const auto& v : views)
+    if (v.v.p)
+      CHECK(check_rows(v.name, v.v.p, v.dtype, batch, tokens, width, v.v.b, v.v.n, v.output));
+  const uintptr_t align = weight_dtype == RECAP_F32 ? 3 : 1;
+  for (const void* w : {a.branch_weight, a.branch_bias, a.weight, a.bias})
+    REQUIRE((reinterpret_cast<uintptr_t>(w) & align) == 0, "%s: a weight is misaligned", what);
+  a.rows = batch * tokens;
+  a.tokens = tokens;
+  a.width = (int)width;
+  a.wide_mod = mod_dtype == RECAP_F32;
+  a.wide_weight = weight_dtype == RECAP_F32;
+  return hip_status(run_residual(a, x_dtype, dtype, as_stream(stream)), what);
+}
+
+}  // namespace
+
+int recap_norm_modulate(const void* x, int x_dtype, int64_t batch, int64_t tokens,
+                        int64_t width, int64_t x_stride_b, int64_t x_stride_n,
+                        const void* scale, int64_t scale_stride_b, int64_t scale_stride_n,
+                        const void* shift, int64_t shift_stride_b, int64_t shift_stride_n,
+                        int mod_dtype, const void* weight, const void* bias, int weight_dtype,
+                        int norm, float eps, void* out, int dtype, int64_t out_stride_b,
+                        int64_t out_stride_n, void* stream) {
+  REQUIRE(x && out, "norm_modulate: x and out must be non-NULL");
+  REQUIRE(norm == RECAP_NORM_RMS || norm == RECAP_NORM_LAYER, "norm_modulate: unknown norm %d",
+          norm);
+  ResidualArgs a{};
+  a.x = {x, x_stride_b, x_stride_n};
+  a.scale = {scale, scale_stride_b, scale_stride_n};
+  a.shift = {shift, shift_stride_b, shift_stride_n};
+  a.y = {out, out_stride_b, out_stride_n};
+  a.weight = weight;
+  a.bias = bias;
+  a.norm = norm;
+  a.eps = eps;
+  return residual(a, "norm_modulate", x_dtype, dtype, mod_dtype, weight_dtype, batch, tokens,
+                  width, stream);
+}
+
+int recap_gated_residual(const void* x, int x_dtype, int64_t batch, int64_t tokens,
+                         int64_t width, int64_t x_stride_b, int64_t x_stride_n,
+                         const void* branch, int dtype, int64_t branch_stride_b,
+                         int64_t branch_stride_n, const void* gate, int64_t gate_stride_b,
+                         int64_t gate_stride_n, int mod_dtype, const void* branch_weight,
+                         const void* branch_bias, int weight_dtype, int branch_norm, float eps,
+                         void* residual_out, int64_t residual_stride_b,
+                         int64_t residual_stride_n, void* stream) {
+  REQUIRE(x && branch && residual_out,
+          "gated_residual: x, branch and residual_out must be non-NULL");
+  REQUIRE(branch_norm >= RECAP_NORM_NONE && branch_norm <= RECAP_NORM_LAYER,
+          "gated_residual: unknown branch norm %d", branch_norm);
+  REQUIRE(branch_norm != RECAP_NORM_NONE || !(branch_weight || branch_bias),
+          "gated_residual: branch weights need a branch norm");
+  ResidualArgs a{};
+  a.x = {x, x_stride_b, x_stride_n};
+  a.branch = {branch, branch_stride_b, branch_stride_n};
+  a.gate = {gate, gate_stride_b, gate_stride_n};
+  a.r = {residual_out, residual_stride_b, residual_stride_n};
+  a.branch_weight = branch_weight;
+  a.branch_bias = branch_bias;
+  a.post = branch_norm;
+  a.eps = eps;
+  return residual(a, "gated_residual", x_dtype, dtype, mod_dtype, weight_dtype, batch, tokens,
+                  width, stream);
+}
+
+int recap_gated_residual_norm(const void* x, int x_dtype, int64_t batch, int64_t tokens,
+                              int64_t width, int64_t x_stride_b, int64_t x_stride_n,
+                              const void* branch, int dtype, int64_t branch_stride_b,
+                              int64_t branch_stride_n, const void* gate, int64_t gate_stride_b,
+                              int64_t gate_stride_n, const void* scale, int64_t scale_stride_b,
+                              int64_t scale_stride_n, const void* shift, int64_t shift_stride_b,
+                              int64_t shift_stride_n, int mod_dtype, const void* branch_weight,
+                              const void* branch_bias, const void* weight, const void* bias,
+                              int weight_dtype, int branch_norm, int norm, float eps,
+                              void* residual_out, int64_t residual_stride_b,
+                              int64_t residual_stride_n, void* out, int64_t out_stride_b,
+                              int64_t out_stride_n, void* stream) {
+  REQUIRE(x && branch && residual_out && out,
+          "gated_residual_norm: x, branch, residual_out and out must be non-NULL");
+  REQUIRE(branch_norm >= RECAP_NORM_NONE && branch_norm <= RECAP_NORM_LAYER,
+          "gated_residual_norm: unknown branch norm %d", branch_norm);
+  REQUIRE(branch_norm != RECAP_NORM_NONE || !(branch_weight || branch_bias),
+          "gated_residual_norm: branch weights need a branch norm");
+  REQUIRE(norm == RECAP_NORM_RMS || norm == RECAP_NORM_LAYER,
+          "gated_residual_norm: unknown norm %d", norm);
+  ResidualArgs a{};
+  a.x = {x, x_stride_b, x_stride_n};
+  a.branch = {branch, branch_stride_b, branch_stride_n};
+  a.gate = {gate, gate_stride_b, gate_stride_n};
+  a.scale = {scale, scale_stride_b, scale_stride_n};
+  a.shift = {shift, shift_stride_b, shift_stride_n};
+  a.r = {residual_out, residual_stride_b, residual_stride_n};
+  a.y = {out, out_stride_b, out_stride_n};
+  a.branch_weight = branch_weight;
+  a.branch_bias = branch_bias;
+  a.weight = weight;
+  a.bias = bias;
+  a.post = branch_norm;
+  a.norm = norm;
+  a.eps = eps;
+  return residual(a, "gated_residual_norm", x_dtype, dtype, mod_dtype, weight_dtype, batch,
+                  tokens, width, stream);
+}
+
 }  // extern "C"

@@ -162,6 +162,43 @@ hipError_t capture_scratch_pointer(float** out);
 hipError_t run_drift_center(const float* part, int banks, int tiles, int rows, float* center,
                             hipStream_t s);
 
+// Norms before and after a block with its scale, shift, gate and residual (residual.hip).
+enum NormKind { kNormNone = 0, kNormRms = 1, kNormLayer = 2 };
+struct RowView {                                 // rows [batch][tokens] of unit-stride channels
+  const void* p; int64_t b, n;                   // element strides; p null: absent
+};
+struct ResidualArgs {
+  RowView x, branch, gate, scale, shift;
+  RowView r, y;                                  // outputs: new residual, normalised rows
+  const void* branch_weight; const void* branch_bias;
+  const void* weight; const void* bias;
+  int64_t rows, tokens; int width;
+  int post, norm;                                // NormKind of the branch and of the result
+  bool wide_mod, wide_weight;                    // fp32 gate/scale/shift, fp32 weights
+  float eps;
+};
+hipError_t run_residual(const ResidualArgs& a, int x_dtype, int dtype, hipStream_t s);
+
+// Norm and rotation of queries and keys (rotary.hip).
+constexpr int kRotaryMaxHeads = 1 << 16;
+enum RotaryNorm { kRotaryNone = 0, kRotaryRms = 1, kRotaryLayer = 2, kRotaryRmsAll = 3 };
+struct RotaryAxis {
+  const float* table; int length, pairs;         // (cos, sin) [length][pairs][2]
+};
+struct RotaryTensor {
+  const uint16_t* in; int64_t in_b, in_h, in_n;
+  uint16_t* out; int64_t out_b, out_h, out_n;
+  const void* weight; const void* bias; int heads;
+};
+struct RotaryArgs {
+  RotaryTensor x[2]; int tensors;                // q, then k
+  RotaryAxis axis[3];                            // time, height, width
+  int64_t rows, tokens, offset, video;           // batch * tokens; first and number of video tokens
+  int norm; bool halves, wide_weight;
+  float eps;
+};
+hipError_t run_rotary(const RotaryArgs& a, int dtype, int dim, hipStream_t s);
+
 // Host-bank pager (pager.hip): pinned host banks, device slots, prefetch and write-back
 // streams.  Slot and key indices are checked by the caller (abi.hip).
 struct Pager;

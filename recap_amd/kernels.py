@@ -626,6 +626,351 @@ def refresh_capture_noalloc(dense_out: torch.Tensor, dense_lse: torch.Tensor,
          _p(glref), _p(center), _p(stats), _stream())
 
 
+# -- around the attention call --------------------------------------------------------------
+
+_NORMS = {None: _lib.NORM_NONE, "rms": _lib.NORM_RMS, "layer": _lib.NORM_LAYER}
+_QK_NORMS = {**_NORMS, "rms_all": _lib.NORM_RMS_ALL}
+_PAIRINGS = {"interleaved": _lib.PAIRS_INTERLEAVED, "halves": _lib.PAIRS_HALVES}
+_STREAM_DTYPES = {torch.float16: _lib.RECAP_F16, torch.bfloat16: _lib.RECAP_BF16,
+                  torch.float32: _lib.RECAP_F32}
+
+
+def _choice(table: dict, value, what: str) -> int:
+    if value not in table:
+        raise ValueError(f"unknown {what} {value!r}; use one of {list(table)}")
+    return table[value]
+
+
+def _together(tensors: dict[str, torch.Tensor | None]) -> torch.device:
+    """The GPU that all tensors of a call are on.  The kernels have no backward pass, so a
+    call that would have to record one is refused."""
+    device = next(iter(tensors.values())).device
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a GPU tensor")
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the call on {device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} requires a gradient, which this call does not record: run it "
+                             "under torch.no_grad()")
+    return device
+
+
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """Call on the current stream of `device`, which need not be the current device."""
+    if torch.cuda.current_device() == device.index:
+        call(name, *args, _stream())
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, _stream())
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """First and one-past-last byte address of a tensor's elements."""
+    last = sum((size - 1) * stride for size, stride in zip(t.shape, t.stride()))
+    start = t.data_ptr()
+    return start, start + (last + 1) * t.element_size()
+
+
+def _interleaved(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Two tensors that take turns within rows of one pitch (q and k of a fused projection)
+    and share no element."""
+    if a.element_size() != b.element_size() or (b.data_ptr() - a.data_ptr()) % a.element_size():
+        return False
+    steps = [[(st, n) for st, n in zip(t.stride(), t.shape) if n > 1] for t in (a, b)]
+    for pitch in {st for st, _ in steps[0]} & {st for st, _ in steps[1]}:
+        if any(st > pitch and st % pitch for t in steps for st, _ in t):
+            continue
+        width_a, width_b = (1 + sum((n - 1) * st for st, n in t if st < pitch) for t in steps)
+        shift = (b.data_ptr() - a.data_ptr()) // a.element_size() % pitch
+        if width_a <= shift and shift + width_b <= pitch:
+            return True
+    return False
+
+
+def _check_output(name: str, out: torch.Tensor, shape, dtype: torch.dtype,
+                  inputs: dict[str, torch.Tensor | None], same: str) -> None:
+    """A given output: of the right kind, no element of it twice in memory, and over no input's
+    memory but that of input `same`, whose exact view it may be."""
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
+        raise ValueError(f"{name} is {tuple(out.shape)} {out.dtype}, expected {tuple(shape)} "
+                         f"{dtype}")
+    if out.stride(-1) != 1 and out.shape[-1] > 1:
+        raise ValueError(f"{name} must have unit stride along its last dimension")
+    extent = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(out.stride(), out.shape) if sz > 1):
+        if stride < extent:
+            raise ValueError(f"{name} has elements that share memory")
+        extent += (size - 1) * stride
+    if out.numel() == 0:
+        return
+    lo, hi = _span(out)
+    for other, t in inputs.items():
+        if t is None or t.numel() == 0:
+            continue
+        if other == same and t.data_ptr() == lo and t.dtype == dtype and all(
+                a == b or n == 1 for a, b, n in zip(t.stride(), out.stride(), out.shape)):
+            continue
+        start, end = _span(t)
+        if start < hi and lo < end and not _interleaved(out, t):
+            raise ValueError(f"{name} overlaps the memory of {other}")
+
+
+def _qk_weights(kind: int, extent: int, dtype: torch.dtype, vectors: dict) -> int:
+    """Type code of the weights and biases of a norm over `extent` channels."""
+    given = {name: v for name, v in vectors.items() if v is not None}
+    if given and kind == _lib.NORM_NONE:
+        raise ValueError(f"{next(iter(given))} needs a norm")
+    types = {v.dtype for v in given.values()} or {dtype}
+    if len(types) > 1 or not types <= {dtype, torch.float32}:
+        raise ValueError(f"weights and biases must all be {dtype} or all torch.float32")
+    for name, v in given.items():
+        if tuple(v.shape) != (extent,):
+            raise ValueError(f"{name} is {tuple(v.shape)}, expected ({extent},)")
+    return _STREAM_DTYPES[types.pop()]
+
+
+def qk_rotary(q: torch.Tensor, k: torch.Tensor | None = None, axes=None, *, offset: int = 0,
+              pairing: str = "interleaved", norm: str | None = None,
+              q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
+              q_bias: torch.Tensor | None = None, k_bias: torch.Tensor | None = None,
+              eps: float = 1e-6, q_out: torch.Tensor | None = None,
+              k_out: torch.Tensor | None = None):
+    """Queries and keys for the attention call from their projections: (q, k), k None without
+    one.  ``q`` and ``k`` are ``[B, heads, N, d]`` (any strides: views of a projection
+    ``[B, N, heads * d]`` or of a fused one are read in place), each with its own heads.
+
+    ``norm`` comes first: ``"rms"`` or ``"layer"`` over a head's channels (weights ``[d]``),
+    ``"rms_all"`` over all heads' of a token (weights ``[heads * d]``), or None.  Then the tokens
+    ``offset .. offset + T*H*W - 1`` are rotated by their place on the (T, H, W) grid of ``axes``,
+    three fp32 tables ``[length, channels / 2, 2]`` of (cos, sin), as recap_amd.rotary_axes makes
+    them; the others (text) are not.  ``pairing``: channels ``(2i, 2i + 1)`` (``"interleaved"``) or
+    ``(i, i + d / 2)`` (``"halves"``).  ``axes=None`` rotates nothing.
+
+    ``q_out`` and ``k_out`` may be ``q`` and ``k`` themselves, or views into a longer sequence
+    (a text stream's part of it)."""
+    kind = _choice(_QK_NORMS, norm, "norm")
+    pairs = _choice(_PAIRINGS, pairing, "pairing")
+    given = {"q": q, "k": k}
+    for name, x in given.items():
+        if x is None:
+            continue
+        if x.ndim != 4:
+            raise ValueError(f"{name} must be [batch, heads, tokens, dim], got {tuple(x.shape)}")
+        dtype_code(x.dtype)
+        if x.shape[-1] not in (64, 128):
+            raise ValueError(f"{name}: head dim {x.shape[-1]} unsupported (64 or 128)")
+    if k is not None and (k.dtype != q.dtype or k.shape[0] != q.shape[0]
+                          or k.shape[2:] != q.shape[2:]):
+        raise ValueError(f"K {tuple(k.shape)} {k.dtype} does not match Q {tuple(q.shape)} {q.dtype}")
+    if k is None and not k_weight is k_bias is k_out is None:
+        raise ValueError("k_weight, k_bias and k_out need a k")
+    b, h, n, d = q.shape
+    heads_k = 0 if k is None else k.shape[1]
+    spread = lambda heads: heads * d if kind == _lib.NORM_RMS_ALL else d  # noqa: E731
+    wide = {_qk_weights(kind, spread(heads), q.dtype, vectors)
+            for heads, vectors in ((h, {"q_weight": q_weight, "q_bias": q_bias}),
+                                   (heads_k, {"k_weight": k_weight, "k_bias": k_bias}))
+            if any(v is not None for v in vectors.values())}
+    if len(wide) > 1:
+        raise ValueError("the weights of q and k must have one type")
+    weight_code = wide.pop() if wide else _STREAM_DTYPES[q.dtype]
+    tables: list[torch.Tensor] = []
+    if axes is not None:
+        tables = list(axes)
+        if len(tables) != 3:
+            raise ValueError(f"axes must be three tables (time, height, width), got {len(tables)}")
+        for i, t in enumerate(tables):
+            if t.ndim != 3 or t.shape[2] != 2 or t.dtype != torch.float32 or t.shape[0] < 1:
+                raise ValueError(f"axis {i} must be fp32 [length, channels / 2, 2], got "
+                                 f"{tuple(t.shape)} {t.dtype}")
+        if sum(t.shape[1] for t in tables) != d // 2:
+            raise ValueError(f"the axes rotate {[2 * t.shape[1] for t in tables]} channels, the heads "
+                             f"have {d}")
+        video = math.prod(t.shape[0] for t in tables)
+        if not 0 <= offset <= n - video:
+            raise ValueError(f"tokens {offset}..{offset + video - 1} are not all in the sequence "
+                             f"of {n}")
+    inputs = {"q": q, "k": k, "q_weight": q_weight, "q_bias": q_bias, "k_weight": k_weight,
+              "k_bias": k_bias, **{f"axis {i}": t for i, t in enumerate(tables)}}
+    device = _together({**inputs, "q_out": q_out, "k_out": k_out})
+    outs = []
+    for name, x, out in (("q", q, q_out), ("k", k, k_out)):
+        if x is None:
+            outs.append(None)
+        elif out is None:
+            outs.append(torch.empty(x.shape, dtype=x.dtype, device=device))
+        else:
+            _check_output(f"{name}_out", out, x.shape, x.dtype, inputs, name)
+            if out.data_ptr() % 16 or any(s % 8 for s in out.stride()[:3]):
+                raise ValueError(f"{name}_out must have 16-byte aligned rows")
+            outs.append(out)
+    if q_out is not None and k_out is not None:
+        _check_output("k_out", k_out, k.shape, k.dtype, {"q_out": q_out}, "")
+    if q.numel() == 0 and (k is None or k.numel() == 0):
+        return tuple(outs)
+    if q.numel() == 0 or (k is not None and k.numel() == 0):
+        raise ValueError("q and k must both have heads")
+    q, k = prepare(q, "q"), None if k is None else prepare(k, "k")
+    tables = [t.contiguous() for t in tables]
+    vectors = [None if v is None else v.contiguous() for v in (q_weight, q_bias, k_weight, k_bias)]
+    pointers = lengths = counts = None
+    if tables:
+        pointers = (ctypes.c_void_p * 3)(*(t.data_ptr() if t.numel() else None for t in tables))
+        lengths = (ctypes.c_int64 * 3)(*(t.shape[0] for t in tables))
+        counts = (ctypes.c_int64 * 3)(*(t.shape[1] for t in tables))
+    none = (0, 0, 0)
+    _call_on(device, "recap_qk_rotary", q.data_ptr(), _p(k), dtype_code(q.dtype), b, n, d, h,
+             heads_k, *q.stride()[:3], *(none if k is None else k.stride()[:3]), pointers, lengths,
+             counts, int(offset), pairs, kind, *map(_p, vectors), weight_code, float(eps),
+             outs[0].data_ptr(), *outs[0].stride()[:3], _p(outs[1]),
+             *(none if k is None else outs[1].stride()[:3]))
+    return tuple(outs)
+
+
+def _rows(t: torch.Tensor | None) -> tuple:
+    """Pointer and (batch, token) strides of a [batch, tokens, width] tensor."""
+    return (None, 0, 0) if t is None else (t.data_ptr(), *t.stride()[:2])
+
+
+def _unit(t: torch.Tensor | None) -> torch.Tensor | None:
+    """The tensor with unit stride along its channels, as the kernels read it."""
+    return t if t is None or t.stride(-1) == 1 else t.contiguous()
+
+
+def _modulation(vectors: dict[str, torch.Tensor | None], x: torch.Tensor,
+                dtype: torch.dtype) -> tuple[int, list]:
+    """(type code, (pointer, batch stride, token stride) each) of gate, scale and shift:
+    ``[width]``, ``[B or 1, width]`` or ``[B or 1, N or 1, width]``."""
+    given = [v for v in vectors.values() if v is not None]
+    types = {v.dtype for v in given} or {dtype}
+    if len(types) > 1 or not types <= {dtype, torch.float32}:
+        raise ValueError(f"{', '.join(vectors)} must all be {dtype} or all torch.float32")
+    batch, tokens, width = x.shape
+    rows = []
+    for name, v in vectors.items():
+        if v is None:
+            rows.append(None)
+            continue
+        lead = tuple(v.shape[:-1])
+        if v.ndim < 1 or v.ndim > 3 or v.shape[-1] != width or not all(
+                got in (1, full) for got, full in zip(lead, (batch, tokens))):
+            raise ValueError(f"{name} is {tuple(v.shape)}: expected [{width}], [{batch} or 1, {width}] "
+                             f"or [{batch} or 1, {tokens} or 1, {width}]")
+        v = _unit(v)
+        rows.append((v, *(v.stride(i) if v.shape[i] > 1 else 0 for i in range(len(lead))),
+                     *(0,) * (2 - len(lead))))
+    return _STREAM_DTYPES[types.pop()], rows
+
+
+def _residual_call(name: str, x: torch.Tensor, dtype: torch.dtype, *, branch=None, mods=None,
+                   norms=(), eps=1e-6, outs=()) -> tuple[torch.Tensor, ...]:
+    """Checks and launch of the residual-stream calls.  ``mods``: gate, scale and shift by
+    name; ``norms``: (kind, prefix, weight, bias) of the branch's and the result's norm;
+    ``outs``: (name, given tensor or None, type, the input it may be)."""
+    if x.ndim != 3 or x.shape[-1] < 1:
+        raise ValueError(f"x must be [batch, tokens, width], got {tuple(x.shape)}")
+    if x.dtype not in _STREAM_DTYPES or dtype not in _STREAM_DTYPES:
+        raise ValueError(f"unsupported dtype {x.dtype if x.dtype not in _STREAM_DTYPES else dtype}; "
+                         "use bfloat16, float16 or float32")
+    if x.dtype not in (dtype, torch.float32):
+        raise ValueError(f"a {x.dtype} stream goes with a branch and an output of its own type, not "
+                         f"{dtype}; a float32 stream goes with any")
+    if branch is not None and branch.shape != x.shape:
+        raise ValueError(f"branch is {tuple(branch.shape)}, the stream {tuple(x.shape)}")
+    inputs = {"x": x, "branch": branch, **mods}
+    vectors = {}
+    for kind, prefix, weight, bias in norms:
+        pair = {f"{prefix}weight": weight, f"{prefix}bias": bias}
+        _qk_weights(kind, x.shape[-1], dtype, pair)
+        vectors.update(pair)
+    weight_code = _qk_weights(_lib.NORM_RMS, x.shape[-1], dtype, vectors)
+    inputs.update(vectors)
+    mod_code, mod_rows = _modulation(mods, x, dtype)
+    device = _together({**inputs, **{o[0]: o[1] for o in outs}})
+    made = []
+    for out_name, out, out_dtype, same in outs:
+        if out is None:
+            out = torch.empty(x.shape, dtype=out_dtype, device=device)
+        else:
+            others = {f"the other output ({o[0]})": m for o, m in zip(outs, made)}
+            _check_output(out_name, out, x.shape, out_dtype, {**inputs, **others}, same)
+        made.append(out)
+    if x.numel() == 0:
+        return tuple(made)
+    x, branch = _unit(x), _unit(branch)
+    vectors = {key: _unit(v) for key, v in vectors.items()}
+    mod_args = [(None, 0, 0) if m is None else (m[0].data_ptr(), *m[1:]) for m in mod_rows]
+    args = [x.data_ptr(), _STREAM_DTYPES[x.dtype], *x.shape, *x.stride()[:2]]
+    if branch is not None:
+        args += [branch.data_ptr(), _STREAM_DTYPES[dtype], *branch.stride()[:2]]
+    args += [a for m in mod_args for a in m]
+    args += [mod_code, *map(_p, vectors.values()), weight_code, *(n[0] for n in norms), float(eps)]
+    for i, out in enumerate(made):
+        args += [out.data_ptr(), *out.stride()[:2]]
+        if branch is None:
+            args.insert(-2, _STREAM_DTYPES[dtype])
+    _call_on(device, name, *args)
+    return tuple(made)
+
+
+def norm_modulate(x: torch.Tensor, scale: torch.Tensor | None = None,
+                  shift: torch.Tensor | None = None, *, norm: str = "layer",
+                  weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                  eps: float = 1e-6, dtype: torch.dtype | None = None,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """``norm(x) * (1 + scale) + shift`` of a residual stream ``[B, N, width]``: the norm before a
+    block.  ``norm`` is ``"layer"`` or ``"rms"`` over the width, with an optional ``weight`` and
+    ``bias``.  ``scale`` and ``shift`` are ``[width]``, ``[B or 1, width]`` or ``[B or 1, N or 1,
+    width]``.  ``dtype`` is the output's: x's own, or any for an fp32 stream.  ``out`` may be x
+    itself where the types agree."""
+    if norm is None:
+        raise ValueError("norm must be 'layer' or 'rms'")
+    dtype = dtype or x.dtype
+    kind = _choice(_NORMS, norm, "norm")
+    return _residual_call("recap_norm_modulate", x, dtype, mods={"scale": scale, "shift": shift},
+                          norms=[(kind, "", weight, bias)], eps=eps,
+                          outs=[("out", out, dtype, "x")])[0]
+
+
+def gated_residual(x: torch.Tensor, branch: torch.Tensor, gate: torch.Tensor | None = None, *,
+                   branch_norm: str | None = None, branch_weight: torch.Tensor | None = None,
+                   branch_bias: torch.Tensor | None = None, eps: float = 1e-6,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """``x + gate * branch_norm(branch)``: a block's output added to the residual stream
+    ``[B, N, width]`` (of the branch's type or fp32), after an optional norm of its own.  ``gate``
+    has the shapes of norm_modulate's ``scale``; None adds the branch as it is.  ``out`` may be x
+    itself."""
+    kind = _choice(_NORMS, branch_norm, "branch_norm")
+    return _residual_call("recap_gated_residual", x, branch.dtype, branch=branch,
+                          mods={"gate": gate}, norms=[(kind, "branch_", branch_weight, branch_bias)],
+                          eps=eps, outs=[("out", out, x.dtype, "x")])[0]
+
+
+def gated_residual_norm(x: torch.Tensor, branch: torch.Tensor, gate: torch.Tensor | None = None,
+                        scale: torch.Tensor | None = None, shift: torch.Tensor | None = None, *,
+                        norm: str = "layer", weight: torch.Tensor | None = None,
+                        bias: torch.Tensor | None = None, branch_norm: str | None = None,
+                        branch_weight: torch.Tensor | None = None,
+                        branch_bias: torch.Tensor | None = None, eps: float = 1e-6,
+                        out: torch.Tensor | None = None, norm_out: torch.Tensor | None = None):
+    """A block's end and the next one's start in one pass over the residual stream:
+    ``r = x + gate * branch_norm(branch)`` and ``norm(r) * (1 + scale) + shift``, as (r, y).  Arguments
+    as in gated_residual and norm_modulate; y has the branch's type and is taken from r before
+    its rounding.  ``out`` (of r) may be x itself and ``norm_out`` (of y) branch itself."""
+    if norm is None:
+        raise ValueError("norm must be 'layer' or 'rms'")
+    kinds = _choice(_NORMS, branch_norm, "branch_norm"), _choice(_NORMS, norm, "norm")
+    return _residual_call("recap_gated_residual_norm", x, branch.dtype, branch=branch,
+                          mods={"gate": gate, "scale": scale, "shift": shift},
+                          norms=[(kinds[0], "branch_", branch_weight, branch_bias),
+                                 (kinds[1], "", weight, bias)], eps=eps,
+                          outs=[("out", out, x.dtype, "x"),
+                                ("norm_out", norm_out, branch.dtype, "branch")])
+
+
 def bank_copy_async(dst: torch.Tensor, src: torch.Tensor, stream=None) -> None:
     """Asynchronous device <-> pinned-host copy of a whole bank tensor on ``stream``."""
     if dst.numel() * dst.element_size() != src.numel() * src.element_size():

@@ -1,0 +1,104 @@
+"""AttentionBlock on the GPU: the whole attention half of a block, refresh then sparse steps,
+against its parts one by one (bit for bit) and against 64 bits around the oracle's attention."""
+
+import pytest
+import torch
+
+import oracle as O
+import recap_amd
+from around_util import qk, residual
+from gpu_util import SMALL, metrics
+from recap_amd import EXACT, REFRESH, SPARSE, OperatorConfig, kernels as K
+from recap_amd.layout import Layout, SparseGeometry, hilbert_permutation
+
+pytestmark = pytest.mark.gpu
+
+CHANNELS = {64: (16, 24, 24), 128: (44, 42, 42)}
+
+
+def build(wl, cuda, qk_norm, stream, batch, width=320, seed=0):
+    perm = hilbert_permutation(wl.grid)
+    layout = Layout.from_permutation(perm, text_tokens=wl.text_tokens, text_first=wl.text_first)
+    op = recap_amd.Operator.build(OperatorConfig(head_density=wl.density),
+                                  SparseGeometry.build(layout, 128), n_layers=1)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    inner, dtype = wl.heads * wl.dim, wl.dtype
+    w = {n: (rand(*s) * s[1] ** -0.5).to(dtype) for n, s in
+         (("q", (inner, width)), ("k", (inner, width)), ("v", (inner, width)), ("o", (width, inner)))}
+    linear = {n: (lambda y, m=m: y @ m.T) for n, m in w.items()}
+    extent = inner if qk_norm == "rms_all" else wl.dim
+    block = recap_amd.AttentionBlock(
+        op, 0, wl.heads, linear["q"], linear["k"], linear["v"], linear["o"],
+        axes=recap_amd.rotary_axes(wl.grid, CHANNELS[wl.dim], device=cuda), qk_norm=qk_norm,
+        q_weight=(1 + 0.2 * rand(extent)).to(dtype), k_weight=(1 + 0.2 * rand(extent)).to(dtype),
+        branch_norm="rms", branch_weight=(1 + 0.2 * rand(width)).to(dtype), next_norm="rms", dtype=dtype)
+    emb = 0.3 * rand(batch, 5, width)
+    steps = [rand(batch, wl.tokens, width)]
+    for _ in range(2):
+        steps.append(steps[-1] + 0.02 * rand(batch, wl.tokens, width))
+    return block, w, [emb[:, i:i + 1] for i in range(5)], [s.to(stream) for s in steps], perm
+
+
+@pytest.mark.parametrize("name,qk_norm,stream,batch", [
+    ("text-last-d128", "rms", torch.bfloat16, 1), ("text-first-ragged", "layer", torch.float32, 2),
+    ("video-ragged-d128", "rms_all", torch.float32, 1)])
+def test_block_steps(cuda, name, qk_norm, stream, batch):
+    wl = SMALL[name]
+    block, w, mods, steps, perm = build(wl, cuda, qk_norm, stream, batch)
+    op = block.operator
+    ref = recap_amd.Operator.build(op.config, op.layers[0][0].geometry, n_layers=1)
+    oracle = O.OracleOperator(wl.grid, wl.text_tokens, wl.text_first, wl.density, permutation=perm)
+    scale, shift, gate, scale2, shift2 = mods
+    for step, (x, kind) in enumerate(zip(steps, (REFRESH, SPARSE, SPARSE))):
+        print(f"case {name} {qk_norm} step {step} {kind}", flush=True)
+        op.begin_step(step, kind)
+        ref.begin_step(step, kind)
+        r, y = block(x, scale, shift, gate, scale2, shift2)
+        # its parts, one by one
+        h = K.norm_modulate(x, scale, shift, dtype=wl.dtype)
+        q, k, v = ((h @ w[n].T).unflatten(2, (wl.heads, wl.dim)).transpose(1, 2) for n in "qkv")
+        qr, kr = K.qk_rotary(q, k, block.axes, offset=op.layout.video_offset, norm=qk_norm,
+                             q_weight=block.q_weight, k_weight=block.k_weight)
+        out = ref.attend(0, qr, kr, v)
+        branch = out.transpose(1, 2).flatten(2) @ w["o"].T
+        parts = K.gated_residual_norm(x, branch, gate, scale2, shift2, norm="rms",
+                                      branch_norm="rms", branch_weight=block.branch_weight)
+        assert torch.equal(r, parts[0]) and torch.equal(y, parts[1])
+        # the definitions in 64 bits around the oracle's attention, each part on its own inputs'
+        # rounding: queries and keys rounded once as the kernels take them
+        exact_q, exact_k = (qk(t, block.axes, offset=op.layout.video_offset, kind=qk_norm,
+                               weight=wt)[0].to(wl.dtype)
+                            for t, wt in ((q, block.q_weight), (k, block.k_weight)))
+        args = (0, exact_q.cpu(), exact_k.cpu(), v.cpu())
+        want = (oracle.refresh if kind == REFRESH else oracle.sparse)(*args).to(wl.dtype).to(cuda)
+        branch = want.transpose(1, 2).flatten(2) @ w["o"].T
+        (er, _), (ey, _) = residual(x, branch, gate, scale2, shift2, kind="rms", post="rms",
+                                    branch_weight=block.branch_weight)
+        for label, got, exact in (("residual", r, er), ("normed", y, ey)):
+            _, cos = metrics(got, exact)
+            assert cos >= 0.999, (label, cos)
+
+
+def test_block_exact_step_and_text_length(cuda):
+    """An EXACT step, and a per-prompt text length that moves the video's first token."""
+    wl = SMALL["text-first-ragged"]
+    block, w, mods, steps, _ = build(wl, cuda, "rms", torch.bfloat16, 1)
+    op = block.operator
+    op.begin_step(0, EXACT)
+    x = steps[0]
+    long = block(x, *mods)
+    op.layout.text_tokens -= 100   # the prompt lost its first 100 tokens
+    op.layout._gather_cache.clear()
+    q = torch.randn(1, wl.heads, wl.tokens - 100, wl.dim, device=cuda).to(wl.dtype)
+    h = K.norm_modulate(x[:, 100:], mods[0], mods[1], dtype=wl.dtype)
+    seen = {}
+    attend = op.attend
+    op.attend = lambda layer, query, key, value: seen.update(q=query) or attend(layer, query, key, value)
+    short = block(x[:, 100:], *mods)
+    q = (h @ w["q"].T).unflatten(2, (wl.heads, wl.dim)).transpose(1, 2)
+    want = K.qk_rotary(q, None, block.axes, offset=wl.text_tokens - 100, norm="rms",
+                       q_weight=block.q_weight)[0]
+    assert torch.equal(seen["q"], want)
+    assert short[0].shape[1] == wl.tokens - 100 and torch.isfinite(short[1]).all()
+    assert torch.isfinite(long[1]).all()
