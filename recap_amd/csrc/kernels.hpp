@@ -189,6 +189,7 @@ struct RotaryTensor {
   const uint16_t* in; int64_t in_b, in_h, in_n;
   uint16_t* out; int64_t out_b, out_h, out_n;
   const void* weight; const void* bias; int heads;
+  int side = 1;                                  // heads a wave takes at once, chosen at launch
 };
 struct RotaryArgs {
   RotaryTensor x[2]; int tensors;                // q, then k

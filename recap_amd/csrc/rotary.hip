@@ -5,110 +5,212 @@
 //   that axis's table at the token's position on it;
 //   its channels (p, q), 2i and 2i + 1 or i and i + d/2, become (p c - q s, q c + p s).
 // Statistics and products are fp32, rounded once.
+//
+// A lane holds 16 channels of a (token, head) row in two 16-byte chunks, u and u + d/16, so
+// that both pairings stay within the lane; d/16 lanes hold the row.  A wave takes `side` heads
+// of each of its tokens at once (side a power of two that divides the heads) and walks the
+// others, so a token's (cos, sin) are looked up once per wave.
+#include <algorithm>
+
 #include "kernels.hpp"
+#include "rows.hpp"
 
 namespace recap {
 namespace {
 
-constexpr int kWaves = 4;
+constexpr int kThreads = 256;
+constexpr int kBatch = 4;  // head rows in flight per lane
 
-// One workgroup per token of q or k, one wave per head in turn, one lane per pair.
-template <class T, int D>
-__global__ __launch_bounds__(64 * kWaves) void rotary_kernel(RotaryArgs a) {
-  constexpr int kPairs = D / 2;
-  __shared__ float part[kWaves];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int which = blockIdx.y;
-  const RotaryTensor& t = a.x[which];
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const int64_t b = row / a.tokens, n = row - b * a.tokens;
-    const int64_t v = n - a.offset;
-    const bool video = v >= 0 && v < a.video, live = lane < kPairs;
-    float c = 1.0f, s = 0.0f;
-    if (video && live) {
-      const int64_t plane = (int64_t)a.axis[1].length * a.axis[2].length;
-      const int64_t pos[3] = {v / plane, v / a.axis[2].length % a.axis[1].length,
-                              v % a.axis[2].length};
-      int first = 0;
-      for (int i = 0; i < 3; ++i) {
-        const int pairs = a.axis[i].pairs;
-        if (lane >= first && lane < first + pairs) {
-          const float* e = a.axis[i].table + 2 * (pos[i] * pairs + lane - first);
-          c = e[0];
-          s = e[1];
+template <class T>
+__device__ inline void load16(const void* p, bool wide, int64_t i, int half, float (&v)[16]) {
+  float lo[8], hi[8];
+  load8_either<T>(p, wide, i, lo);
+  load8_either<T>(p, wide, i + half, hi);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    v[e] = lo[e];
+    v[8 + e] = hi[e];
+  }
+}
+
+template <class T, int D, bool HALVES, int NORM>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
+  constexpr int kLanes = D / 16, kRows = 64 / kLanes;
+  const RotaryTensor& t = a.x[blockIdx.y];
+  const int side = t.side;
+  const int lane = threadIdx.x & 63, u = lane & (kLanes - 1), g = lane / kLanes;
+  const int hl = g & (side - 1), tokens = kRows / side, tl = g / side;
+  const int64_t wave = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  if (wave * tokens >= a.rows) return;  // q and k need not take the same number of waves
+  const int64_t row = wave * tokens + tl;
+  const bool live = row < a.rows;
+  const unsigned r32 = (unsigned)(live ? row : a.rows - 1);
+  const unsigned b = r32 / (unsigned)a.tokens, n = r32 - b * (unsigned)a.tokens;
+
+  // (cos, sin) of the lane's 8 frequencies; identity outside the video.
+  float c[8], s[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    c[e] = 1.0f;
+    s[e] = 0.0f;
+  }
+  const int64_t v64 = (int64_t)n - a.offset;
+  if (v64 >= 0 && v64 < a.video) {
+    const unsigned v = (unsigned)v64, wd = a.axis[2].length, ht = a.axis[1].length;
+    const unsigned line = v / wd, x = v - line * wd, z = line / ht, y = line - z * ht;
+    const int p0 = a.axis[0].pairs, p1 = p0 + a.axis[1].pairs;
+    const float* t0 = a.axis[0].table + (int64_t)z * (2 * a.axis[0].pairs);
+    const float* t1 = a.axis[1].table + ((int64_t)y * a.axis[1].pairs - p0) * 2;
+    const float* t2 = a.axis[2].table + ((int64_t)x * a.axis[2].pairs - p1) * 2;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int i = HALVES ? 8 * u + e : (e < 4 ? 4 * u + e : D / 4 + 4 * u + e - 4);
+      const float* q = i < p0 ? t0 : i < p1 ? t1 : t2;
+      const float2 cs = *reinterpret_cast<const float2*>(q + 2 * i);
+      c[e] = cs.x;
+      s[e] = cs.y;
+    }
+  }
+
+  float w[16], bias[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    w[e] = 1.0f;
+    bias[e] = 0.0f;
+  }
+  if (NORM == kRotaryRms || NORM == kRotaryLayer) {
+    if (t.weight) load16<T>(t.weight, a.wide_weight, 8 * u, D / 2, w);
+    if (t.bias) load16<T>(t.bias, a.wide_weight, 8 * u, D / 2, bias);
+  }
+
+  const uint16_t* src = t.in + b * t.in_b + n * t.in_n + hl * t.in_h + 8 * u;
+  uint16_t* dst = t.out + b * t.out_b + n * t.out_n + hl * t.out_h + 8 * u;
+  const int steps = t.heads / side;
+  u32x4 raw[kBatch][2];
+  const auto fetch = [&](int first) {
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (first + j < steps) {
+        const uint16_t* p = src + (int64_t)(first + j) * side * t.in_h;
+        raw[j][0] = *reinterpret_cast<const u32x4*>(p);
+        raw[j][1] = *reinterpret_cast<const u32x4*>(p + D / 2);
+      }
+  };
+  const auto widen = [&](int j, float (&x)[16]) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[8 * k + 2 * e] = T::to_f((uint16_t)raw[j][k][e]);
+        x[8 * k + 2 * e + 1] = T::to_f((uint16_t)(raw[j][k][e] >> 16));
+      }
+  };
+  float all = 1.0f;
+  if (NORM == kRotaryRmsAll) {
+    float sq = 0.0f;
+    for (int first = 0; first < steps; first += kBatch) {
+      fetch(first);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (first + j < steps) {
+          float x[16];
+          widen(j, x);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sq = fmaf(x[e], x[e], sq);
         }
-        first += pairs;
-      }
     }
-    const int i0 = a.halves ? lane : 2 * lane, i1 = a.halves ? lane + kPairs : 2 * lane + 1;
-    const uint16_t* src = t.in + b * t.in_b + n * t.in_n;
-    uint16_t* dst = t.out + b * t.out_b + n * t.out_n;
-    const auto load = [&](int h, float& p, float& q) {
-      p = live ? T::to_f(src[h * t.in_h + i0]) : 0.0f;
-      q = live ? T::to_f(src[h * t.in_h + i1]) : 0.0f;
-    };
-    float inv = 1.0f;
-    if (a.norm == kRotaryRmsAll) {
-      float sq = 0.0f, p, q;
-      for (int h = wave; h < t.heads; h += kWaves) {
-        load(h, p, q);
-        sq += p * p + q * q;
+    all = 1.0f / sqrtf(row_sum(sq, kLanes * side, nullptr) / (float)(t.heads * D) + a.eps);
+  }
+  for (int first = 0; first < steps; first += kBatch) {
+    if (NORM != kRotaryRmsAll || steps > kBatch) fetch(first);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (first + j >= steps) break;
+      float x[16], y[16];
+      widen(j, x);
+      float inv = all;
+      if (NORM == kRotaryLayer) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum += x[e];
+        const float mean = row_sum(sum, kLanes, nullptr) * (1.0f / D);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] -= mean;
       }
-      sq = wave_sum(sq);
-      __syncthreads();
-      if (lane == 0) part[wave] = sq;
-      __syncthreads();
-      sq = 0.0f;
-      for (int w = 0; w < kWaves; ++w) sq += part[w];
-      inv = 1.0f / sqrtf(sq / (float)(t.heads * D) + a.eps);
-    }
-    for (int h = wave; h < t.heads; h += kWaves) {
-      float p, q;
-      load(h, p, q);
-      if (a.norm == kRotaryLayer) {
-        const float mean = wave_sum(p + q) / (float)D;
-        p = live ? p - mean : 0.0f;
-        q = live ? q - mean : 0.0f;
+      if (NORM == kRotaryRms || NORM == kRotaryLayer) {
+        float sq = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sq = fmaf(x[e], x[e], sq);
+        inv = 1.0f / sqrtf(row_sum(sq, kLanes, nullptr) * (1.0f / D) + a.eps);
       }
-      if (a.norm == kRotaryRms || a.norm == kRotaryLayer)
-        inv = 1.0f / sqrtf(wave_sum(p * p + q * q) / (float)D + a.eps);
-      p *= inv;
-      q *= inv;
-      if (!live) continue;
-      const int w = a.norm == kRotaryRmsAll ? h * D : 0;
-      if (t.weight) {
-        p *= a.wide_weight ? ((const float*)t.weight)[w + i0]
-                           : T::to_f(((const uint16_t*)t.weight)[w + i0]);
-        q *= a.wide_weight ? ((const float*)t.weight)[w + i1]
-                           : T::to_f(((const uint16_t*)t.weight)[w + i1]);
+      if (NORM == kRotaryRmsAll) {
+        const int64_t at = (int64_t)((first + j) * side + hl) * D + 8 * u;
+        if (t.weight) load16<T>(t.weight, a.wide_weight, at, D / 2, w);
+        if (t.bias) load16<T>(t.bias, a.wide_weight, at, D / 2, bias);
       }
-      if (t.bias) {
-        p += a.wide_weight ? ((const float*)t.bias)[w + i0]
-                           : T::to_f(((const uint16_t*)t.bias)[w + i0]);
-        q += a.wide_weight ? ((const float*)t.bias)[w + i1]
-                           : T::to_f(((const uint16_t*)t.bias)[w + i1]);
+      if (NORM != kRotaryNone) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = fmaf(x[e] * inv, w[e], bias[e]);
       }
-      dst[h * t.out_h + i0] = T::from_f(p * c - q * s);
-      dst[h * t.out_h + i1] = T::from_f(q * c + p * s);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int p = HALVES ? e : 2 * e, q = HALVES ? e + 8 : 2 * e + 1;
+        y[p] = x[p] * c[e] - x[q] * s[e];
+        y[q] = x[q] * c[e] + x[p] * s[e];
+      }
+      u32x4 lo, hi;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        lo[e] = pack2<T>(y[2 * e], y[2 * e + 1]);
+        hi[e] = pack2<T>(y[8 + 2 * e], y[8 + 2 * e + 1]);
+      }
+      if (live) {
+        uint16_t* o = dst + (int64_t)(first + j) * side * t.out_h;
+        *reinterpret_cast<u32x4*>(o) = lo;
+        *reinterpret_cast<u32x4*>(o + D / 2) = hi;
+      }
     }
   }
 }
 
-template <class T>
-hipError_t launch(const RotaryArgs& a, int dim, hipStream_t s) {
-  const dim3 grid((unsigned)(a.rows < (1 << 20) ? a.rows : (1 << 20)), a.tensors);
-  if (dim == 128) {
-    rotary_kernel<T, 128><<<grid, dim3(64 * kWaves), 0, s>>>(a);
-  } else {
-    rotary_kernel<T, 64><<<grid, dim3(64 * kWaves), 0, s>>>(a);
+template <class T, int D, bool HALVES, int NORM>
+hipError_t launch(const RotaryArgs& a, hipStream_t s) {
+  constexpr int kRows = 64 / (D / 16);
+  RotaryArgs b = a;
+  int64_t waves = 1;
+  for (int i = 0; i < a.tensors; ++i) {
+    // Each tensor by its own heads, so that q's sums do not depend on k's.
+    int side = 1;
+    while (side < kRows && a.x[i].heads % (2 * side) == 0) side *= 2;
+    b.x[i].side = side;
+    waves = std::max(waves, (a.rows + kRows / side - 1) / (kRows / side));
   }
+  constexpr int kWaves = kThreads / 64;
+  const dim3 grid((unsigned)((waves + kWaves - 1) / kWaves), a.tensors);
+  rotary_kernel<T, D, HALVES, NORM><<<grid, dim3(kThreads), 0, s>>>(b);
   return hipGetLastError();
+}
+
+template <class T, int D, bool HALVES>
+hipError_t by_norm(const RotaryArgs& a, hipStream_t s) {
+  switch (a.norm) {
+    case kRotaryNone: return launch<T, D, HALVES, kRotaryNone>(a, s);
+    case kRotaryRms: return launch<T, D, HALVES, kRotaryRms>(a, s);
+    case kRotaryLayer: return launch<T, D, HALVES, kRotaryLayer>(a, s);
+    default: return launch<T, D, HALVES, kRotaryRmsAll>(a, s);
+  }
+}
+
+template <class T>
+hipError_t by_shape(const RotaryArgs& a, int dim, hipStream_t s) {
+  if (dim == 128) return a.halves ? by_norm<T, 128, true>(a, s) : by_norm<T, 128, false>(a, s);
+  return a.halves ? by_norm<T, 64, true>(a, s) : by_norm<T, 64, false>(a, s);
 }
 
 }  // namespace
 
 hipError_t run_rotary(const RotaryArgs& a, int dtype, int dim, hipStream_t s) {
-  return dtype == BF16::code ? launch<BF16>(a, dim, s) : launch<F16>(a, dim, s);
+  return dtype == BF16::code ? by_shape<BF16>(a, dim, s) : by_shape<F16>(a, dim, s);
 }
 
 }  // namespace recap
