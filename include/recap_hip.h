@@ -455,22 +455,22 @@ int recap_bank_copy_async(void* dst, const void* src, int64_t bytes, void* strea
  *    RECAP_NORM_RMS_ALL over the heads * dim channels of a token (weight, bias
  *    [heads * dim], head by head), RECAP_NORM_NONE for none.  Weights and biases may be NULL;
  *    weight_dtype is the tensors' type or RECAP_F32.
- *  - axis_tables[i] (fp32 [lengths[i], pairs[i], 2], device memory, 8-byte aligned): the
- *    (cos, sin) of axis i (time, height, width) at each position; pairs[0] + pairs[1] +
- *    pairs[2] = dim / 2, and an axis of no pairs may have a NULL table.  Token offset + v with
+ *  - table_t, table_h, table_w (fp32 [lengths[i], pairs[i], 2], device memory, 8-byte
+ *    aligned): the (cos, sin) of axis i (time, height, width) at each position; pairs[0] +
+ *    pairs[1] + pairs[2] = dim / 2, and an axis of no pairs may have a NULL table.  Token offset + v with
  *    0 <= v < lengths[0] * lengths[1] * lengths[2] sits at (v / (H * W), v / W % H, v % W);
  *    the other tokens (text) are not rotated.  Frequency i rotates channels (2i, 2i + 1)
- *    (RECAP_PAIRS_INTERLEAVED) or (i, i + dim / 2) (RECAP_PAIRS_HALVES).  axis_tables NULL: no
- *    rotation.
+ *    (RECAP_PAIRS_INTERLEAVED) or (i, i + dim / 2) (RECAP_PAIRS_HALVES).  lengths and pairs (host arrays
+ *    of 3) NULL: no rotation.
  *  - k may be NULL.  An output may be its own input, and overlaps nothing else.
  * No weights, sums or angles are kept from call to call.  Covers the query/key norm and the rotary embedding
  * before operator.attend in the model processors, recap/models/hunyuan.py:79-154. */
 int recap_qk_rotary(const void* q, const void* k, int dtype, int64_t batch, int64_t tokens,
                     int64_t dim, int64_t q_heads, int64_t k_heads, int64_t q_stride_b,
                     int64_t q_stride_h, int64_t q_stride_n, int64_t k_stride_b,
-                    int64_t k_stride_h, int64_t k_stride_n, const float* const* axis_tables,
-                    const int64_t* lengths, const int64_t* pairs, int64_t offset, int pairing,
-                    int norm, const void* q_weight, const void* q_bias, const void* k_weight,
+                    int64_t k_stride_h, int64_t k_stride_n, const float* table_t,
+                    const float* table_h, const float* table_w, const int64_t* lengths,
+                    const int64_t* pairs, int64_t offset, int pairing, int norm, const void* q_weight, const void* q_bias, const void* k_weight,
                     const void* k_bias, int weight_dtype, float eps, void* q_out,
                     int64_t qo_stride_b, int64_t qo_stride_h, int64_t qo_stride_n, void* k_out,
                     int64_t ko_stride_b, int64_t ko_stride_h, int64_t ko_stride_n, void* stream);

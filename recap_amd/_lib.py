@@ -99,8 +99,8 @@ SIGNATURES: dict[str, tuple] = {
     "recap_pager_copy_time": (_I, [_P, _P, _P]),
     "recap_pager_resize": (_I, [_P, _P, ctypes.c_int32]),
     "recap_bank_copy_async": (_I, [_P, _P, _I64, _P]),
-    "recap_qk_rotary": (_I, [_P, _P, _I, *([_I64] * 5), *_STRIDES, *_STRIDES, _P, _P, _P, _I64, _I,
-                             _I, _P, _P, _P, _P, _I, _F, _P, *_STRIDES, _P, *_STRIDES, _P]),
+    "recap_qk_rotary": (_I, [_P, _P, _I, *([_I64] * 5), *_STRIDES, *_STRIDES, _P, _P, _P, _P, _P,
+                             _I64, _I, _I, _P, _P, _P, _P, _I, _F, _P, *_STRIDES, _P, *_STRIDES, _P]),
     "recap_norm_modulate": (_I, [_P, _I, _I64, _I64, _I64, _I64, _I64, *_ROWS, *_ROWS, _I, _P, _P,
                                  _I, _I, _F, _P, _I, _I64, _I64, _P]),
     "recap_gated_residual": (_I, [_P, _I, _I64, _I64, _I64, _I64, _I64, _P, _I, _I64, _I64, *_ROWS,

@@ -1067,9 +1067,9 @@ int recap_bank_copy_async(void* dst, const void* src, int64_t bytes, void* strea
 int recap_qk_rotary(const void* q, const void* k, int dtype, int64_t batch, int64_t tokens,
                     int64_t dim, int64_t q_heads, int64_t k_heads, int64_t q_stride_b,
                     int64_t q_stride_h, int64_t q_stride_n, int64_t k_stride_b,
-                    int64_t k_stride_h, int64_t k_stride_n, const float* const* axis_tables,
-                    const int64_t* lengths, const int64_t* pairs, int64_t offset, int pairing,
-                    int norm, const void* q_weight, const void* q_bias, const void* k_weight,
+                    int64_t k_stride_h, int64_t k_stride_n, const float* table_t,
+                    const float* table_h, const float* table_w, const int64_t* lengths,
+                    const int64_t* pairs, int64_t offset, int pairing, int norm, const void* q_weight, const void* q_bias, const void* k_weight,
                     const void* k_bias, int weight_dtype, float eps, void* q_out,
                     int64_t qo_stride_b, int64_t qo_stride_h, int64_t qo_stride_n, void* k_out,
                     int64_t ko_stride_b, int64_t ko_stride_h, int64_t ko_stride_n,
@@ -1109,8 +1109,9 @@ int recap_qk_rotary(const void* q, const void* k, int dtype, int64_t batch, int6
   const uintptr_t weight_align = weight_dtype == RECAP_F32 ? 3 : 1;
   for (const void* w : {q_weight, q_bias, k_weight, k_bias})
     REQUIRE((reinterpret_cast<uintptr_t>(w) & weight_align) == 0, "a weight is misaligned");
-  if (axis_tables != nullptr) {
-    REQUIRE(lengths && pairs, "lengths and pairs must be non-NULL");
+  REQUIRE((lengths == nullptr) == (pairs == nullptr), "lengths and pairs go together");
+  if (lengths != nullptr) {
+    const float* const axis_tables[3] = {table_t, table_h, table_w};
     int64_t total = 0, video = 1;
     for (int i = 0; i < 3; ++i) {
       REQUIRE(lengths[i] >= 1 && lengths[i] <= tokens, "axis %d: length %lld outside 1..tokens", i,

@@ -641,18 +641,26 @@ def _choice(table: dict, value, what: str) -> int:
     return table[value]
 
 
-def _together(tensors: dict[str, torch.Tensor | None]) -> torch.device:
+def _spec(t: torch.Tensor | None):
+    """What a call's checks look at of a tensor, hashable: everything but its address."""
+    if t is None:
+        return None
+    return (t.shape, t.stride(), t.dtype, t.device,
+            t.requires_grad and torch.is_grad_enabled())
+
+
+def _together(specs: dict) -> torch.device:
     """The GPU that all tensors of a call are on.  The kernels have no backward pass, so a
     call that would have to record one is refused."""
-    device = next(iter(tensors.values())).device
-    for name, t in tensors.items():
-        if t is None:
+    device = next(iter(specs.values()))[3]
+    for name, spec in specs.items():
+        if spec is None:
             continue
-        if not t.is_cuda:
+        if spec[3].type != "cuda":
             raise ValueError(f"{name} must be a GPU tensor")
-        if t.device != device:
-            raise ValueError(f"{name} is on {t.device}, the call on {device}")
-        if t.requires_grad and torch.is_grad_enabled():
+        if spec[3] != device:
+            raise ValueError(f"{name} is on {spec[3]}, the call on {device}")
+        if spec[4]:
             raise ValueError(f"{name} requires a gradient, which this call does not record: run it "
                              "under torch.no_grad()")
     return device
@@ -660,11 +668,12 @@ def _together(tensors: dict[str, torch.Tensor | None]) -> torch.device:
 
 def _call_on(device: torch.device, name: str, *args) -> None:
     """Call on the current stream of `device`, which need not be the current device."""
-    if torch.cuda.current_device() == device.index:
-        call(name, *args, _stream())
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            call(name, *args, _stream())
+            call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
@@ -718,18 +727,106 @@ def _check_output(name: str, out: torch.Tensor, shape, dtype: torch.dtype,
             raise ValueError(f"{name} overlaps the memory of {other}")
 
 
-def _qk_weights(kind: int, extent: int, dtype: torch.dtype, vectors: dict) -> int:
-    """Type code of the weights and biases of a norm over `extent` channels."""
-    given = {name: v for name, v in vectors.items() if v is not None}
+def _weights(kind: int, extent: int, dtype: torch.dtype, specs: dict) -> set:
+    """Types of the given weights and biases of a norm over `extent` channels."""
+    given = {name: v for name, v in specs.items() if v is not None}
     if given and kind == _lib.NORM_NONE:
         raise ValueError(f"{next(iter(given))} needs a norm")
-    types = {v.dtype for v in given.values()} or {dtype}
-    if len(types) > 1 or not types <= {dtype, torch.float32}:
-        raise ValueError(f"weights and biases must all be {dtype} or all torch.float32")
-    for name, v in given.items():
-        if tuple(v.shape) != (extent,):
-            raise ValueError(f"{name} is {tuple(v.shape)}, expected ({extent},)")
-    return _STREAM_DTYPES[types.pop()]
+    for name, (shape, _, got, _, _) in given.items():
+        if got not in (dtype, torch.float32):
+            raise ValueError(f"{name} is {got}; weights and biases are {dtype} or torch.float32")
+        if tuple(shape) != (extent,):
+            raise ValueError(f"{name} is {tuple(shape)}, expected ({extent},)")
+    return {v[2] for v in given.values()}
+
+
+def _one_type(types: set, dtype: torch.dtype, what: str) -> int:
+    if len(types) > 1:
+        raise ValueError(f"{what} must have one type, got {sorted(map(str, types))}")
+    return _STREAM_DTYPES[next(iter(types), dtype)]
+
+
+@dataclass(frozen=True)
+class _QKPlan:
+    """What a qk_rotary call of given shapes, strides and types passes besides addresses."""
+
+    device: torch.device
+    copies: bool      # some input is first laid out as the kernel reads it
+    empty: bool
+    sizes: tuple      # dtype, batch, tokens, dim, heads of q and of k
+    lengths: object   # int64 [3], or None without axes
+    pairs: object
+    codes: tuple      # pairing, norm
+    weight_code: int
+    strides: tuple    # of q and k, and of outputs made here
+    out_strides: tuple
+
+
+def _aligned_rows(spec) -> bool:
+    shape, strides = spec[:2]
+    return strides[-1] == 1 and not any(s % 8 for s, n in zip(strides[:3], shape) if n > 1)
+
+
+def _row_strides(shape, strides) -> tuple:
+    """Batch, head and token strides; of a dimension of one, whose stride means nothing, d."""
+    return tuple(s if n > 1 else shape[3] for s, n in zip(strides[:3], shape))
+
+
+@functools.lru_cache(maxsize=1024)
+def _qk_plan(q, k, axes, offset: int, pairing: str, norm, vectors) -> _QKPlan:
+    """Checks of a qk_rotary call, from its tensors' specs."""
+    kind = _choice(_QK_NORMS, norm, "norm")
+    pairs = _choice(_PAIRINGS, pairing, "pairing")
+    for name, spec in (("q", q), ("k", k)):
+        if spec is None:
+            continue
+        if len(spec[0]) != 4:
+            raise ValueError(f"{name} must be [batch, heads, tokens, dim], got {tuple(spec[0])}")
+        dtype_code(spec[2])
+        if spec[0][3] not in (64, 128):
+            raise ValueError(f"{name}: head dim {spec[0][3]} unsupported (64 or 128)")
+    b, h, n, d = q[0]
+    dtype = q[2]
+    if k is not None and (k[2] != dtype or k[0][0] != b or k[0][2:] != q[0][2:]):
+        raise ValueError(f"K {tuple(k[0])} {k[2]} does not match Q {tuple(q[0])} {dtype}")
+    if k is None and not vectors[2] is vectors[3] is None:
+        raise ValueError("k_weight and k_bias need a k")
+    heads_k = 0 if k is None else k[0][1]
+    named = dict(zip(("q_weight", "q_bias", "k_weight", "k_bias"), vectors))
+    types = set()
+    for heads, prefix in ((h, "q_"), (heads_k, "k_")):
+        types |= _weights(kind, heads * d if kind == _lib.NORM_RMS_ALL else d, dtype,
+                          {key: v for key, v in named.items() if key.startswith(prefix)})
+    weight_code = _one_type(types, dtype, "weights and biases")
+    lengths = counts = None
+    if axes is not None:
+        if len(axes) != 3:
+            raise ValueError(f"axes must be three tables (time, height, width), got {len(axes)}")
+        for i, (shape, _, got, _, _) in enumerate(axes):
+            if len(shape) != 3 or shape[2] != 2 or got != torch.float32 or shape[0] < 1:
+                raise ValueError(f"axis {i} must be fp32 [length, channels / 2, 2], got "
+                                 f"{tuple(shape)} {got}")
+        if sum(t[0][1] for t in axes) != d // 2:
+            raise ValueError(f"the axes rotate {[2 * t[0][1] for t in axes]} channels, the heads "
+                             f"have {d}")
+        video = math.prod(t[0][0] for t in axes)
+        if not 0 <= offset <= n - video:
+            raise ValueError(f"tokens {offset}..{offset + video - 1} are not all in the sequence "
+                             f"of {n}")
+        lengths = (ctypes.c_int64 * 3)(*(t[0][0] for t in axes))
+        counts = (ctypes.c_int64 * 3)(*(t[0][1] for t in axes))
+    tables = axes or ()
+    device = _together({"q": q, "k": k, **named, **{f"axis {i}": t for i, t in enumerate(tables)}})
+    empty = b * h * n == 0
+    if k is not None and empty != (b * heads_k * n == 0):
+        raise ValueError("q and k must both have heads")
+    copies = not all(_aligned_rows(t) for t in (q, k) if t is not None) or any(
+        t[1][0] != 1 and t[0][0] > 1 for t in vectors if t is not None) or any(
+        t[1][1:] != (2, 1) or t[1][0] != 2 * t[0][1] for t in tables if t[0][1] > 0)
+    return _QKPlan(device, copies, empty, (dtype_code(dtype), b, n, d, h, heads_k), lengths, counts,
+                   (pairs, kind), weight_code,
+                   tuple((0, 0, 0) if t is None else _row_strides(*t[:2]) for t in (q, k)),
+                   tuple((0, 0, 0) if t is None else (t[0][1] * n * d, n * d, d) for t in (q, k)))
 
 
 def qk_rotary(q: torch.Tensor, k: torch.Tensor | None = None, axes=None, *, offset: int = 0,
@@ -751,168 +848,153 @@ def qk_rotary(q: torch.Tensor, k: torch.Tensor | None = None, axes=None, *, offs
 
     ``q_out`` and ``k_out`` may be ``q`` and ``k`` themselves, or views into a longer sequence
     (a text stream's part of it)."""
-    kind = _choice(_QK_NORMS, norm, "norm")
-    pairs = _choice(_PAIRINGS, pairing, "pairing")
-    given = {"q": q, "k": k}
-    for name, x in given.items():
-        if x is None:
-            continue
-        if x.ndim != 4:
-            raise ValueError(f"{name} must be [batch, heads, tokens, dim], got {tuple(x.shape)}")
-        dtype_code(x.dtype)
-        if x.shape[-1] not in (64, 128):
-            raise ValueError(f"{name}: head dim {x.shape[-1]} unsupported (64 or 128)")
-    if k is not None and (k.dtype != q.dtype or k.shape[0] != q.shape[0]
-                          or k.shape[2:] != q.shape[2:]):
-        raise ValueError(f"K {tuple(k.shape)} {k.dtype} does not match Q {tuple(q.shape)} {q.dtype}")
-    if k is None and not k_weight is k_bias is k_out is None:
-        raise ValueError("k_weight, k_bias and k_out need a k")
-    b, h, n, d = q.shape
-    heads_k = 0 if k is None else k.shape[1]
-    spread = lambda heads: heads * d if kind == _lib.NORM_RMS_ALL else d  # noqa: E731
-    wide = {_qk_weights(kind, spread(heads), q.dtype, vectors)
-            for heads, vectors in ((h, {"q_weight": q_weight, "q_bias": q_bias}),
-                                   (heads_k, {"k_weight": k_weight, "k_bias": k_bias}))
-            if any(v is not None for v in vectors.values())}
-    if len(wide) > 1:
-        raise ValueError("the weights of q and k must have one type")
-    weight_code = wide.pop() if wide else _STREAM_DTYPES[q.dtype]
-    tables: list[torch.Tensor] = []
-    if axes is not None:
-        tables = list(axes)
-        if len(tables) != 3:
-            raise ValueError(f"axes must be three tables (time, height, width), got {len(tables)}")
-        for i, t in enumerate(tables):
-            if t.ndim != 3 or t.shape[2] != 2 or t.dtype != torch.float32 or t.shape[0] < 1:
-                raise ValueError(f"axis {i} must be fp32 [length, channels / 2, 2], got "
-                                 f"{tuple(t.shape)} {t.dtype}")
-        if sum(t.shape[1] for t in tables) != d // 2:
-            raise ValueError(f"the axes rotate {[2 * t.shape[1] for t in tables]} channels, the heads "
-                             f"have {d}")
-        video = math.prod(t.shape[0] for t in tables)
-        if not 0 <= offset <= n - video:
-            raise ValueError(f"tokens {offset}..{offset + video - 1} are not all in the sequence "
-                             f"of {n}")
-    inputs = {"q": q, "k": k, "q_weight": q_weight, "q_bias": q_bias, "k_weight": k_weight,
-              "k_bias": k_bias, **{f"axis {i}": t for i, t in enumerate(tables)}}
-    device = _together({**inputs, "q_out": q_out, "k_out": k_out})
-    outs = []
-    for name, x, out in (("q", q, q_out), ("k", k, k_out)):
-        if x is None:
-            outs.append(None)
-        elif out is None:
-            outs.append(torch.empty(x.shape, dtype=x.dtype, device=device))
-        else:
+    vectors = (q_weight, q_bias, k_weight, k_bias)
+    axes = None if axes is None else tuple(axes)
+    plan = _qk_plan(_spec(q), _spec(k), None if axes is None else tuple(map(_spec, axes)),
+                    int(offset), pairing, norm, tuple(map(_spec, vectors)))
+    if k is None and k_out is not None:
+        raise ValueError("k_out needs a k")
+    if q_out is not None or k_out is not None:
+        inputs = {"q": q, "k": k, "q_weight": q_weight, "q_bias": q_bias, "k_weight": k_weight,
+                  "k_bias": k_bias, **{f"axis {i}": t for i, t in enumerate(axes or ())}}
+        _together({"q": _spec(q), "q_out": _spec(q_out), "k_out": _spec(k_out)})
+        for name, x, out in (("q", q, q_out), ("k", k, k_out)):
+            if out is None:
+                continue
             _check_output(f"{name}_out", out, x.shape, x.dtype, inputs, name)
-            if out.data_ptr() % 16 or any(s % 8 for s in out.stride()[:3]):
+            if not _aligned_rows(_spec(out)) or out.data_ptr() % 16:
                 raise ValueError(f"{name}_out must have 16-byte aligned rows")
-            outs.append(out)
-    if q_out is not None and k_out is not None:
-        _check_output("k_out", k_out, k.shape, k.dtype, {"q_out": q_out}, "")
-    if q.numel() == 0 and (k is None or k.numel() == 0):
-        return tuple(outs)
-    if q.numel() == 0 or (k is not None and k.numel() == 0):
-        raise ValueError("q and k must both have heads")
-    q, k = prepare(q, "q"), None if k is None else prepare(k, "k")
-    tables = [t.contiguous() for t in tables]
-    vectors = [None if v is None else v.contiguous() for v in (q_weight, q_bias, k_weight, k_bias)]
-    pointers = lengths = counts = None
-    if tables:
-        pointers = (ctypes.c_void_p * 3)(*(t.data_ptr() if t.numel() else None for t in tables))
-        lengths = (ctypes.c_int64 * 3)(*(t.shape[0] for t in tables))
-        counts = (ctypes.c_int64 * 3)(*(t.shape[1] for t in tables))
-    none = (0, 0, 0)
-    _call_on(device, "recap_qk_rotary", q.data_ptr(), _p(k), dtype_code(q.dtype), b, n, d, h,
-             heads_k, *q.stride()[:3], *(none if k is None else k.stride()[:3]), pointers, lengths,
-             counts, int(offset), pairs, kind, *map(_p, vectors), weight_code, float(eps),
-             outs[0].data_ptr(), *outs[0].stride()[:3], _p(outs[1]),
-             *(none if k is None else outs[1].stride()[:3]))
-    return tuple(outs)
-
-
-def _rows(t: torch.Tensor | None) -> tuple:
-    """Pointer and (batch, token) strides of a [batch, tokens, width] tensor."""
-    return (None, 0, 0) if t is None else (t.data_ptr(), *t.stride()[:2])
+        if q_out is not None and k_out is not None:
+            _check_output("k_out", k_out, k.shape, k.dtype, {"q_out": q_out}, "")
+    strides, out_strides = plan.strides, plan.out_strides
+    if q_out is not None or k_out is not None:
+        out_strides = tuple(made if out is None else _row_strides(out.shape, out.stride())
+                            for out, made in zip((q_out, k_out), out_strides))
+    if q_out is None:
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if k_out is None and k is not None:
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+    if plan.empty:
+        return q_out, k_out
+    if plan.copies or q.data_ptr() % 16 or (k is not None and k.data_ptr() % 16):
+        q, k = prepare(q, "q"), None if k is None else prepare(k, "k")
+        axes = None if axes is None else tuple(t.contiguous() for t in axes)
+        vectors = tuple(None if v is None else v.contiguous() for v in vectors)
+        strides = tuple((0, 0, 0) if t is None else _row_strides(t.shape, t.stride())
+                        for t in (q, k))
+    _call_on(plan.device, "recap_qk_rotary", q.data_ptr(), _p(k), *plan.sizes, *strides[0],
+             *strides[1],
+             *((None,) * 3 if axes is None else [t.data_ptr() or None for t in axes]), plan.lengths,
+             plan.pairs, int(offset), *plan.codes, *map(_p, vectors), plan.weight_code, float(eps),
+             q_out.data_ptr(), *out_strides[0], _p(k_out), *out_strides[1])
+    return q_out, k_out
 
 
 def _unit(t: torch.Tensor | None) -> torch.Tensor | None:
     """The tensor with unit stride along its channels, as the kernels read it."""
-    return t if t is None or t.stride(-1) == 1 else t.contiguous()
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _modulation(vectors: dict[str, torch.Tensor | None], x: torch.Tensor,
-                dtype: torch.dtype) -> tuple[int, list]:
-    """(type code, (pointer, batch stride, token stride) each) of gate, scale and shift:
-    ``[width]``, ``[B or 1, width]`` or ``[B or 1, N or 1, width]``."""
-    given = [v for v in vectors.values() if v is not None]
-    types = {v.dtype for v in given} or {dtype}
-    if len(types) > 1 or not types <= {dtype, torch.float32}:
-        raise ValueError(f"{', '.join(vectors)} must all be {dtype} or all torch.float32")
-    batch, tokens, width = x.shape
-    rows = []
-    for name, v in vectors.items():
-        if v is None:
-            rows.append(None)
-            continue
-        lead = tuple(v.shape[:-1])
-        if v.ndim < 1 or v.ndim > 3 or v.shape[-1] != width or not all(
-                got in (1, full) for got, full in zip(lead, (batch, tokens))):
-            raise ValueError(f"{name} is {tuple(v.shape)}: expected [{width}], [{batch} or 1, {width}] "
-                             f"or [{batch} or 1, {tokens} or 1, {width}]")
-        v = _unit(v)
-        rows.append((v, *(v.stride(i) if v.shape[i] > 1 else 0 for i in range(len(lead))),
-                     *(0,) * (2 - len(lead))))
-    return _STREAM_DTYPES[types.pop()], rows
+@dataclass(frozen=True)
+class _ResidualPlan:
+    """What a residual-stream call of given shapes, strides and types passes besides addresses."""
+
+    device: torch.device
+    copies: bool       # some input is first laid out with unit channel stride
+    stream: tuple      # type, sizes and strides of x
+    branch: tuple      # type and strides of the branch, empty without one
+    mods: tuple        # (batch, token) strides of gate, scale and shift
+    codes: tuple       # their type, the weights' type, the norms
 
 
-def _residual_call(name: str, x: torch.Tensor, dtype: torch.dtype, *, branch=None, mods=None,
-                   norms=(), eps=1e-6, outs=()) -> tuple[torch.Tensor, ...]:
-    """Checks and launch of the residual-stream calls.  ``mods``: gate, scale and shift by
-    name; ``norms``: (kind, prefix, weight, bias) of the branch's and the result's norm;
-    ``outs``: (name, given tensor or None, type, the input it may be)."""
-    if x.ndim != 3 or x.shape[-1] < 1:
-        raise ValueError(f"x must be [batch, tokens, width], got {tuple(x.shape)}")
-    if x.dtype not in _STREAM_DTYPES or dtype not in _STREAM_DTYPES:
-        raise ValueError(f"unsupported dtype {x.dtype if x.dtype not in _STREAM_DTYPES else dtype}; "
-                         "use bfloat16, float16 or float32")
-    if x.dtype not in (dtype, torch.float32):
-        raise ValueError(f"a {x.dtype} stream goes with a branch and an output of its own type, not "
+@functools.lru_cache(maxsize=1024)
+def _residual_plan(names, dtype: torch.dtype, x, branch, mods, vectors, norms) -> _ResidualPlan:
+    """Checks of a residual-stream call, from its tensors' specs.  ``names``: of the modulation
+    and of the weights; ``norms``: (argument, name) of the branch's and the result's norm, each
+    with a weight and a bias among ``vectors``."""
+    kinds = [_choice(_NORMS, value, what) for what, value in norms]
+    shape = tuple(x[0])
+    if len(shape) != 3 or shape[2] < 1:
+        raise ValueError(f"x must be [batch, tokens, width], got {shape}")
+    for got in (x[2], dtype):
+        if got not in _STREAM_DTYPES:
+            raise ValueError(f"unsupported dtype {got}; use bfloat16, float16 or float32")
+    if x[2] not in (dtype, torch.float32):
+        raise ValueError(f"a {x[2]} stream goes with a branch and an output of its own type, not "
                          f"{dtype}; a float32 stream goes with any")
-    if branch is not None and branch.shape != x.shape:
-        raise ValueError(f"branch is {tuple(branch.shape)}, the stream {tuple(x.shape)}")
-    inputs = {"x": x, "branch": branch, **mods}
-    vectors = {}
-    for kind, prefix, weight, bias in norms:
-        pair = {f"{prefix}weight": weight, f"{prefix}bias": bias}
-        _qk_weights(kind, x.shape[-1], dtype, pair)
-        vectors.update(pair)
-    weight_code = _qk_weights(_lib.NORM_RMS, x.shape[-1], dtype, vectors)
-    inputs.update(vectors)
-    mod_code, mod_rows = _modulation(mods, x, dtype)
-    device = _together({**inputs, **{o[0]: o[1] for o in outs}})
+    if branch is not None and branch[0] != x[0]:
+        raise ValueError(f"branch is {tuple(branch[0])}, the stream {shape}")
+    batch, tokens, width = shape
+    types, strides = set(), []
+    for name, mod in zip(names[0], mods):
+        if mod is None:
+            strides.append((0, 0))
+            continue
+        lead, steps = tuple(mod[0][:-1]), mod[1]
+        if not 1 <= len(mod[0]) <= 3 or mod[0][-1] != width or not all(
+                got in (1, full) for got, full in zip(lead, (batch, tokens))):
+            raise ValueError(f"{name} is {tuple(mod[0])}: expected [{width}], [{batch} or 1, {width}] "
+                             f"or [{batch} or 1, {tokens} or 1, {width}]")
+        if mod[2] not in (dtype, torch.float32):
+            raise ValueError(f"{name} is {mod[2]}; gates, scales and shifts are {dtype} or "
+                             "torch.float32")
+        types.add(mod[2])
+        strides.append(tuple([steps[i] if lead[i] > 1 else 0 for i in range(len(lead))]
+                             + [0] * (2 - len(lead))))
+    mod_code = _one_type(types, dtype, " and ".join(names[0]))
+    types = set()
+    for i, kind in enumerate(kinds):
+        types |= _weights(kind, width, dtype, dict(zip(names[1][2 * i:2 * i + 2],
+                                                       vectors[2 * i:2 * i + 2])))
+    weight_code = _one_type(types, dtype, "weights and biases")
+    device = _together({"x": x, "branch": branch, **dict(zip(names[0], mods)),
+                        **dict(zip(names[1], vectors))})
+    copies = any(t[1][-1] != 1 and t[0][-1] > 1 for t in (x, branch, *mods, *vectors)
+                 if t is not None)
+    code = _STREAM_DTYPES[dtype]
+    return _ResidualPlan(device, copies, (_STREAM_DTYPES[x[2]], *shape, *x[1][:2]),
+                         () if branch is None else (code, *branch[1][:2]), tuple(strides),
+                         (mod_code, weight_code, *kinds))
+
+
+_SCALES, _GATES = ("scale", "shift"), ("gate",)
+_AFFINE, _BRANCH_AFFINE = ("weight", "bias"), ("branch_weight", "branch_bias")
+
+
+def _residual_call(name: str, names, x, dtype, branch, mods, vectors, norms, eps,
+                   outs) -> tuple[torch.Tensor, ...]:
+    """Checks and launch of the residual-stream calls.  ``outs``: (name, given tensor or None,
+    type, the input it may be)."""
+    plan = _residual_plan(names, dtype, _spec(x), _spec(branch), tuple(map(_spec, mods)),
+                          tuple(map(_spec, vectors)), norms)
     made = []
     for out_name, out, out_dtype, same in outs:
         if out is None:
-            out = torch.empty(x.shape, dtype=out_dtype, device=device)
+            out = torch.empty_like(x, dtype=out_dtype, memory_format=torch.contiguous_format)
         else:
-            others = {f"the other output ({o[0]})": m for o, m in zip(outs, made)}
-            _check_output(out_name, out, x.shape, out_dtype, {**inputs, **others}, same)
+            inputs = {"x": x, "branch": branch, **dict(zip(names[0], mods)),
+                      **dict(zip(names[1], vectors)),
+                      **{f"the other output ({o[0]})": m for o, m in zip(outs, made)}}
+            _together({"x": _spec(x), out_name: _spec(out)})
+            _check_output(out_name, out, x.shape, out_dtype, inputs, same)
         made.append(out)
     if x.numel() == 0:
         return tuple(made)
-    x, branch = _unit(x), _unit(branch)
-    vectors = {key: _unit(v) for key, v in vectors.items()}
-    mod_args = [(None, 0, 0) if m is None else (m[0].data_ptr(), *m[1:]) for m in mod_rows]
-    args = [x.data_ptr(), _STREAM_DTYPES[x.dtype], *x.shape, *x.stride()[:2]]
+    if plan.copies:
+        return _residual_call(name, names, _unit(x), dtype, _unit(branch), tuple(map(_unit, mods)),
+                              tuple(map(_unit, vectors)), norms, eps,
+                              [(*o[:1], m, *o[2:]) for o, m in zip(outs, made)])
+    args = [x.data_ptr(), *plan.stream]
     if branch is not None:
-        args += [branch.data_ptr(), _STREAM_DTYPES[dtype], *branch.stride()[:2]]
-    args += [a for m in mod_args for a in m]
-    args += [mod_code, *map(_p, vectors.values()), weight_code, *(n[0] for n in norms), float(eps)]
-    for i, out in enumerate(made):
-        args += [out.data_ptr(), *out.stride()[:2]]
-        if branch is None:
-            args.insert(-2, _STREAM_DTYPES[dtype])
-    _call_on(device, name, *args)
+        args += (branch.data_ptr(), *plan.branch)
+    for t, steps in zip(mods, plan.mods):
+        args += (_p(t), *steps)
+    args += (plan.codes[0], *map(_p, vectors), *plan.codes[1:], float(eps))
+    for out in made:
+        args += (out.data_ptr(), *out.stride()[:2])
+    if branch is None:
+        args.insert(-2, _STREAM_DTYPES[dtype])
+    _call_on(plan.device, name, *args)
     return tuple(made)
 
 
@@ -929,10 +1011,8 @@ def norm_modulate(x: torch.Tensor, scale: torch.Tensor | None = None,
     if norm is None:
         raise ValueError("norm must be 'layer' or 'rms'")
     dtype = dtype or x.dtype
-    kind = _choice(_NORMS, norm, "norm")
-    return _residual_call("recap_norm_modulate", x, dtype, mods={"scale": scale, "shift": shift},
-                          norms=[(kind, "", weight, bias)], eps=eps,
-                          outs=[("out", out, dtype, "x")])[0]
+    return _residual_call("recap_norm_modulate", (_SCALES, _AFFINE), x, dtype, None, (scale, shift),
+                          (weight, bias), (("norm", norm),), eps, [("out", out, dtype, "x")])[0]
 
 
 def gated_residual(x: torch.Tensor, branch: torch.Tensor, gate: torch.Tensor | None = None, *,
@@ -943,10 +1023,9 @@ def gated_residual(x: torch.Tensor, branch: torch.Tensor, gate: torch.Tensor | N
     ``[B, N, width]`` (of the branch's type or fp32), after an optional norm of its own.  ``gate``
     has the shapes of norm_modulate's ``scale``; None adds the branch as it is.  ``out`` may be x
     itself."""
-    kind = _choice(_NORMS, branch_norm, "branch_norm")
-    return _residual_call("recap_gated_residual", x, branch.dtype, branch=branch,
-                          mods={"gate": gate}, norms=[(kind, "branch_", branch_weight, branch_bias)],
-                          eps=eps, outs=[("out", out, x.dtype, "x")])[0]
+    return _residual_call("recap_gated_residual", (_GATES, _BRANCH_AFFINE), x, branch.dtype, branch,
+                          (gate,), (branch_weight, branch_bias), (("branch_norm", branch_norm),),
+                          eps, [("out", out, x.dtype, "x")])[0]
 
 
 def gated_residual_norm(x: torch.Tensor, branch: torch.Tensor, gate: torch.Tensor | None = None,
@@ -962,13 +1041,11 @@ def gated_residual_norm(x: torch.Tensor, branch: torch.Tensor, gate: torch.Tenso
     its rounding.  ``out`` (of r) may be x itself and ``norm_out`` (of y) branch itself."""
     if norm is None:
         raise ValueError("norm must be 'layer' or 'rms'")
-    kinds = _choice(_NORMS, branch_norm, "branch_norm"), _choice(_NORMS, norm, "norm")
-    return _residual_call("recap_gated_residual_norm", x, branch.dtype, branch=branch,
-                          mods={"gate": gate, "scale": scale, "shift": shift},
-                          norms=[(kinds[0], "branch_", branch_weight, branch_bias),
-                                 (kinds[1], "", weight, bias)], eps=eps,
-                          outs=[("out", out, x.dtype, "x"),
-                                ("norm_out", norm_out, branch.dtype, "branch")])
+    return _residual_call("recap_gated_residual_norm",
+                          (_GATES + _SCALES, _BRANCH_AFFINE + _AFFINE), x, branch.dtype, branch,
+                          (gate, scale, shift), (branch_weight, branch_bias, weight, bias),
+                          (("branch_norm", branch_norm), ("norm", norm)), eps,
+                          [("out", out, x.dtype, "x"), ("norm_out", norm_out, branch.dtype, "branch")])
 
 
 def bank_copy_async(dst: torch.Tensor, src: torch.Tensor, stream=None) -> None:

@@ -64,6 +64,7 @@ def axes64():
     (dict(q_weight=torch.zeros(32, dtype=BF), norm="rms"), "expected"),
     (dict(q_weight=torch.zeros(64, dtype=BF), norm="rms_all"), "expected"),
     (dict(q_weight=torch.zeros(64, dtype=FP), norm="rms"), "weights"),
+    (dict(q_weight=torch.zeros(64, dtype=BF), q_bias=torch.zeros(64), norm="rms"), "one type"),
     (dict(axes=axes64()[:2]), "three"), (dict(axes=[t.double() for t in axes64()]), "fp32"),
     (dict(axes=recap_amd.rotary_axes((2, 3, 4), (16, 24, 22))), "channels"),
     (dict(axes=axes64(), offset=7), "sequence"), (dict(axes=axes64(), offset=-1), "sequence"),
@@ -92,8 +93,8 @@ X32 = torch.zeros(2, 5, 24)
     (lambda: K.norm_modulate(X, torch.zeros(3, 24, dtype=BF)), "scale is"),
     (lambda: K.norm_modulate(X, None, torch.zeros(2, 4, 24, dtype=BF)), "shift is"),
     (lambda: K.norm_modulate(X, torch.zeros(1, 2, 5, 24, dtype=BF)), "scale is"),
-    (lambda: K.norm_modulate(X, torch.zeros(24, dtype=FP)), "must all be"),
-    (lambda: K.norm_modulate(X, torch.zeros(24), torch.zeros(24, dtype=BF)), "must all be"),
+    (lambda: K.norm_modulate(X, torch.zeros(24, dtype=FP)), "scale is"),
+    (lambda: K.norm_modulate(X, torch.zeros(24), torch.zeros(24, dtype=BF)), "one type"),
     (lambda: K.norm_modulate(X, weight=torch.zeros(23, dtype=BF)), "expected"),
     (lambda: K.norm_modulate(X, weight=torch.zeros(24), bias=torch.zeros(24, dtype=BF)), "weights"),
     (lambda: K.gated_residual(X, X[:, :4]), "branch is"),
@@ -144,7 +145,7 @@ def test_output_overlap_rule():
 
 
 GOOD_QK = dict(q=16, k=16, dtype=_lib.RECAP_BF16, batch=1, tokens=30, dim=64, qh=2, kh=2, qb=0, qs=64,
-               qn=128, kb=0, ks=64, kn=128, tables=(16, 16, 16), lengths=(2, 3, 4), pairs=(8, 12, 12),
+               qn=128, kb=0, ks=64, kn=128, t0=16, t1=16, t2=16, lengths=(2, 3, 4), pairs=(8, 12, 12),
                offset=6, pairing=0, norm=1, qw=16, qbias=None, kw=16, kbias=None, wt=_lib.RECAP_BF16,
                eps=1e-6, qo=16, qob=0, qos=64, qon=128, ko=16, kob=0, kos=64, kon=128)
 
@@ -153,15 +154,15 @@ GOOD_QK = dict(q=16, k=16, dtype=_lib.RECAP_BF16, batch=1, tokens=30, dim=64, qh
     dict(q=None), dict(q=8), dict(qo=None), dict(ko=None), dict(k=None), dict(dtype=_lib.RECAP_F32),
     dict(dim=96), dict(tokens=0), dict(batch=0), dict(qh=0), dict(qh=1 << 17), dict(kn=3), dict(kon=0),
     dict(batch=1 << 30), dict(pairing=2), dict(norm=4), dict(norm=-1), dict(norm=0), dict(eps=0.0),
-    dict(eps=float("nan")), dict(wt=_lib.RECAP_F16), dict(qw=17), dict(tables=(0, 16, 16)),
-    dict(tables=(16, 12, 16)), dict(lengths=(2, 3, 0)), dict(lengths=(2, 3, 31)),
+    dict(eps=float("nan")), dict(wt=_lib.RECAP_F16), dict(qw=17), dict(t0=None),
+    dict(t1=12), dict(lengths=None), dict(lengths=(2, 3, 0)), dict(lengths=(2, 3, 31)),
     dict(lengths=(3, 4, 4)), dict(pairs=(8, 12, 11)), dict(pairs=(-8, 28, 12)), dict(offset=7),
     dict(offset=-1)])
 def test_qk_rotary_entry_refusals(bad):
     import ctypes
     a = {**GOOD_QK, **bad}
-    a["tables"] = (ctypes.c_void_p * 3)(*(p or None for p in a["tables"]))
-    a["lengths"], a["pairs"] = ((ctypes.c_int64 * 3)(*a[n]) for n in ("lengths", "pairs"))
+    for name in ("lengths", "pairs"):
+        a[name] = a[name] and (ctypes.c_int64 * 3)(*a[name])
     with pytest.raises(ValueError):
         _lib.call("recap_qk_rotary", *a.values(), None)
 

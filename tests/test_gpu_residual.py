@@ -207,6 +207,16 @@ def test_a_large_mean(cuda):
     check_all(a, "layer", None, "large mean")
 
 
+def test_one_channel_with_another_stride(cuda):
+    """Rows of one channel, whose stride means nothing (transposed from [batch, 1, tokens])."""
+    x = torch.randn(2, 1, 5, device=cuda).transpose(1, 2)
+    scale = torch.randn(1, 3, device=cuda)[:, ::3]
+    assert x.stride() == (5, 1, 5)
+    want = K.gated_residual_norm(x.contiguous(), x.contiguous(), None, scale.clone(), norm="rms")
+    got = K.gated_residual_norm(x, x, None, scale, norm="rms")
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_empty(cuda):
     for shape in [(0, 5, 64), (2, 0, 64)]:
         x = torch.zeros(shape, dtype=BF, device=cuda)

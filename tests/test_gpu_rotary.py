@@ -118,6 +118,12 @@ def test_layouts(cuda, d, norm):
     odd[:, :, 1:] = a["q"].transpose(1, 2).reshape(b, n, h * d)
     view = odd[:, :, 1:].unflatten(2, (h, d)).transpose(1, 2)
     assert torch.equal(run({**a, "q": view}, axes, norm=norm, offset=off)[0], want[0])
+    apart = torch.zeros(2, h * n * d + 4, dtype=BF, device=cuda)   # an odd pitch of a batch of one
+    apart[0, :h * n * d] = a["q"][0].reshape(-1)
+    single = apart.as_strided((1, h, n, d), (apart.stride(0), n * d, d, 1))
+    assert single.stride(0) % 8 == 4
+    assert torch.equal(run({"q": single, **{m: v for m, v in rest.items() if m[0] == "q"}}, axes, norm=norm,
+                           offset=off)[0][0], want[0][0])
     one = run({**a, "q": a["q"][:1].expand(b, h, n, d)}, axes, norm=norm, offset=off)[0]
     assert torch.equal(one[1], want[0][0])
     whole = torch.full((b, h, n + 9, d), 5.0, dtype=BF, device=cuda)
