@@ -4,6 +4,8 @@
 //   y = norm(r) * (1 + scale) + shift           norm: none, RMS norm or LayerNorm
 // without a branch r = x.  Statistics, sums and products are fp32; r and y are each rounded
 // once, to their own type, and y is taken from the unrounded r.
+#include <algorithm>
+
 #include "kernels.hpp"
 #include "rows.hpp"
 
@@ -12,9 +14,9 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// A vector of fp32 or T values, by a flag that is uniform over the launch.
+// One value of an fp32 or T vector, by a flag that is uniform over the launch.
 template <class T>
-__device__ inline float load_either(const void* p, bool wide, int64_t i) {
+__device__ inline float load_one(const void* p, bool wide, int64_t i) {
   return wide ? load_elem<F32>(p, i) : load_elem<T>(p, i);
 }
 
@@ -68,9 +70,9 @@ __global__ __launch_bounds__(kThreads) void residual_rows_kernel(ResidualArgs a)
       float r = load_elem<X>(a.x.p, xo + c);
       if (a.branch.p) {
         float f = (added(c) - post.mean) * post.inv;
-        if (a.branch_weight) f *= load_either<T>(a.branch_weight, a.wide_weight, c);
-        if (a.branch_bias) f += load_either<T>(a.branch_bias, a.wide_weight, c);
-        r = a.gate.p ? fmaf(load_either<T>(a.gate.p, a.wide_mod, go + c), f, r) : r + f;
+        if (a.branch_weight) f *= load_one<T>(a.branch_weight, a.wide_weight, c);
+        if (a.branch_bias) f += load_one<T>(a.branch_bias, a.wide_weight, c);
+        r = a.gate.p ? fmaf(load_one<T>(a.gate.p, a.wide_mod, go + c), f, r) : r + f;
       }
       return r;
     };
@@ -82,10 +84,10 @@ __global__ __launch_bounds__(kThreads) void residual_rows_kernel(ResidualArgs a)
       const float r = value(c);
       if (a.y.p) {
         float y = (r - s.mean) * s.inv;
-        if (a.weight) y *= load_either<T>(a.weight, a.wide_weight, c);
-        if (a.bias) y += load_either<T>(a.bias, a.wide_weight, c);
-        if (a.scale.p) y *= 1.0f + load_either<T>(a.scale.p, a.wide_mod, so + c);
-        if (a.shift.p) y += load_either<T>(a.shift.p, a.wide_mod, ho + c);
+        if (a.weight) y *= load_one<T>(a.weight, a.wide_weight, c);
+        if (a.bias) y += load_one<T>(a.bias, a.wide_weight, c);
+        if (a.scale.p) y *= 1.0f + load_one<T>(a.scale.p, a.wide_mod, so + c);
+        if (a.shift.p) y += load_one<T>(a.shift.p, a.wide_mod, ho + c);
         store_elem<T>(const_cast<void*>(a.y.p), yo + c, y);
       }
       if (a.r.p) store_elem<X>(const_cast<void*>(a.r.p), ro + c, r);
@@ -100,10 +102,13 @@ __global__ __launch_bounds__(kThreads) void residual_rows_kernel(ResidualArgs a)
 // The row's last chunk is loaded from its last 8 elements, its elements before the chunk's
 // own (`skip` of them) left out of sums and stores; lanes past the row load it too.
 
+template <class X>
+constexpr int kChunk = X::code == 3 ? 4 : 8;  // 16 bytes of the stream
+
 enum ResidualKind { kPre, kGate, kBoth };
 
-template <int CHUNKS>
-__device__ Stats chunk_stats(int kind, const float (&v)[CHUNKS][8], int skip, int width, float eps,
+template <int CHUNKS, int N>
+__device__ Stats chunk_stats(int kind, const float (&v)[CHUNKS][N], int skip, int width, float eps,
                              int lanes, float* part) {
   Stats s{0.0f, 1.0f};
   if (kind == kNormNone) return s;
@@ -113,14 +118,14 @@ __device__ Stats chunk_stats(int kind, const float (&v)[CHUNKS][8], int skip, in
 #pragma unroll
     for (int j = 0; j < CHUNKS; ++j)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += j < CHUNKS - 1 || e >= skip ? v[j][e] : 0.0f;
+      for (int e = 0; e < N; ++e) sum += j < CHUNKS - 1 || e >= skip ? v[j][e] : 0.0f;
     s.mean = row_sum(sum, lanes, part) * per;
   }
   float sq = 0.0f;
 #pragma unroll
   for (int j = 0; j < CHUNKS; ++j)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < N; ++e) {
       const float d = j < CHUNKS - 1 || e >= skip ? v[j][e] - s.mean : 0.0f;
       sq = fmaf(d, d, sq);
     }
@@ -128,118 +133,134 @@ __device__ Stats chunk_stats(int kind, const float (&v)[CHUNKS][8], int skip, in
   return s;
 }
 
-template <class X, class T, int CHUNKS, int KIND>
-__global__ __launch_bounds__(1024) void residual_kernel(ResidualArgs a, int lanes) {
+// Combines a vector of fp32 or T values with a row, all of its loads sent out together.
+template <class T, int CHUNKS, int N, class F>
+__device__ inline void combine(const void* p, bool wide, int64_t base,
+                               const unsigned (&at)[CHUNKS], float (&v)[CHUNKS][N], F f) {
+  if (p == nullptr) return;
+  float w[CHUNKS][N];
+  if (wide) {
+    const void* row = row_of<F32>(p, base);
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) load_chunk<F32>(row, at[j], w[j]);
+  } else {
+    const void* row = row_of<T>(p, base);
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) load_chunk<T>(row, at[j], w[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < CHUNKS; ++j)
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[j][e] = f(v[j][e], w[j][e]);
+}
+
+template <class X, class T, int CHUNKS, int KIND, bool STREAM>
+__global__ __launch_bounds__(1024) void residual_kernel(ResidualArgs a, int lanes,
+                                                        int64_t first) {
+  constexpr int N = kChunk<X>;
   __shared__ float part[16];
   const int shift = 31 - __clz(lanes);
   int group = threadIdx.x >> shift;
   if (CHUNKS > 1) group = __builtin_amdgcn_readfirstlane(group);  // 64 lanes or more
   const int lane = threadIdx.x & (lanes - 1), per_block = blockDim.x >> shift;
-  int at[CHUNKS];
+  unsigned at[CHUNKS];
 #pragma unroll
-  for (int j = 0; j < CHUNKS; ++j) at[j] = 8 * (lane + lanes * j);
-  const int skip = min(max(at[CHUNKS - 1] - (a.width - 8), 0), 8);
-  at[CHUNKS - 1] = min(at[CHUNKS - 1], a.width - 8);
+  for (int j = 0; j < CHUNKS; ++j) at[j] = N * (lane + lanes * j);
+  const int last = a.width - N, skip = min(max((int)at[CHUNKS - 1] - last, 0), N);
+  at[CHUNKS - 1] = min((int)at[CHUNKS - 1], last);
 
-  const int64_t row = (int64_t)blockIdx.x * per_block + group;
+  const int64_t row = (first + blockIdx.x) * per_block + group;
   const bool live = row < a.rows;
   const unsigned r32 = (unsigned)(live ? row : a.rows - 1);
   const int64_t b = r32 / (unsigned)a.tokens, n = r32 - (unsigned)b * (unsigned)a.tokens;
-  float v[CHUNKS][8];
+  const auto times = [](float x, float w) { return x * w; };
+  const auto plus = [](float x, float w) { return x + w; };
+  const auto scaled = [](float x, float w) { return fmaf(x, w, x); };
+  const int64_t go = b * a.gate.b + n * a.gate.n, so = b * a.scale.b + n * a.scale.n,
+                ho = b * a.shift.b + n * a.shift.n;
+  float v[CHUNKS][N], f[KIND == kPre ? 1 : CHUNKS][N];
+  Rounded<X, N> r[CHUNKS];
   {
-    const int64_t base = b * a.x.b + n * a.x.n;
+    const void* x = row_of<X>(a.x.p, b * a.x.b + n * a.x.n);
 #pragma unroll
-    for (int j = 0; j < CHUNKS; ++j) load8<X>(a.x.p, base + at[j], v[j]);
+    for (int j = 0; j < CHUNKS; ++j) load_chunk<X, STREAM>(x, at[j], v[j]);
+    if constexpr (KIND != kPre) {
+      const void* added = row_of<T>(a.branch.p, b * a.branch.b + n * a.branch.n);
+#pragma unroll
+      for (int j = 0; j < CHUNKS; ++j) load_chunk<T, STREAM>(added, at[j], f[j]);
+    }
   }
   if constexpr (KIND != kPre) {
-    float f[CHUNKS][8];
-    const int64_t base = b * a.branch.b + n * a.branch.n, go = b * a.gate.b + n * a.gate.n;
-#pragma unroll
-    for (int j = 0; j < CHUNKS; ++j) load8<T>(a.branch.p, base + at[j], f[j]);
-    const Stats s = chunk_stats<CHUNKS>(a.post, f, skip, a.width, a.eps, lanes, part);
-#pragma unroll
-    for (int j = 0; j < CHUNKS; ++j) {
-      float w[8];
-      if (a.post != kNormNone) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[j][e] = (f[j][e] - s.mean) * s.inv;
-        if (a.branch_weight) {
-          load8_either<T>(a.branch_weight, a.wide_weight, at[j], w);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[j][e] *= w[e];
-        }
-        if (a.branch_bias) {
-          load8_either<T>(a.branch_bias, a.wide_weight, at[j], w);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[j][e] += w[e];
-        }
-      }
-      if (a.gate.p) {
-        load8_either<T>(a.gate.p, a.wide_mod, go + at[j], w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[j][e] = fmaf(w[e], f[j][e], v[j][e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[j][e] += f[j][e];
-      }
-    }
-    const int64_t ro = b * a.r.b + n * a.r.n;
-    if (live) {
+    if (a.post != kNormNone) {
+      const Stats s = chunk_stats(a.post, f, skip, a.width, a.eps, lanes, part);
 #pragma unroll
       for (int j = 0; j < CHUNKS; ++j)
-        store8<X>(const_cast<void*>(a.r.p), ro + at[j], v[j], j < CHUNKS - 1 ? 0 : skip);
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[j][e] = (f[j][e] - s.mean) * s.inv;
+    }
+    combine<T>(a.branch_weight, a.wide_weight, 0, at, f, times);
+    combine<T>(a.branch_bias, a.wide_weight, 0, at, f, plus);
+    combine<T>(a.gate.p, a.wide_mod, go, at, f, times);
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[j][e] += f[j][e];
+      r[j].set(v[j]);
     }
   }
   if constexpr (KIND != kGate) {
-    const Stats s = chunk_stats<CHUNKS>(a.norm, v, skip, a.width, a.eps, lanes, part);
-    const int64_t yo = b * a.y.b + n * a.y.n, so = b * a.scale.b + n * a.scale.n,
-                  ho = b * a.shift.b + n * a.shift.n;
+    const Stats s = chunk_stats(a.norm, v, skip, a.width, a.eps, lanes, part);
 #pragma unroll
-    for (int j = 0; j < CHUNKS; ++j) {
-      float w[8], y[8];
+    for (int j = 0; j < CHUNKS; ++j)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = (v[j][e] - s.mean) * s.inv;
-      if (a.weight) {
-        load8_either<T>(a.weight, a.wide_weight, at[j], w);
+      for (int e = 0; e < N; ++e) v[j][e] = (v[j][e] - s.mean) * s.inv;
+    combine<T>(a.weight, a.wide_weight, 0, at, v, times);
+    combine<T>(a.bias, a.wide_weight, 0, at, v, plus);
+    combine<T>(a.scale.p, a.wide_mod, so, at, v, scaled);
+    combine<T>(a.shift.p, a.wide_mod, ho, at, v, plus);
+  }
+  // Stores last: a load behind a store would have to wait for it.
+  if (!live) return;
+  void* ro = const_cast<void*>(row_of<X>(a.r.p, b * a.r.b + n * a.r.n));
+  void* yo = const_cast<void*>(row_of<T>(a.y.p, b * a.y.b + n * a.y.n));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] *= w[e];
-      }
-      if (a.bias) {
-        load8_either<T>(a.bias, a.wide_weight, at[j], w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] += w[e];
-      }
-      if (a.scale.p) {
-        load8_either<T>(a.scale.p, a.wide_mod, so + at[j], w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = fmaf(y[e], w[e], y[e]);
-      }
-      if (a.shift.p) {
-        load8_either<T>(a.shift.p, a.wide_mod, ho + at[j], w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] += w[e];
-      }
-      if (live)
-        store8<T>(const_cast<void*>(a.y.p), yo + at[j], y, j < CHUNKS - 1 ? 0 : skip);
+  for (int j = 0; j < CHUNKS; ++j) {
+    const int from = j < CHUNKS - 1 ? 0 : skip;
+    if constexpr (KIND != kPre) r[j].template store<true>(ro, at[j], from);
+    if constexpr (KIND != kGate) {
+      Rounded<T, N> y;
+      y.set(v[j]);
+      y.template store<false>(yo, at[j], from);
     }
   }
 }
 
-constexpr int kMinWidth = 8, kMaxWidth = 8 * 1024 * 4;
+constexpr int kMinWidth = 8, kMaxWidth = 4 * 1024 * 4;
 
 template <class X, class T, int CHUNKS, int KIND>
 hipError_t launch_rows(const ResidualArgs& a, int lanes, hipStream_t s) {
   const int threads = lanes > kThreads ? lanes : kThreads;
   const int64_t per_block = threads / lanes;
-  const int64_t grid = (a.rows + per_block - 1) / per_block;
-  residual_kernel<X, T, CHUNKS, KIND>
-      <<<dim3((unsigned)grid), dim3((unsigned)threads), 0, s>>>(a, lanes);
+  const int64_t all = (a.rows + per_block - 1) / per_block;
+  const int64_t bytes = a.rows * a.width *
+                        (KIND == kPre    ? kBytes<X> + kBytes<T>
+                         : KIND == kGate ? 2 * kBytes<X> + kBytes<T>
+                                         : 2 * kBytes<X> + 2 * kBytes<T>);
+  for (int64_t first = 0; first < all; first += kMaxBlocks) {
+    const dim3 grid((unsigned)std::min(all - first, kMaxBlocks)), block((unsigned)threads);
+    if (bytes >= kStreamBytes) {
+      residual_kernel<X, T, CHUNKS, KIND, true><<<grid, block, 0, s>>>(a, lanes, first);
+    } else {
+      residual_kernel<X, T, CHUNKS, KIND, false><<<grid, block, 0, s>>>(a, lanes, first);
+    }
+  }
   return hipGetLastError();
 }
 
 template <class X, class T, int KIND>
 hipError_t launch_kind(const ResidualArgs& a, hipStream_t s) {
-  const int chunks = (a.width + 7) / 8;
+  constexpr int N = kChunk<X>;
+  const int chunks = (a.width + N - 1) / N;
   int lanes = 1;
   while (lanes < chunks && lanes < 64) lanes *= 2;
   while (lanes * 4 < chunks) lanes *= 2;  // up to 4 chunks a lane, then more waves a row
@@ -257,7 +278,7 @@ hipError_t launch(const ResidualArgs& a, hipStream_t s) {
     if (!a.branch.p) return launch_kind<X, T, kPre>(a, s);
     return a.y.p ? launch_kind<X, T, kBoth>(a, s) : launch_kind<X, T, kGate>(a, s);
   }
-  const int64_t grid = a.rows < (1 << 20) ? a.rows : (1 << 20);
+  const int64_t grid = std::min(a.rows, kMaxBlocks);
   residual_rows_kernel<X, T><<<dim3((unsigned)grid), dim3(kThreads), 0, s>>>(a);
   return hipGetLastError();
 }

@@ -22,10 +22,16 @@ constexpr int kThreads = 256;
 constexpr int kBatch = 4;  // head rows in flight per lane
 
 template <class T>
-__device__ inline void load16(const void* p, bool wide, int64_t i, int half, float (&v)[16]) {
+__device__ inline void load16(const void* p, bool wide, unsigned i, unsigned half,
+                              float (&v)[16]) {
   float lo[8], hi[8];
-  load8_either<T>(p, wide, i, lo);
-  load8_either<T>(p, wide, i + half, hi);
+  if (wide) {
+    load_chunk<F32>(p, i, lo);
+    load_chunk<F32>(p, i + half, hi);
+  } else {
+    load_chunk<T>(p, i, lo);
+    load_chunk<T>(p, i + half, hi);
+  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     v[e] = lo[e];
@@ -33,14 +39,14 @@ __device__ inline void load16(const void* p, bool wide, int64_t i, int half, flo
   }
 }
 
-template <class T, int D, bool HALVES, int NORM>
-__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
+template <class T, int D, bool HALVES, int NORM, bool STREAM>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, int64_t first_block) {
   constexpr int kLanes = D / 16, kRows = 64 / kLanes;
   const RotaryTensor& t = a.x[blockIdx.y];
   const int side = t.side;
   const int lane = threadIdx.x & 63, u = lane & (kLanes - 1), g = lane / kLanes;
   const int hl = g & (side - 1), tokens = kRows / side, tl = g / side;
-  const int64_t wave = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  const int64_t wave = (first_block + blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
   if (wave * tokens >= a.rows) return;  // q and k need not take the same number of waves
   const int64_t row = wave * tokens + tl;
   const bool live = row < a.rows;
@@ -72,15 +78,13 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
     }
   }
 
-  float w[16], bias[16];
+  float w[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
     w[e] = 1.0f;
-    bias[e] = 0.0f;
   }
   if (NORM == kRotaryRms || NORM == kRotaryLayer) {
     if (t.weight) load16<T>(t.weight, a.wide_weight, 8 * u, D / 2, w);
-    if (t.bias) load16<T>(t.bias, a.wide_weight, 8 * u, D / 2, bias);
   }
 
   const uint16_t* src = t.in + b * t.in_b + n * t.in_n + hl * t.in_h + 8 * u;
@@ -92,8 +96,8 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
     for (int j = 0; j < kBatch; ++j)
       if (first + j < steps) {
         const uint16_t* p = src + (int64_t)(first + j) * side * t.in_h;
-        raw[j][0] = *reinterpret_cast<const u32x4*>(p);
-        raw[j][1] = *reinterpret_cast<const u32x4*>(p + D / 2);
+        raw[j][0] = load_words4<STREAM && D == 128>(p);
+        raw[j][1] = load_words4<STREAM && D == 128>(p + D / 2);
       }
   };
   const auto widen = [&](int j, float (&x)[16]) {
@@ -143,14 +147,19 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
         for (int e = 0; e < 16; ++e) sq = fmaf(x[e], x[e], sq);
         inv = 1.0f / sqrtf(row_sum(sq, kLanes, nullptr) * (1.0f / D) + a.eps);
       }
-      if (NORM == kRotaryRmsAll) {
-        const int64_t at = (int64_t)((first + j) * side + hl) * D + 8 * u;
-        if (t.weight) load16<T>(t.weight, a.wide_weight, at, D / 2, w);
-        if (t.bias) load16<T>(t.bias, a.wide_weight, at, D / 2, bias);
-      }
+      // The head's place in the weights: those over a head's channels are the same for all.
+      const unsigned at =
+          8 * u + (NORM == kRotaryRmsAll ? (unsigned)((first + j) * side + hl) * D : 0);
+      if (NORM == kRotaryRmsAll && t.weight) load16<T>(t.weight, a.wide_weight, at, D / 2, w);
       if (NORM != kRotaryNone) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = fmaf(x[e] * inv, w[e], bias[e]);
+        for (int e = 0; e < 16; ++e) x[e] = x[e] * inv * w[e];
+        if (t.bias) {
+          float bias[16];
+          load16<T>(t.bias, a.wide_weight, at, D / 2, bias);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[e] += bias[e];
+        }
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -166,8 +175,8 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
       }
       if (live) {
         uint16_t* o = dst + (int64_t)(first + j) * side * t.out_h;
-        *reinterpret_cast<u32x4*>(o) = lo;
-        *reinterpret_cast<u32x4*>(o + D / 2) = hi;
+        store_words4<STREAM>(o, lo);
+        store_words4<STREAM>(o + D / 2, hi);
       }
     }
   }
@@ -177,17 +186,25 @@ template <class T, int D, bool HALVES, int NORM>
 hipError_t launch(const RotaryArgs& a, hipStream_t s) {
   constexpr int kRows = 64 / (D / 16);
   RotaryArgs b = a;
-  int64_t waves = 1;
+  int64_t waves = 1, values = 0;  // rows of d
   for (int i = 0; i < a.tensors; ++i) {
     // Each tensor by its own heads, so that q's sums do not depend on k's.
     int side = 1;
     while (side < kRows && a.x[i].heads % (2 * side) == 0) side *= 2;
     b.x[i].side = side;
+    values += a.rows * a.x[i].heads;
     waves = std::max(waves, (a.rows + kRows / side - 1) / (kRows / side));
   }
   constexpr int kWaves = kThreads / 64;
-  const dim3 grid((unsigned)((waves + kWaves - 1) / kWaves), a.tensors);
-  rotary_kernel<T, D, HALVES, NORM><<<grid, dim3(kThreads), 0, s>>>(b);
+  const int64_t blocks = (waves + kWaves - 1) / kWaves;
+  for (int64_t first = 0; first < blocks; first += kMaxBlocks) {
+    const dim3 grid((unsigned)std::min(blocks - first, kMaxBlocks), a.tensors);
+    if (4 * D * values >= kStreamBytes) {
+      rotary_kernel<T, D, HALVES, NORM, true><<<grid, dim3(kThreads), 0, s>>>(b, first);
+    } else {
+      rotary_kernel<T, D, HALVES, NORM, false><<<grid, dim3(kThreads), 0, s>>>(b, first);
+    }
+  }
   return hipGetLastError();
 }
 

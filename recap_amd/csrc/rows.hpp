@@ -28,58 +28,133 @@ __device__ inline void store_elem(void* p, int64_t i, float v) {
   }
 }
 
-typedef u32x4 u32x4_any __attribute__((aligned(2)));
-typedef f32x4 f32x4_any __attribute__((aligned(4)));
-
 template <class T>
-__device__ inline void load8(const void* p, int64_t i, float (&v)[8]) {
+constexpr unsigned kBytes = T::code == 3 ? 4 : 2;
+
+constexpr int64_t kMaxBlocks = 1 << 20;  // of a launch, whose threads have to be under 2^32
+
+// A call that moves this much or more loads its rows past the caches.
+constexpr int64_t kStreamBytes = int64_t(192) << 20;
+
+// 16 and 8 bytes at any address; STREAM: past the caches, for data that is used once.  (A vector
+// type's alignment is lost in a template argument, so the types are named here.)
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+
+template <bool STREAM>
+__device__ inline u32x4 load_words4(const void* p) {
+  const u32x4_any* q = static_cast<const u32x4_any*>(p);
+  return STREAM ? __builtin_nontemporal_load(q) : *q;
+}
+template <bool STREAM>
+__device__ inline u32x2 load_words2(const void* p) {
+  const u32x2_any* q = static_cast<const u32x2_any*>(p);
+  return STREAM ? __builtin_nontemporal_load(q) : *q;
+}
+template <bool STREAM>
+__device__ inline void store_words4(void* p, u32x4 w) {
+  u32x4_any* q = static_cast<u32x4_any*>(p);
+  if (STREAM) {
+    __builtin_nontemporal_store(w, q);
+  } else {
+    *q = w;
+  }
+}
+template <bool STREAM>
+__device__ inline void store_words2(void* p, u32x2 w) {
+  u32x2_any* q = static_cast<u32x2_any*>(p);
+  if (STREAM) {
+    __builtin_nontemporal_store(w, q);
+  } else {
+    *q = w;
+  }
+}
+
+// Address of element i of a row: the row's own address is uniform over a wave of 64 lanes a row,
+// and a 32-bit byte offset to it is the form the memory instructions take without arithmetic.
+template <class T>
+__device__ inline const char* place(const void* row, unsigned i) {
+  return static_cast<const char*>(row) + i * kBytes<T>;
+}
+template <class T>
+__device__ inline char* place(void* row, unsigned i) {
+  return static_cast<char*>(row) + i * kBytes<T>;
+}
+template <class T>
+__device__ inline const void* row_of(const void* p, int64_t i) {
+  return static_cast<const char*>(p) + i * kBytes<T>;
+}
+
+// N elements (4 or 8) of a row from element i on, as fp32.
+template <class T, bool STREAM = false, int N>
+__device__ inline void load_chunk(const void* row, unsigned i, float (&v)[N]) {
   if constexpr (T::code == 3) {
-    const f32x4_any* q = reinterpret_cast<const f32x4_any*>(static_cast<const float*>(p) + i);
-    const f32x4 lo = q[0], hi = q[1];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = lo[e];
-      v[4 + e] = hi[e];
+    for (int k = 0; k < N; k += 4) {
+      const u32x4 w = load_words4<STREAM>(place<T>(row, i + k));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[k + e] = __uint_as_float(w[e]);
     }
   } else {
-    const u32x4 w =
-        *reinterpret_cast<const u32x4_any*>(static_cast<const uint16_t*>(p) + i);
+    unsigned w[N / 2];
+    if constexpr (N == 8) {
+      const u32x4 u = load_words4<STREAM>(place<T>(row, i));
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 4; ++e) w[e] = u[e];
+    } else {
+      const u32x2 u = load_words2<STREAM>(place<T>(row, i));
+      w[0] = u[0];
+      w[1] = u[1];
+    }
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) {
       v[2 * e] = T::to_f((uint16_t)w[e]);
       v[2 * e + 1] = T::to_f((uint16_t)(w[e] >> 16));
     }
   }
 }
 
-template <class T>
-__device__ inline void load8_either(const void* p, bool wide, int64_t i, float (&v)[8]) {
-  if (wide) {
-    load8<F32>(p, i, v);
-  } else {
-    load8<T>(p, i, v);
-  }
-}
+// N elements rounded to T, as they go to memory.
+template <class T, int N>
+struct Rounded {
+  static constexpr int kWords = T::code == 3 ? N : N / 2;
+  unsigned w[kWords];
 
-template <class T>
-__device__ inline void store8(void* p, int64_t i, const float (&v)[8], int skip) {
-  if (skip == 0) {
+  __device__ inline void set(const float (&v)[N]) {
     if constexpr (T::code == 3) {
-      f32x4_any* q = reinterpret_cast<f32x4_any*>(static_cast<float*>(p) + i);
-      q[0] = f32x4{v[0], v[1], v[2], v[3]};
-      q[1] = f32x4{v[4], v[5], v[6], v[7]};
+#pragma unroll
+      for (int e = 0; e < N; ++e) w[e] = __float_as_uint(v[e]);
     } else {
-      u32x4 w;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = pack2<T>(v[2 * e], v[2 * e + 1]);
-      *reinterpret_cast<u32x4_any*>(static_cast<uint16_t*>(p) + i) = w;
+      for (int e = 0; e < N / 2; ++e) w[e] = pack2<T>(v[2 * e], v[2 * e + 1]);
     }
-  } else if (skip < 8) {
-#pragma unroll
-    for (int e = 1; e < 8; ++e)
-      if (e >= skip) store_elem<T>(p, i + e, v[e]);
   }
-}
+
+  // To elements i.. of a row, those from `skip` on.
+  template <bool STREAM>
+  __device__ inline void store(void* row, unsigned i, int skip) const {
+    if (skip == 0) {
+      if constexpr (kWords >= 4) {
+#pragma unroll
+        for (int k = 0; k < kWords; k += 4)
+          store_words4<STREAM>(place<T>(row, i) + 4 * k, u32x4{w[k], w[k + 1], w[k + 2], w[k + 3]});
+      } else {
+        store_words2<STREAM>(place<T>(row, i), u32x2{w[0], w[1]});
+      }
+    } else if (skip < N) {
+#pragma unroll
+      for (int e = 1; e < N; ++e)
+        if (e >= skip) {
+          if constexpr (T::code == 3) {
+            *reinterpret_cast<unsigned*>(place<T>(row, i + e)) = w[e];
+          } else {
+            *reinterpret_cast<uint16_t*>(place<T>(row, i + e)) =
+                (uint16_t)(e & 1 ? w[e / 2] >> 16 : w[e / 2]);
+          }
+        }
+    }
+  }
+};
 
 // Sum over the `lanes` lanes of a row, in each of them: within 64 lanes a butterfly on the
 // VALU (both lanes of a pair add the same two values), then the row's waves in order.

@@ -767,6 +767,14 @@ def _aligned_rows(spec) -> bool:
     return strides[-1] == 1 and not any(s % 8 for s, n in zip(strides[:3], shape) if n > 1)
 
 
+def _order(spec) -> tuple:
+    """Batch, head and token strides of an output without gaps in its input's order: tokens
+    before heads (a projection's) or heads before tokens."""
+    (_, h, n, d), (_, by_head, by_token, _) = spec[:2]
+    token_major = h > 1 and n > 1 and by_head < by_token
+    return (h * n * d, d, h * d) if token_major else (h * n * d, n * d, d)
+
+
 def _row_strides(shape, strides) -> tuple:
     """Batch, head and token strides; of a dimension of one, whose stride means nothing, d."""
     return tuple(s if n > 1 else shape[3] for s, n in zip(strides[:3], shape))
@@ -826,7 +834,7 @@ def _qk_plan(q, k, axes, offset: int, pairing: str, norm, vectors) -> _QKPlan:
     return _QKPlan(device, copies, empty, (dtype_code(dtype), b, n, d, h, heads_k), lengths, counts,
                    (pairs, kind), weight_code,
                    tuple((0, 0, 0) if t is None else _row_strides(*t[:2]) for t in (q, k)),
-                   tuple((0, 0, 0) if t is None else (t[0][1] * n * d, n * d, d) for t in (q, k)))
+                   tuple((0, 0, 0) if t is None else _order(t) for t in (q, k)))
 
 
 def qk_rotary(q: torch.Tensor, k: torch.Tensor | None = None, axes=None, *, offset: int = 0,
@@ -846,8 +854,9 @@ def qk_rotary(q: torch.Tensor, k: torch.Tensor | None = None, axes=None, *, offs
     them; the others (text) are not.  ``pairing``: channels ``(2i, 2i + 1)`` (``"interleaved"``) or
     ``(i, i + d / 2)`` (``"halves"``).  ``axes=None`` rotates nothing.
 
-    ``q_out`` and ``k_out`` may be ``q`` and ``k`` themselves, or views into a longer sequence
-    (a text stream's part of it)."""
+    The outputs have no gaps and keep their input's order in memory (tokens before heads, as a
+    projection has them, or heads before tokens).  ``q_out`` and ``k_out`` may be ``q`` and ``k``
+    themselves, or views into a longer sequence (a text stream's part of it)."""
     vectors = (q_weight, q_bias, k_weight, k_bias)
     axes = None if axes is None else tuple(axes)
     plan = _qk_plan(_spec(q), _spec(k), None if axes is None else tuple(map(_spec, axes)),
@@ -871,9 +880,9 @@ def qk_rotary(q: torch.Tensor, k: torch.Tensor | None = None, axes=None, *, offs
         out_strides = tuple(made if out is None else _row_strides(out.shape, out.stride())
                             for out, made in zip((q_out, k_out), out_strides))
     if q_out is None:
-        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        q_out = q.new_empty_strided(q.shape, (*out_strides[0], 1))
     if k_out is None and k is not None:
-        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        k_out = k.new_empty_strided(k.shape, (*out_strides[1], 1))
     if plan.empty:
         return q_out, k_out
     if plan.copies or q.data_ptr() % 16 or (k is not None and k.data_ptr() % 16):

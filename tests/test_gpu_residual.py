@@ -298,3 +298,27 @@ def test_offsets_beyond_32_bits(cuda):
     want = K.norm_modulate(tail["x"])
     got = K.norm_modulate(x, out=x)
     assert torch.equal(got[:, -9:], want) and not got[:, :-9].any()
+
+
+def test_more_rows_than_one_launch(cuda):
+    """Rows beyond a launch's 2^20 workgroups (of 256 rows each at this width)."""
+    rows = (1 << 28) + 1000
+    x = torch.zeros(1, rows, 8, dtype=BF, device=cuda)
+    tail = make(31, 1, 700, 8, (BF, BF, BF), "none", affine=False)["x"]
+    x[:, -700:] = tail
+    want = K.gated_residual(tail, tail, branch_norm="rms")
+    got = K.gated_residual(x, x.clone(), branch_norm="rms", out=x)
+    assert torch.equal(got[:, -700:], want) and not got[:, :-700].any()
+
+
+@pytest.mark.parametrize("types", [(BF, BF, F32), (F32, FP, F32), (F32, F32, F32)], ids=str)
+def test_large_calls_equal_small_ones(cuda, types):
+    """A call large enough to load past the caches gives each row what a call of its own does."""
+    a = make(32, 1, 40000, 1536, types)
+    whole, pre, gate = run_both(a, "layer", "rms"), run_pre(a, "rms", types[1]), run_gate(a, None)
+    for rows in (slice(0, 3), slice(17000, 17009), slice(39995, 40000)):
+        part = {n: v[:, rows] if v.ndim == 3 and v.shape[1] > 1 else v for n, v in a.items()}
+        got = run_both(part, "layer", "rms")
+        assert torch.equal(got[0], whole[0][:, rows]) and torch.equal(got[1], whole[1][:, rows])
+        assert torch.equal(run_pre(part, "rms", types[1]), pre[:, rows])
+        assert torch.equal(run_gate(part, None), gate[:, rows])

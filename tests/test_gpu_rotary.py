@@ -112,6 +112,7 @@ def test_layouts(cuda, d, norm):
         print(f"case {label}", flush=True)
         got = run({**tensors, **rest}, axes, norm=norm, offset=off)
         assert all(torch.equal(x, y) for x, y in zip(got, want)), label
+        assert all(x.transpose(1, 2).is_contiguous() for x in got), label
         run({**tensors, **rest}, axes, norm=norm, offset=off, q_out=tensors["q"], k_out=tensors["k"])
         assert all(torch.equal(tensors[m], y) for m, y in zip("qk", want)), label
     assert torch.equal(fused[:, :, 2], torch.ones_like(fused[:, :, 2]))
@@ -205,3 +206,33 @@ def test_offsets_beyond_32_bits(cuda):
     want = K.qk_rotary(tail["q"], None, axes, norm="rms", q_weight=weight)[0]
     got = K.qk_rotary(q, None, axes, offset=n - 11, norm="rms", q_weight=weight, q_out=q)[0]
     assert torch.equal(got[:, :, -11:], want) and not got[:, :, :-11].any()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("norm", [None, "rms", "layer", "rms_all"])
+def test_large_calls_equal_small_ones(cuda, d, norm):
+    """A call large enough to pass the caches by gives each token what a call of its own does."""
+    h, n = 12, 3 * 64 * 100 * 128 // d
+    a = make(13, 1, h, n, d, norm=norm)
+    axes = recap_amd.rotary_axes((3, 1, n // 3), CHANNELS[d], device=cuda)
+    whole = run(a, axes, norm=norm)
+    for first in (0, n // 3 - 5, n - 9):
+        where = [torch.arange(first, first + 9) // (n // 3), torch.arange(first, first + 9) % (n // 3)]
+        rows = slice(first, first + 9)
+        for i in range(9):   # a grid of one position, the token's own
+            one = (axes[0][where[0][i]][None], axes[1], axes[2][where[1][i]][None])
+            part = {m: v[:, :, first + i:first + i + 1] if len(m) == 1 else v for m, v in a.items()}
+            got = run(part, one, norm=norm)
+            assert all(torch.equal(x, y[:, :, rows][:, :, i:i + 1]) for x, y in zip(got, whole))
+
+
+def test_more_tokens_than_one_launch(cuda):
+    """Tokens beyond a launch's 2^20 workgroups (of 4 tokens each with 16 heads of 64)."""
+    n = (1 << 22) + 50
+    q = torch.zeros(1, n, 16, 64, dtype=BF, device=cuda).transpose(1, 2)
+    tail = make(14, 1, 16, 40, 64, norm="rms")
+    q[:, :, -40:] = tail["q"]
+    axes = recap_amd.rotary_axes((1, 2, 20), CHANNELS[64], device=cuda)
+    want = K.qk_rotary(tail["q"], None, axes, norm="rms", q_weight=tail["q_weight"])[0]
+    got = K.qk_rotary(q, None, axes, offset=n - 40, norm="rms", q_weight=tail["q_weight"], q_out=q)[0]
+    assert torch.equal(got[:, :, -40:], want) and not got[:, :, :-40].any()
