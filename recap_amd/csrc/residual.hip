@@ -133,10 +133,11 @@ __device__ Stats chunk_stats(int kind, const float (&v)[CHUNKS][N], int skip, in
   return s;
 }
 
-// Combines a vector of fp32 or T values with a row, all of its loads sent out together.
-template <class T, int CHUNKS, int N, class F>
+// Combines a vector of fp32 or T values with the rows that share it, all of its loads sent out
+// together.
+template <class T, int ROWS, int CHUNKS, int N, class F>
 __device__ inline void combine(const void* p, bool wide, int64_t base,
-                               const unsigned (&at)[CHUNKS], float (&v)[CHUNKS][N], F f) {
+                               const unsigned (&at)[CHUNKS], float (&v)[ROWS][CHUNKS][N], F f) {
   if (p == nullptr) return;
   float w[CHUNKS][N];
   if (wide) {
@@ -149,14 +150,31 @@ __device__ inline void combine(const void* p, bool wide, int64_t base,
     for (int j = 0; j < CHUNKS; ++j) load_chunk<T>(row, at[j], w[j]);
   }
 #pragma unroll
-  for (int j = 0; j < CHUNKS; ++j)
+  for (int i = 0; i < ROWS; ++i)
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[j][e] = f(v[j][e], w[j][e]);
+    for (int j = 0; j < CHUNKS; ++j)
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[i][j][e] = f(v[i][j][e], w[j][e]);
 }
 
-template <class X, class T, int CHUNKS, int KIND, bool STREAM>
-__global__ __launch_bounds__(1024) void residual_kernel(ResidualArgs a, int lanes,
-                                                        int64_t first) {
+// Each row's norm, before its weight and bias.
+template <int ROWS, int CHUNKS, int N>
+__device__ inline void normalise(int kind, int skip, int width, float eps, int lanes, float* part,
+                                 float (&v)[ROWS][CHUNKS][N]) {
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const Stats s = chunk_stats(kind, v[i], skip, width, eps, lanes, part);
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j)
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[i][j][e] = (v[i][j][e] - s.mean) * s.inv;
+  }
+}
+
+// ROWS > 1: rows of one sample (`per_sample` workgroups each) that share gate, scale and shift.
+template <class X, class T, int ROWS, int CHUNKS, int KIND, bool STREAM>
+__global__ __launch_bounds__(1024) void residual_kernel(ResidualArgs a, int lanes, int64_t first,
+                                                        int per_sample) {
   constexpr int N = kChunk<X>;
   __shared__ float part[16];
   const int shift = 31 - __clz(lanes);
@@ -169,79 +187,91 @@ __global__ __launch_bounds__(1024) void residual_kernel(ResidualArgs a, int lane
   const int last = a.width - N, skip = min(max((int)at[CHUNKS - 1] - last, 0), N);
   at[CHUNKS - 1] = min((int)at[CHUNKS - 1], last);
 
-  const int64_t row = (first + blockIdx.x) * per_block + group;
-  const bool live = row < a.rows;
-  const unsigned r32 = (unsigned)(live ? row : a.rows - 1);
-  const int64_t b = r32 / (unsigned)a.tokens, n = r32 - (unsigned)b * (unsigned)a.tokens;
+  int64_t b, n[ROWS];
+  bool live[ROWS];
+  if constexpr (ROWS == 1) {
+    const int64_t row = (first + blockIdx.x) * per_block + group;
+    live[0] = row < a.rows;
+    const unsigned r32 = (unsigned)(live[0] ? row : a.rows - 1);
+    b = r32 / (unsigned)a.tokens;
+    n[0] = r32 - (unsigned)b * (unsigned)a.tokens;
+  } else {
+    const unsigned block = (unsigned)first + blockIdx.x;
+    b = block / (unsigned)per_sample;
+    const int64_t n0 = (int64_t)(block - (unsigned)b * (unsigned)per_sample) * per_block * ROWS;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      n[i] = n0 + i * per_block + group;
+      live[i] = n[i] < a.tokens;
+      n[i] = live[i] ? n[i] : a.tokens - 1;
+    }
+  }
   const auto times = [](float x, float w) { return x * w; };
   const auto plus = [](float x, float w) { return x + w; };
   const auto scaled = [](float x, float w) { return fmaf(x, w, x); };
-  const int64_t go = b * a.gate.b + n * a.gate.n, so = b * a.scale.b + n * a.scale.n,
-                ho = b * a.shift.b + n * a.shift.n;
-  float v[CHUNKS][N], f[KIND == kPre ? 1 : CHUNKS][N];
-  Rounded<X, N> r[CHUNKS];
-  {
-    const void* x = row_of<X>(a.x.p, b * a.x.b + n * a.x.n);
+  float v[ROWS][CHUNKS][N], f[KIND == kPre ? 1 : ROWS][CHUNKS][N];
+  Rounded<X, N> r[ROWS][CHUNKS];
 #pragma unroll
-    for (int j = 0; j < CHUNKS; ++j) load_chunk<X, STREAM>(x, at[j], v[j]);
-    if constexpr (KIND != kPre) {
-      const void* added = row_of<T>(a.branch.p, b * a.branch.b + n * a.branch.n);
+  for (int i = 0; i < ROWS; ++i) {
+    const void* x = row_of<X>(a.x.p, b * a.x.b + n[i] * a.x.n);
 #pragma unroll
-      for (int j = 0; j < CHUNKS; ++j) load_chunk<T, STREAM>(added, at[j], f[j]);
-    }
+    for (int j = 0; j < CHUNKS; ++j) load_chunk<X, STREAM>(x, at[j], v[i][j]);
   }
   if constexpr (KIND != kPre) {
-    if (a.post != kNormNone) {
-      const Stats s = chunk_stats(a.post, f, skip, a.width, a.eps, lanes, part);
 #pragma unroll
-      for (int j = 0; j < CHUNKS; ++j)
+    for (int i = 0; i < ROWS; ++i) {
+      const void* added = row_of<T>(a.branch.p, b * a.branch.b + n[i] * a.branch.n);
 #pragma unroll
-        for (int e = 0; e < N; ++e) f[j][e] = (f[j][e] - s.mean) * s.inv;
+      for (int j = 0; j < CHUNKS; ++j) load_chunk<T, STREAM>(added, at[j], f[i][j]);
     }
+    if (a.post != kNormNone) normalise(a.post, skip, a.width, a.eps, lanes, part, f);
     combine<T>(a.branch_weight, a.wide_weight, 0, at, f, times);
     combine<T>(a.branch_bias, a.wide_weight, 0, at, f, plus);
-    combine<T>(a.gate.p, a.wide_mod, go, at, f, times);
+    combine<T>(a.gate.p, a.wide_mod, b * a.gate.b + n[0] * a.gate.n, at, f, times);
 #pragma unroll
-    for (int j = 0; j < CHUNKS; ++j) {
+    for (int i = 0; i < ROWS; ++i)
 #pragma unroll
-      for (int e = 0; e < N; ++e) v[j][e] += f[j][e];
-      r[j].set(v[j]);
-    }
+      for (int j = 0; j < CHUNKS; ++j) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[i][j][e] += f[i][j][e];
+        r[i][j].set(v[i][j]);
+      }
   }
   if constexpr (KIND != kGate) {
-    const Stats s = chunk_stats(a.norm, v, skip, a.width, a.eps, lanes, part);
-#pragma unroll
-    for (int j = 0; j < CHUNKS; ++j)
-#pragma unroll
-      for (int e = 0; e < N; ++e) v[j][e] = (v[j][e] - s.mean) * s.inv;
+    normalise(a.norm, skip, a.width, a.eps, lanes, part, v);
     combine<T>(a.weight, a.wide_weight, 0, at, v, times);
     combine<T>(a.bias, a.wide_weight, 0, at, v, plus);
-    combine<T>(a.scale.p, a.wide_mod, so, at, v, scaled);
-    combine<T>(a.shift.p, a.wide_mod, ho, at, v, plus);
+    combine<T>(a.scale.p, a.wide_mod, b * a.scale.b + n[0] * a.scale.n, at, v, scaled);
+    combine<T>(a.shift.p, a.wide_mod, b * a.shift.b + n[0] * a.shift.n, at, v, plus);
   }
-  // Stores last: a load behind a store would have to wait for it.
-  if (!live) return;
-  void* ro = const_cast<void*>(row_of<X>(a.r.p, b * a.r.b + n * a.r.n));
-  void* yo = const_cast<void*>(row_of<T>(a.y.p, b * a.y.b + n * a.y.n));
+  // Stores last: a load behind a store would have to wait for it.  The new residual goes past
+  // the caches (the next half's block comes first), the normalised rows to their next reader.
 #pragma unroll
-  for (int j = 0; j < CHUNKS; ++j) {
-    const int from = j < CHUNKS - 1 ? 0 : skip;
-    if constexpr (KIND != kPre) r[j].template store<true>(ro, at[j], from);
-    if constexpr (KIND != kGate) {
-      Rounded<T, N> y;
-      y.set(v[j]);
-      y.template store<false>(yo, at[j], from);
+  for (int i = 0; i < ROWS; ++i) {
+    if (!live[i]) continue;
+    void* ro = const_cast<void*>(row_of<X>(a.r.p, b * a.r.b + n[i] * a.r.n));
+    void* yo = const_cast<void*>(row_of<T>(a.y.p, b * a.y.b + n[i] * a.y.n));
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) {
+      const int from = j < CHUNKS - 1 ? 0 : skip;
+      if constexpr (KIND != kPre) r[i][j].template store<true>(ro, at[j], from);
+      if constexpr (KIND != kGate) {
+        Rounded<T, N> y;
+        y.set(v[i][j]);
+        y.template store<false>(yo, at[j], from);
+      }
     }
   }
 }
 
 constexpr int kMinWidth = 8, kMaxWidth = 4 * 1024 * 4;
+constexpr int64_t kAllLanes = 256 * 2048;  // that the chip holds at once
 
-template <class X, class T, int CHUNKS, int KIND>
-hipError_t launch_rows(const ResidualArgs& a, int lanes, hipStream_t s) {
-  const int threads = lanes > kThreads ? lanes : kThreads;
+template <class X, class T, int ROWS, int CHUNKS, int KIND>
+hipError_t launch_rows(const ResidualArgs& a, int lanes, int threads, hipStream_t s) {
   const int64_t per_block = threads / lanes;
-  const int64_t all = (a.rows + per_block - 1) / per_block;
+  const int64_t sample = (a.tokens + per_block * ROWS - 1) / (per_block * ROWS);
+  const int64_t all = ROWS > 1 ? sample * (a.rows / a.tokens) : (a.rows + per_block - 1) / per_block;
   const int64_t bytes = a.rows * a.width *
                         (KIND == kPre    ? kBytes<X> + kBytes<T>
                          : KIND == kGate ? 2 * kBytes<X> + kBytes<T>
@@ -249,12 +279,43 @@ hipError_t launch_rows(const ResidualArgs& a, int lanes, hipStream_t s) {
   for (int64_t first = 0; first < all; first += kMaxBlocks) {
     const dim3 grid((unsigned)std::min(all - first, kMaxBlocks)), block((unsigned)threads);
     if (bytes >= kStreamBytes) {
-      residual_kernel<X, T, CHUNKS, KIND, true><<<grid, block, 0, s>>>(a, lanes, first);
+      residual_kernel<X, T, ROWS, CHUNKS, KIND, true>
+          <<<grid, block, 0, s>>>(a, lanes, first, (int)sample);
     } else {
-      residual_kernel<X, T, CHUNKS, KIND, false><<<grid, block, 0, s>>>(a, lanes, first);
+      residual_kernel<X, T, ROWS, CHUNKS, KIND, false>
+          <<<grid, block, 0, s>>>(a, lanes, first, (int)sample);
     }
   }
   return hipGetLastError();
+}
+
+// Rows a lane holds where they share their vectors.  A row's vectors are up to six times its own
+// bytes, and their loads, though they hit the caches, are what bounds one row a lane.  Measured
+// at 400 MB a call, us, one row -> several: norm_modulate at widths 256 / 768 / 2560 / 8192
+// 101 -> 77 / 100 -> 81 / 93 -> 79 / 99 -> 80 (bf16), 88 -> 73 / 75 -> 72 / 90 -> 76 / 83 -> 76
+// (fp32); gated_residual_norm 79 -> 69 / 81 -> 72 (bf16), 77 -> 68 at 4096 (fp32 stream).  Two
+// rows of three chunks of 8 and a branch no longer fit the registers (480p: 72 -> 91), and a gate
+// alone gains nothing from them (720p: 169 -> 176).
+template <class X, int CHUNKS, int KIND>
+constexpr int kRows = CHUNKS == 1                              ? 4
+                      : CHUNKS == 2                            ? 2
+                      : KIND == kPre || kChunk<X> == 4         ? 2
+                                                               : 1;
+
+template <class X, class T, int CHUNKS, int KIND>
+hipError_t launch_chunks(const ResidualArgs& a, int lanes, hipStream_t s) {
+  constexpr int ROWS = kRows<X, CHUNKS, KIND>;
+  const int threads = lanes > kThreads ? lanes : kThreads;
+  if constexpr (ROWS > 1) {
+    // Where there are vectors, enough rows to fill the chip all the same, and samples long enough
+    // that their last workgroups' idle rows do not count.
+    const bool vectors = a.branch_weight || a.branch_bias || a.gate.p || a.weight || a.bias ||
+                         a.scale.p || a.shift.p;
+    if (vectors && a.gate.n == 0 && a.scale.n == 0 && a.shift.n == 0 &&
+        a.rows * lanes >= ROWS * kAllLanes && a.tokens >= 8 * ROWS * (threads / lanes))
+      return launch_rows<X, T, ROWS, CHUNKS, KIND>(a, lanes, threads, s);
+  }
+  return launch_rows<X, T, 1, CHUNKS, KIND>(a, lanes, threads, s);
 }
 
 template <class X, class T, int KIND>
@@ -265,10 +326,10 @@ hipError_t launch_kind(const ResidualArgs& a, hipStream_t s) {
   while (lanes < chunks && lanes < 64) lanes *= 2;
   while (lanes * 4 < chunks) lanes *= 2;  // up to 4 chunks a lane, then more waves a row
   switch ((chunks + lanes - 1) / lanes) {
-    case 1: return launch_rows<X, T, 1, KIND>(a, lanes, s);
-    case 2: return launch_rows<X, T, 2, KIND>(a, lanes, s);
-    case 3: return launch_rows<X, T, 3, KIND>(a, lanes, s);
-    default: return launch_rows<X, T, 4, KIND>(a, lanes, s);
+    case 1: return launch_chunks<X, T, 1, KIND>(a, lanes, s);
+    case 2: return launch_chunks<X, T, 2, KIND>(a, lanes, s);
+    case 3: return launch_chunks<X, T, 3, KIND>(a, lanes, s);
+    default: return launch_chunks<X, T, 4, KIND>(a, lanes, s);
   }
 }
 

@@ -312,12 +312,16 @@ def test_more_rows_than_one_launch(cuda):
 
 
 @pytest.mark.parametrize("types", [(BF, BF, F32), (F32, FP, F32), (F32, F32, F32)], ids=str)
-def test_large_calls_equal_small_ones(cuda, types):
-    """A call large enough to load past the caches gives each row what a call of its own does."""
-    a = make(32, 1, 40000, 1536, types)
+@pytest.mark.parametrize("batch,tokens,width", [(1, 40000, 1536), (3, 90001, 100), (2, 30011, 520),
+                                                (3, 9001, 700), (2, 9007, 1155), (2, 7001, 2048),
+                                                (1, 9001, 3001), (2, 2001, 8192)])
+def test_large_calls_equal_small_ones(cuda, types, batch, tokens, width):
+    """A call large enough to load past the caches, or to take several rows a lane, gives each
+    row what a call of its own does."""
+    a = make(32, batch, tokens, width, types)
     whole, pre, gate = run_both(a, "layer", "rms"), run_pre(a, "rms", types[1]), run_gate(a, None)
-    for rows in (slice(0, 3), slice(17000, 17009), slice(39995, 40000)):
-        part = {n: v[:, rows] if v.ndim == 3 and v.shape[1] > 1 else v for n, v in a.items()}
+    for rows in (slice(0, 3), slice(tokens // 2, tokens // 2 + 9), slice(tokens - 5, tokens)):
+        part = {n: v[:, rows] if v.ndim == 3 else v for n, v in a.items()}
         got = run_both(part, "layer", "rms")
         assert torch.equal(got[0], whole[0][:, rows]) and torch.equal(got[1], whole[1][:, rows])
         assert torch.equal(run_pre(part, "rms", types[1]), pre[:, rows])
