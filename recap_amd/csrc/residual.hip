@@ -171,10 +171,17 @@ __device__ inline void normalise(int kind, int skip, int width, float eps, int l
   }
 }
 
+// Two rows of three chunks of 8 and a branch take more than the 128 registers that workgroups of
+// 1024 leave a lane.
+template <class X, int ROWS, int CHUNKS, int KIND>
+constexpr bool kWideRows = ROWS > 1 && CHUNKS == 3 && KIND == kBoth && kChunk<X> == 8;
+template <class X, int ROWS, int CHUNKS, int KIND>
+constexpr int kMaxThreads = kWideRows<X, ROWS, CHUNKS, KIND> ? kThreads : 1024;
+
 // ROWS > 1: rows of one sample (`per_sample` workgroups each) that share gate, scale and shift.
 template <class X, class T, int ROWS, int CHUNKS, int KIND, bool STREAM>
-__global__ __launch_bounds__(1024) void residual_kernel(ResidualArgs a, int lanes, int64_t first,
-                                                        int per_sample) {
+__global__ __launch_bounds__((kMaxThreads<X, ROWS, CHUNKS, KIND>)) void residual_kernel(
+    ResidualArgs a, int lanes, int64_t first, int per_sample) {
   constexpr int N = kChunk<X>;
   __shared__ float part[16];
   const int shift = 31 - __clz(lanes);
@@ -293,14 +300,15 @@ hipError_t launch_rows(const ResidualArgs& a, int lanes, int threads, hipStream_
 // bytes, and their loads, though they hit the caches, are what bounds one row a lane.  Measured
 // at 400 MB a call, us, one row -> several: norm_modulate at widths 256 / 768 / 2560 / 8192
 // 101 -> 77 / 100 -> 81 / 93 -> 79 / 99 -> 80 (bf16), 88 -> 73 / 75 -> 72 / 90 -> 76 / 83 -> 76
-// (fp32); gated_residual_norm 79 -> 69 / 81 -> 72 (bf16), 77 -> 68 at 4096 (fp32 stream).  Two
-// rows of three chunks of 8 and a branch no longer fit the registers (480p: 72 -> 91), and a gate
-// alone gains nothing from them (720p: 169 -> 176).
+// (fp32); gated_residual_norm 79 -> 69 / 81 -> 72 (bf16), 77 -> 68 at 4096 (fp32 stream).  A gate
+// alone gains nothing from more than two chunks of 8 (720p: 169 -> 176), and four of them and a
+// branch spill (gate_norm at 2048: 321 -> 596).
 template <class X, int CHUNKS, int KIND>
-constexpr int kRows = CHUNKS == 1                              ? 4
-                      : CHUNKS == 2                            ? 2
-                      : KIND == kPre || kChunk<X> == 4         ? 2
-                                                               : 1;
+constexpr int kRows = CHUNKS == 1                                               ? 4
+                      : CHUNKS == 2                                             ? 2
+                      : KIND == kPre || kChunk<X> == 4                          ? 2
+                      : KIND == kBoth && CHUNKS == 3                            ? 2
+                                                                                : 1;
 
 template <class X, class T, int CHUNKS, int KIND>
 hipError_t launch_chunks(const ResidualArgs& a, int lanes, hipStream_t s) {
@@ -309,11 +317,14 @@ hipError_t launch_chunks(const ResidualArgs& a, int lanes, hipStream_t s) {
   if constexpr (ROWS > 1) {
     // Where there are vectors, enough rows to fill the chip all the same, and samples long enough
     // that their last workgroups' idle rows do not count.
-    const bool vectors = a.branch_weight || a.branch_bias || a.gate.p || a.weight || a.bias ||
-                         a.scale.p || a.shift.p;
-    if (vectors && a.gate.n == 0 && a.scale.n == 0 && a.shift.n == 0 &&
-        a.rows * lanes >= ROWS * kAllLanes && a.tokens >= 8 * ROWS * (threads / lanes))
-      return launch_rows<X, T, ROWS, CHUNKS, KIND>(a, lanes, threads, s);
+    bool several = a.branch_weight || a.branch_bias || a.gate.p || a.weight || a.bias ||
+                   a.scale.p || a.shift.p;
+    several = several && a.gate.n == 0 && a.scale.n == 0 && a.shift.n == 0 &&
+              a.rows * lanes >= ROWS * kAllLanes && a.tokens >= 8 * ROWS * (threads / lanes);
+    // These leave a lane's registers to three waves a SIMD: worth it for fp32 vectors, twice the
+    // loads (480p: 72 -> 66), not for 16-bit ones (63 -> 65).
+    if (kWideRows<X, ROWS, CHUNKS, KIND>) several = several && a.wide_mod && threads == kThreads;
+    if (several) return launch_rows<X, T, ROWS, CHUNKS, KIND>(a, lanes, threads, s);
   }
   return launch_rows<X, T, 1, CHUNKS, KIND>(a, lanes, threads, s);
 }
