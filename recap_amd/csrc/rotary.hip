@@ -8,9 +8,10 @@
 //
 // A lane holds 16 channels of a (token, head) row in two 16-byte chunks, u and u + d/16, so
 // that both pairings stay within the lane; d/16 lanes hold the row.  A wave takes `side` heads
-// of each of its tokens at once (side a power of two that divides the heads) and walks the
-// others, so a token's (cos, sin) are looked up once per wave.
+// of each of its tokens at once (side a power of two) and walks the others, so a token's
+// (cos, sin) are looked up once per wave.
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.hpp"
 #include "rows.hpp"
@@ -87,19 +88,26 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, int64_t 
     if (t.weight) load16<T>(t.weight, a.wide_weight, 8 * u, D / 2, w);
   }
 
-  const uint16_t* src = t.in + b * t.in_b + n * t.in_n + hl * t.in_h + 8 * u;
+  // In the last step a lane's head may be past the heads: it loads the last one and stores none.
+  const int steps = (t.heads + side - 1) / side, left = t.heads - (steps - 1) * side;
+  const int hl_last = min(hl, left - 1);
+  const uint16_t* src = t.in + b * t.in_b + n * t.in_n + 8 * u;
+  const uint16_t* src_last = src + hl_last * t.in_h;
+  src += hl * t.in_h;
   uint16_t* dst = t.out + b * t.out_b + n * t.out_n + hl * t.out_h + 8 * u;
-  const int steps = t.heads / side;
+  const auto there = [&](int step) { return step < steps - 1 || hl < left; };
   u32x4 raw[kBatch][2];
-  const auto fetch = [&](int first) {
+  const auto fetch = [&](int first, auto past) {  // past: past the caches
 #pragma unroll
     for (int j = 0; j < kBatch; ++j)
       if (first + j < steps) {
-        const uint16_t* p = src + (int64_t)(first + j) * side * t.in_h;
-        raw[j][0] = load_words4<STREAM && D == 128>(p);
-        raw[j][1] = load_words4<STREAM && D == 128>(p + D / 2);
+        const uint16_t* p = (first + j < steps - 1 ? src : src_last) +
+                            (int64_t)(first + j) * side * t.in_h;
+        raw[j][0] = load_words4<decltype(past)::value>(p);
+        raw[j][1] = load_words4<decltype(past)::value>(p + D / 2);
       }
   };
+  const std::bool_constant<STREAM && D == 128> past;
   const auto widen = [&](int j, float (&x)[16]) {
 #pragma unroll
     for (int k = 0; k < 2; ++k)
@@ -113,20 +121,26 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, int64_t 
   if (NORM == kRotaryRmsAll) {
     float sq = 0.0f;
     for (int first = 0; first < steps; first += kBatch) {
-      fetch(first);
+      if (steps > kBatch) {
+        fetch(first, std::false_type());  // read again below, from the caches
+      } else {
+        fetch(first, past);
+      }
 #pragma unroll
       for (int j = 0; j < kBatch; ++j)
         if (first + j < steps) {
           float x[16];
           widen(j, x);
+          float part = 0.0f;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) sq = fmaf(x[e], x[e], sq);
+          for (int e = 0; e < 16; ++e) part = fmaf(x[e], x[e], part);
+          sq += there(first + j) ? part : 0.0f;
         }
     }
     all = 1.0f / sqrtf(row_sum(sq, kLanes * side, nullptr) / (float)(t.heads * D) + a.eps);
   }
   for (int first = 0; first < steps; first += kBatch) {
-    if (NORM != kRotaryRmsAll || steps > kBatch) fetch(first);
+    if (NORM != kRotaryRmsAll || steps > kBatch) fetch(first, past);
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       if (first + j >= steps) break;
@@ -149,7 +163,9 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, int64_t 
       }
       // The head's place in the weights: those over a head's channels are the same for all.
       const unsigned at =
-          8 * u + (NORM == kRotaryRmsAll ? (unsigned)((first + j) * side + hl) * D : 0);
+          8 * u + (NORM == kRotaryRmsAll
+                       ? (unsigned)((first + j) * side + (there(first + j) ? hl : hl_last)) * D
+                       : 0);
       if (NORM == kRotaryRmsAll && t.weight) load16<T>(t.weight, a.wide_weight, at, D / 2, w);
       if (NORM != kRotaryNone) {
 #pragma unroll
@@ -173,7 +189,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, int64_t 
         lo[e] = pack2<T>(y[2 * e], y[2 * e + 1]);
         hi[e] = pack2<T>(y[8 + 2 * e], y[8 + 2 * e + 1]);
       }
-      if (live) {
+      if (live && there(first + j)) {
         uint16_t* o = dst + (int64_t)(first + j) * side * t.out_h;
         store_words4<STREAM>(o, lo);
         store_words4<STREAM>(o + D / 2, hi);
@@ -189,8 +205,14 @@ hipError_t launch(const RotaryArgs& a, hipStream_t s) {
   int64_t waves = 1, values = 0;  // rows of d
   for (int i = 0; i < a.tensors; ++i) {
     // Each tensor by its own heads, so that q's sums do not depend on k's.
-    int side = 1;
-    while (side < kRows && a.x[i].heads % (2 * side) == 0) side *= 2;
+    // Heads side by side read long pieces of a projection, steps in flight together keep a wave
+    // busy: as many side by side as leave three steps and no more than an eighth of the lanes
+    // without a head.  At 400 MB a call, us: 24 heads of 128 by 8 / by 4 65 / 70, 48 of 64 by
+    // 16 / by 8 70 / 76, 15 of 64 by 16 / by 8 / by 4 / by 1 102 / 73 / 71 / 86.
+    const int heads = a.x[i].heads;
+    const auto steps = [&](int n) { return (heads + n - 1) / n; };
+    int side = kRows;
+    while (side > 1 && (steps(side) < 3 || steps(side) * side * 8 > heads * 9)) side /= 2;
     b.x[i].side = side;
     values += a.rows * a.x[i].heads;
     waves = std::max(waves, (a.rows + kRows / side - 1) / (kRows / side));
