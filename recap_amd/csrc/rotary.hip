@@ -10,6 +10,13 @@
 // that both pairings stay within the lane; d/16 lanes hold the row.  A wave takes `side` heads
 // of each of its tokens at once (side a power of two) and walks the others, so a token's
 // (cos, sin) are looked up once per wave.
+//
+// Bound by memory: 4 bytes and 3 to 10 flop an element; by counters the kernel moves Q and K once
+// in and once out.  24 heads of 128 at 119,056 tokens with RMS norm take 474 us, 6.2 TB/s of the
+// 6.5 that a copy kernel reaches past the caches (495 us where the outputs are put head by head);
+// 12 heads with a norm over all of them at 32,760 tokens 68 us, 5.9; 48 heads of 64 at 45,106
+// tokens with LayerNorm 192 us, 5.8: a load covers half a line of a head of 64, so those go
+// through the caches.  One head alone (90 us for 400 MB) leaves too few loads in flight.
 #include <algorithm>
 #include <type_traits>
 

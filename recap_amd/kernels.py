@@ -641,12 +641,11 @@ def _choice(table: dict, value, what: str) -> int:
     return table[value]
 
 
-def _spec(t: torch.Tensor | None):
-    """What a call's checks look at of a tensor, hashable: everything but its address."""
-    if t is None:
-        return None
-    return (t.shape, t.stride(), t.dtype, t.device,
-            t.requires_grad and torch.is_grad_enabled())
+def _specs(tensors) -> tuple:
+    """What a call's checks look at of its tensors, hashable: everything but their addresses."""
+    grad = torch.is_grad_enabled()
+    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.device,
+                                          grad and t.requires_grad) for t in tensors])
 
 
 def _together(specs: dict) -> torch.device:
@@ -859,19 +858,20 @@ def qk_rotary(q: torch.Tensor, k: torch.Tensor | None = None, axes=None, *, offs
     themselves, or views into a longer sequence (a text stream's part of it)."""
     vectors = (q_weight, q_bias, k_weight, k_bias)
     axes = None if axes is None else tuple(axes)
-    plan = _qk_plan(_spec(q), _spec(k), None if axes is None else tuple(map(_spec, axes)),
-                    int(offset), pairing, norm, tuple(map(_spec, vectors)))
+    specs = _specs((q, k, *vectors, *(axes or ())))
+    plan = _qk_plan(specs[0], specs[1], None if axes is None else specs[6:], int(offset), pairing,
+                    norm, specs[2:6])
     if k is None and k_out is not None:
         raise ValueError("k_out needs a k")
     if q_out is not None or k_out is not None:
         inputs = {"q": q, "k": k, "q_weight": q_weight, "q_bias": q_bias, "k_weight": k_weight,
                   "k_bias": k_bias, **{f"axis {i}": t for i, t in enumerate(axes or ())}}
-        _together({"q": _spec(q), "q_out": _spec(q_out), "k_out": _spec(k_out)})
+        _together(dict(zip(("q", "q_out", "k_out"), _specs((q, q_out, k_out)))))
         for name, x, out in (("q", q, q_out), ("k", k, k_out)):
             if out is None:
                 continue
             _check_output(f"{name}_out", out, x.shape, x.dtype, inputs, name)
-            if not _aligned_rows(_spec(out)) or out.data_ptr() % 16:
+            if not _aligned_rows((out.shape, out.stride())) or out.data_ptr() % 16:
                 raise ValueError(f"{name}_out must have 16-byte aligned rows")
         if q_out is not None and k_out is not None:
             _check_output("k_out", k_out, k.shape, k.dtype, {"q_out": q_out}, "")
@@ -974,8 +974,9 @@ def _residual_call(name: str, names, x, dtype, branch, mods, vectors, norms, eps
                    outs) -> tuple[torch.Tensor, ...]:
     """Checks and launch of the residual-stream calls.  ``outs``: (name, given tensor or None,
     type, the input it may be)."""
-    plan = _residual_plan(names, dtype, _spec(x), _spec(branch), tuple(map(_spec, mods)),
-                          tuple(map(_spec, vectors)), norms)
+    specs = _specs((x, branch, *mods, *vectors))
+    last = 2 + len(mods)
+    plan = _residual_plan(names, dtype, specs[0], specs[1], specs[2:last], specs[last:], norms)
     made = []
     for out_name, out, out_dtype, same in outs:
         if out is None:
@@ -984,7 +985,7 @@ def _residual_call(name: str, names, x, dtype, branch, mods, vectors, norms, eps
             inputs = {"x": x, "branch": branch, **dict(zip(names[0], mods)),
                       **dict(zip(names[1], vectors)),
                       **{f"the other output ({o[0]})": m for o, m in zip(outs, made)}}
-            _together({"x": _spec(x), out_name: _spec(out)})
+            _together(dict(zip(("x", out_name), _specs((x, out)))))
             _check_output(out_name, out, x.shape, out_dtype, inputs, same)
         made.append(out)
     if x.numel() == 0:
