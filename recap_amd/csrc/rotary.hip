@@ -61,15 +61,11 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, int64_t 
   const unsigned r32 = (unsigned)(live ? row : a.rows - 1);
   const unsigned b = r32 / (unsigned)a.tokens, n = r32 - b * (unsigned)a.tokens;
 
-  // (cos, sin) of the lane's 8 frequencies; identity outside the video.
+  // (cos, sin) of the lane's 8 frequencies at a token of the video.
   float c[8], s[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    c[e] = 1.0f;
-    s[e] = 0.0f;
-  }
   const int64_t v64 = (int64_t)n - a.offset;
-  if (v64 >= 0 && v64 < a.video) {
+  const bool turned = v64 >= 0 && v64 < a.video;
+  if (turned) {
     const unsigned v = (unsigned)v64, wd = a.axis[2].length, ht = a.axis[1].length;
     const unsigned line = v / wd, x = v - line * wd, z = line / ht, y = line - z * ht;
     const int p0 = a.axis[0].pairs, p1 = p0 + a.axis[1].pairs;
@@ -184,11 +180,16 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, int64_t 
           for (int e = 0; e < 16; ++e) x[e] += bias[e];
         }
       }
+      // The others keep their values, also beside an infinity.
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int p = HALVES ? e : 2 * e, q = HALVES ? e + 8 : 2 * e + 1;
-        y[p] = x[p] * c[e] - x[q] * s[e];
-        y[q] = x[q] * c[e] + x[p] * s[e];
+      for (int e = 0; e < 16; ++e) y[e] = x[e];
+      if (turned) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int p = HALVES ? e : 2 * e, q = HALVES ? e + 8 : 2 * e + 1;
+          y[p] = x[p] * c[e] - x[q] * s[e];
+          y[q] = x[q] * c[e] + x[p] * s[e];
+        }
       }
       u32x4 lo, hi;
 #pragma unroll

@@ -168,6 +168,24 @@ def test_values_that_are_not_numbers(cuda):
         assert torch.isnan(got[0, 0, 2]).any() and not torch.isfinite(got[0, 1, 4]).all()
 
 
+@pytest.mark.parametrize("pairing", ["interleaved", "halves"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_tokens_outside_the_grid_keep_their_values(cuda, d, pairing):
+    """Text tokens without a norm come out bit for bit, whatever stands beside a value: an
+    infinity and a NaN stay in their own channel; a call without axes copies."""
+    a = make(15, 2, 3, 40, d)
+    q = a["q"]
+    q[0, 1, 2, 8] = float("inf")
+    q[1, 0, 3, 17] = float("nan")
+    q[0, 2, 39, d - 1] = float("-inf")
+    q[1, 2, 38, 0] = -0.0
+    axes = recap_amd.rotary_axes((2, 3, 5), CHANNELS[d], device=cuda)
+    got = K.qk_rotary(q, None, axes, offset=5, pairing=pairing)[0]
+    for rows in (slice(0, 5), slice(35, 40)):
+        assert torch.equal(got[:, :, rows].view(torch.int16), q[:, :, rows].view(torch.int16))
+    assert torch.equal(K.qk_rotary(q, pairing=pairing)[0].view(torch.int16), q.view(torch.int16))
+
+
 def test_streams_and_graph(cuda):
     axes = recap_amd.rotary_axes((3, 20, 20), CHANNELS[128], device=cuda)
     a = make(8, 1, 6, 1250, 128, norm="rms_all")
