@@ -36,7 +36,7 @@ extern "C" {
 #define RECAP_ABI_VERSION 10
 
 enum { RECAP_OK = 0, RECAP_EINVAL = 1, RECAP_EUNSUPPORTED = 2, RECAP_EHIP = 3 };
-enum { RECAP_F16 = 1, RECAP_BF16 = 2, RECAP_F32 = 3 };  /* RECAP_F32: residual stream only */
+enum { RECAP_F16 = 1, RECAP_BF16 = 2, RECAP_F32 = 3 };  /* F32: around the attention call only */
 enum { RECAP_NORM_NONE = 0, RECAP_NORM_RMS = 1, RECAP_NORM_LAYER = 2, RECAP_NORM_RMS_ALL = 3 };
 enum { RECAP_PAIRS_INTERLEAVED = 0, RECAP_PAIRS_HALVES = 1 };
 enum { RECAP_CLOSURE_ROT = 1, RECAP_CLOSURE_CVK = 2, RECAP_CLOSURE_SCATTER = 4 };
@@ -457,20 +457,22 @@ int recap_bank_copy_async(void* dst, const void* src, int64_t bytes, void* strea
  *    weight_dtype is the tensors' type or RECAP_F32.
  *  - table_t, table_h, table_w (fp32 [lengths[i], pairs[i], 2], device memory, 8-byte
  *    aligned): the (cos, sin) of axis i (time, height, width) at each position; pairs[0] +
- *    pairs[1] + pairs[2] = dim / 2, and an axis of no pairs may have a NULL table.  Token offset + v with
- *    0 <= v < lengths[0] * lengths[1] * lengths[2] sits at (v / (H * W), v / W % H, v % W);
- *    the other tokens (text) are not rotated.  Frequency i rotates channels (2i, 2i + 1)
- *    (RECAP_PAIRS_INTERLEAVED) or (i, i + dim / 2) (RECAP_PAIRS_HALVES).  lengths and pairs (host arrays
- *    of 3) NULL: no rotation.
+ *    pairs[1] + pairs[2] = dim / 2, and an axis of no pairs may have a NULL table.  Token
+ *    offset + v with 0 <= v < lengths[0] * lengths[1] * lengths[2] sits at (v / (H * W),
+ *    v / W % H, v % W); the other tokens (text) are not rotated.  Frequency i rotates channels
+ *    (2i, 2i + 1) (RECAP_PAIRS_INTERLEAVED) or (i, i + dim / 2) (RECAP_PAIRS_HALVES).  lengths
+ *    and pairs (host arrays of 3) NULL: no rotation.
  *  - k may be NULL.  An output may be its own input, and overlaps nothing else.
- * No weights, sums or angles are kept from call to call.  Covers the query/key norm and the rotary embedding
- * before operator.attend in the model processors, recap/models/hunyuan.py:79-154. */
+ * Statistics and products are fp32 (a norm's rows stay below about 1e17), rounded once.  Covers
+ * the query/key norm and the rotary embedding before operator.attend in the model processors,
+ * recap/models/hunyuan.py:79-154. */
 int recap_qk_rotary(const void* q, const void* k, int dtype, int64_t batch, int64_t tokens,
                     int64_t dim, int64_t q_heads, int64_t k_heads, int64_t q_stride_b,
                     int64_t q_stride_h, int64_t q_stride_n, int64_t k_stride_b,
                     int64_t k_stride_h, int64_t k_stride_n, const float* table_t,
                     const float* table_h, const float* table_w, const int64_t* lengths,
-                    const int64_t* pairs, int64_t offset, int pairing, int norm, const void* q_weight, const void* q_bias, const void* k_weight,
+                    const int64_t* pairs, int64_t offset, int pairing, int norm,
+                    const void* q_weight, const void* q_bias, const void* k_weight,
                     const void* k_bias, int weight_dtype, float eps, void* q_out,
                     int64_t qo_stride_b, int64_t qo_stride_h, int64_t qo_stride_n, void* k_out,
                     int64_t ko_stride_b, int64_t ko_stride_h, int64_t ko_stride_n, void* stream);
@@ -489,9 +491,9 @@ int recap_qk_rotary(const void* q, const void* k, int dtype, int64_t batch, int6
  *  - Strides are in elements, channels have unit stride, and nothing needs more than its
  *    element's alignment.  residual_out may be x and out may be branch (for
  *    recap_norm_modulate, x); outputs overlap nothing else.
- * Statistics and products are fp32; each output is rounded once.  Covers the modulated norms
- * and gated residuals of the transformer blocks whose processors call operator.attend,
- * recap/models/hunyuan.py:79-154. */
+ * Statistics and products are fp32 (a norm's rows stay below about 1e17); each output is
+ * rounded once.  Covers the modulated norms and gated residuals of the transformer blocks
+ * whose processors call operator.attend, recap/models/hunyuan.py:79-154. */
 int recap_norm_modulate(const void* x, int x_dtype, int64_t batch, int64_t tokens,
                         int64_t width, int64_t x_stride_b, int64_t x_stride_n,
                         const void* scale, int64_t scale_stride_b, int64_t scale_stride_n,

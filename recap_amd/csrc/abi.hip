@@ -1069,7 +1069,8 @@ int recap_qk_rotary(const void* q, const void* k, int dtype, int64_t batch, int6
                     int64_t q_stride_h, int64_t q_stride_n, int64_t k_stride_b,
                     int64_t k_stride_h, int64_t k_stride_n, const float* table_t,
                     const float* table_h, const float* table_w, const int64_t* lengths,
-                    const int64_t* pairs, int64_t offset, int pairing, int norm, const void* q_weight, const void* q_bias, const void* k_weight,
+                    const int64_t* pairs, int64_t offset, int pairing, int norm,
+                    const void* q_weight, const void* q_bias, const void* k_weight,
                     const void* k_bias, int weight_dtype, float eps, void* q_out,
                     int64_t qo_stride_b, int64_t qo_stride_h, int64_t qo_stride_n, void* k_out,
                     int64_t ko_stride_b, int64_t ko_stride_h, int64_t ko_stride_n,

@@ -292,7 +292,8 @@ template <class X, class T, int ROWS, int CHUNKS, int KIND>
 hipError_t launch_rows(const ResidualArgs& a, int lanes, int threads, hipStream_t s) {
   const int64_t per_block = threads / lanes;
   const int64_t sample = (a.tokens + per_block * ROWS - 1) / (per_block * ROWS);
-  const int64_t all = ROWS > 1 ? sample * (a.rows / a.tokens) : (a.rows + per_block - 1) / per_block;
+  const int64_t all =
+      ROWS > 1 ? sample * (a.rows / a.tokens) : (a.rows + per_block - 1) / per_block;
   const int64_t bytes = a.rows * a.width *
                         (KIND == kPre    ? kBytes<X> + kBytes<T>
                          : KIND == kGate ? 2 * kBytes<X> + kBytes<T>
