@@ -8,7 +8,7 @@
 // Bound by memory: 4 to 12 bytes and 2 to 15 flop an element, and by counters the kernels move
 // those bytes and no more.  A copy kernel that goes past the caches reaches 6.5 TB/s; here 360 MB
 // of bf16 with a gate (720p, 118,800 x 1536) take 169 us, 6.5 TB/s; gate and norm (480p,
-// 32,760 x 1536) 66 us, 6.1; gate and norm with a norm of the branch (118,800 x 2048) 335 us, 5.8.
+// 32,760 x 1536) 66 us, 6.1; gate and norm with a norm of the branch (118,800 x 2048) 321 us, 6.1.
 // What the rest goes to: the loads of the row's vectors, which hit the caches, and with a norm of
 // the branch the second sum and the four waves a SIMD that its registers leave.
 //
@@ -17,6 +17,7 @@
 // and 216 us where one takes 175.  Vectors staged in LDS for a workgroup's rows were slower too
 // (480p: 83 us against 72): their barrier holds four waves together.
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.hpp"
 #include "rows.hpp"
@@ -193,7 +194,8 @@ template <class X, int ROWS, int CHUNKS, int KIND>
 constexpr int kMaxThreads = kWideRows<X, ROWS, CHUNKS, KIND> ? kThreads : 1024;
 
 // ROWS > 1: rows of one sample (`per_sample` workgroups each) that share gate, scale and shift.
-template <class X, class T, int ROWS, int CHUNKS, int KIND, bool STREAM>
+// STREAM: 1 loads the rows past the caches, 2 also stores the normalised ones past them.
+template <class X, class T, int ROWS, int CHUNKS, int KIND, int STREAM>
 __global__ __launch_bounds__((kMaxThreads<X, ROWS, CHUNKS, KIND>)) void residual_kernel(
     ResidualArgs a, int lanes, int64_t first, int per_sample) {
   constexpr int N = kChunk<X>;
@@ -236,14 +238,14 @@ __global__ __launch_bounds__((kMaxThreads<X, ROWS, CHUNKS, KIND>)) void residual
   for (int i = 0; i < ROWS; ++i) {
     const void* x = row_of<X>(a.x.p, b * a.x.b + n[i] * a.x.n);
 #pragma unroll
-    for (int j = 0; j < CHUNKS; ++j) load_chunk<X, STREAM>(x, at[j], v[i][j]);
+    for (int j = 0; j < CHUNKS; ++j) load_chunk<X, (STREAM > 0)>(x, at[j], v[i][j]);
   }
   if constexpr (KIND != kPre) {
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       const void* added = row_of<T>(a.branch.p, b * a.branch.b + n[i] * a.branch.n);
 #pragma unroll
-      for (int j = 0; j < CHUNKS; ++j) load_chunk<T, STREAM>(added, at[j], f[i][j]);
+      for (int j = 0; j < CHUNKS; ++j) load_chunk<T, (STREAM > 0)>(added, at[j], f[i][j]);
     }
     if (a.post != kNormNone) normalise(a.post, skip, a.width, a.eps, lanes, part, f);
     combine<T>(a.branch_weight, a.wide_weight, 0, at, f, times);
@@ -266,7 +268,8 @@ __global__ __launch_bounds__((kMaxThreads<X, ROWS, CHUNKS, KIND>)) void residual
     combine<T>(a.shift.p, a.wide_mod, b * a.shift.b + n[0] * a.shift.n, at, v, plus);
   }
   // Stores last: a load behind a store would have to wait for it.  The new residual goes past
-  // the caches (the next half's block comes first), the normalised rows to their next reader.
+  // the caches (the next half's block comes first), the normalised rows to their next reader,
+  // the next projection, unless there are more than the caches hold.
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
     if (!live[i]) continue;
@@ -279,7 +282,7 @@ __global__ __launch_bounds__((kMaxThreads<X, ROWS, CHUNKS, KIND>)) void residual
       if constexpr (KIND != kGate) {
         Rounded<T, N> y;
         y.set(v[i][j]);
-        y.template store<false>(yo, at[j], from);
+        y.template store<(STREAM > 1)>(yo, at[j], from);
       }
     }
   }
@@ -287,6 +290,11 @@ __global__ __launch_bounds__((kMaxThreads<X, ROWS, CHUNKS, KIND>)) void residual
 
 constexpr int kMinWidth = 8, kMaxWidth = 4 * 1024 * 4;
 constexpr int64_t kAllLanes = 256 * 2048;  // that the chip holds at once
+
+// Normalised rows of this many bytes or more go past the caches.  The chain of kStreamBytes in us,
+// through them -> past them: 101 MB of rows 583 -> 605, 201 MB 1,156 -> 1,188, 276 MB
+// 1,747 -> 1,753, 365 MB 2,250 -> 2,237; 487 MB (118,800 x 2048), the call alone, 335 -> 321.
+constexpr int64_t kPastBytes = int64_t(320) << 20;
 
 template <class X, class T, int ROWS, int CHUNKS, int KIND>
 hipError_t launch_rows(const ResidualArgs& a, int lanes, int threads, hipStream_t s) {
@@ -298,14 +306,19 @@ hipError_t launch_rows(const ResidualArgs& a, int lanes, int threads, hipStream_
                         (KIND == kPre    ? kBytes<X> + kBytes<T>
                          : KIND == kGate ? 2 * kBytes<X> + kBytes<T>
                                          : 2 * kBytes<X> + 2 * kBytes<T>);
+  const bool past = KIND != kGate && a.rows * a.width * kBytes<T> >= kPastBytes;
   for (int64_t first = 0; first < all; first += kMaxBlocks) {
     const dim3 grid((unsigned)std::min(all - first, kMaxBlocks)), block((unsigned)threads);
-    if (bytes >= kStreamBytes) {
-      residual_kernel<X, T, ROWS, CHUNKS, KIND, true>
+    const auto launch = [&](auto stream) {
+      residual_kernel<X, T, ROWS, CHUNKS, KIND, decltype(stream)::value>
           <<<grid, block, 0, s>>>(a, lanes, first, (int)sample);
+    };
+    if (past) {
+      launch(std::integral_constant<int, KIND != kGate ? 2 : 1>());
+    } else if (bytes >= kStreamBytes) {
+      launch(std::integral_constant<int, 1>());
     } else {
-      residual_kernel<X, T, ROWS, CHUNKS, KIND, false>
-          <<<grid, block, 0, s>>>(a, lanes, first, (int)sample);
+      launch(std::integral_constant<int, 0>());
     }
   }
   return hipGetLastError();

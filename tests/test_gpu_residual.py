@@ -313,7 +313,7 @@ def test_more_rows_than_one_launch(cuda):
 
 @pytest.mark.parametrize("types", [(BF, BF, F32), (F32, FP, F32), (F32, F32, F32)], ids=str)
 @pytest.mark.parametrize("batch,tokens,width", [(1, 40000, 1536), (3, 90001, 100), (2, 30011, 520),
-                                                (3, 9001, 700), (2, 9007, 1155), (2, 7001, 2048),
+                                                (3, 9001, 700), (2, 9007, 1155), (2, 45001, 2048),
                                                 (1, 9001, 3001), (2, 2001, 8192)])
 def test_large_calls_equal_small_ones(cuda, types, batch, tokens, width):
     """A call large enough to load past the caches, or to take several rows a lane, gives each
