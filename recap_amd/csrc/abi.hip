@@ -1064,6 +1064,28 @@ int recap_bank_copy_async(void* dst, const void* src, int64_t bytes, void* strea
 
 // Around the attention call ---------------------------------------------------------------
 
+namespace {
+
+// An output of qk_rotary: check_qkv, and no two of its elements at one address (dimensions by
+// their strides, each at least what those below it span; the sizes bound a sum of products of
+// 64-bit values by 2^127).
+int check_qk_out(const char* name, const void* p, int64_t batch, int64_t heads, int64_t tokens,
+                 int64_t dim, int64_t sb, int64_t sh, int64_t sn) {
+  CHECK(check_qkv(name, p, batch, heads, sb, sh, sn));
+  std::pair<int64_t, int64_t> steps[] = {{sb, batch}, {sh, heads}, {sn, tokens}};
+  std::sort(std::begin(steps), std::end(steps));
+  __int128 extent = dim;
+  for (const auto& [stride, size] : steps) {
+    if (size == 1) continue;
+    REQUIRE(stride >= extent, "%s strides (%lld, %lld, %lld) let rows overlap", name,
+            (long long)sb, (long long)sh, (long long)sn);
+    extent += (__int128)(size - 1) * stride;
+  }
+  return RECAP_OK;
+}
+
+}  // namespace
+
 int recap_qk_rotary(const void* q, const void* k, int dtype, int64_t batch, int64_t tokens,
                     int64_t dim, int64_t q_heads, int64_t k_heads, int64_t q_stride_b,
                     int64_t q_stride_h, int64_t q_stride_n, int64_t k_stride_b,
@@ -1078,10 +1100,11 @@ int recap_qk_rotary(const void* q, const void* k, int dtype, int64_t batch, int6
   CHECK(check_common(dtype, dim));
   REQUIRE(tokens >= 1 && tokens <= INT32_MAX, "tokens %lld outside 1..2^31-1", (long long)tokens);
   CHECK(check_qkv("q", q, batch, q_heads, q_stride_b, q_stride_h, q_stride_n));
-  CHECK(check_qkv("q_out", q_out, batch, q_heads, qo_stride_b, qo_stride_h, qo_stride_n));
   REQUIRE(batch <= INT32_MAX / tokens, "batch * tokens exceeds 2^31-1");
   REQUIRE(q_heads <= kRotaryMaxHeads, "q_heads %lld exceeds %d", (long long)q_heads,
           kRotaryMaxHeads);
+  CHECK(check_qk_out("q_out", q_out, batch, q_heads, tokens, dim, qo_stride_b, qo_stride_h,
+                     qo_stride_n));
   REQUIRE((k == nullptr) == (k_out == nullptr), "k and k_out go together");
   RotaryArgs a{};
   a.x[0] = {static_cast<const uint16_t*>(q), q_stride_b, q_stride_h, q_stride_n,
@@ -1090,9 +1113,10 @@ int recap_qk_rotary(const void* q, const void* k, int dtype, int64_t batch, int6
   a.tensors = 1;
   if (k != nullptr) {
     CHECK(check_qkv("k", k, batch, k_heads, k_stride_b, k_stride_h, k_stride_n));
-    CHECK(check_qkv("k_out", k_out, batch, k_heads, ko_stride_b, ko_stride_h, ko_stride_n));
     REQUIRE(k_heads <= kRotaryMaxHeads, "k_heads %lld exceeds %d", (long long)k_heads,
             kRotaryMaxHeads);
+    CHECK(check_qk_out("k_out", k_out, batch, k_heads, tokens, dim, ko_stride_b, ko_stride_h,
+                       ko_stride_n));
     a.x[1] = {static_cast<const uint16_t*>(k), k_stride_b, k_stride_h, k_stride_n,
               static_cast<uint16_t*>(k_out), ko_stride_b, ko_stride_h, ko_stride_n, k_weight,
               k_bias, (int)k_heads};

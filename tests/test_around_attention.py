@@ -167,6 +167,21 @@ def test_qk_rotary_entry_refusals(bad):
         _lib.call("recap_qk_rotary", *a.values(), None)
 
 
+@pytest.mark.parametrize("bad", [
+    dict(qos=0), dict(kos=0), dict(qos=32), dict(kon=64), dict(qon=64), dict(qos=64, qon=72),
+    dict(batch=2, qob=0, kob=30 * 128), dict(batch=2, qob=30 * 128, kob=0),
+    dict(batch=2, qob=29 * 128, kob=30 * 128), dict(batch=2, qob=64, kob=30 * 128),
+    dict(batch=3, qob=1 << 62, kob=1 << 62, qos=1 << 62)])
+def test_qk_rotary_entry_refuses_outputs_that_share_memory(bad):
+    """Two (token, head) rows of an output at one address would be written by two waves."""
+    import ctypes
+    a = {**GOOD_QK, **bad}
+    for name in ("lengths", "pairs"):
+        a[name] = (ctypes.c_int64 * 3)(*a[name])
+    with pytest.raises(ValueError, match="overlap"):
+        _lib.call("recap_qk_rotary", *a.values(), None)
+
+
 GOOD_ROWS = dict(x=16, xt=_lib.RECAP_F32, batch=2, tokens=5, width=24, xb=120, xn=24, branch=16,
                  t=_lib.RECAP_BF16, bb=120, bn=24, gate=16, gb=24, gn=0, scale=16, sb=24, sn=0,
                  shift=16, hb=24, hn=0, mt=_lib.RECAP_F32, bw=16, bbias=16, w=16, bias=16,
