@@ -67,12 +67,13 @@ int check_tokens(int64_t n_tokens, int64_t n_video) {
   return RECAP_OK;
 }
 
+// [batch][heads][tokens][dim] for 16-byte accesses; least_sn 0: expanded tokens are read as well.
 int check_qkv(const char* name, const void* p, int64_t batch, int64_t heads, int64_t sb,
-              int64_t sh, int64_t sn) {
+              int64_t sh, int64_t sn, int64_t least_sn = 8) {
   REQUIRE(p != nullptr, "%s is NULL", name);
   REQUIRE(batch >= 1 && heads >= 1, "%s: batch and heads must be positive", name);
   REQUIRE(aligned16(p), "%s is not 16-byte aligned", name);
-  REQUIRE(sb % 8 == 0 && sh % 8 == 0 && sn % 8 == 0 && sb >= 0 && sh >= 0 && sn > 0,
+  REQUIRE(sb % 8 == 0 && sh % 8 == 0 && sn % 8 == 0 && sb >= 0 && sh >= 0 && sn >= least_sn,
           "%s strides (%lld, %lld, %lld) must be non-negative multiples of 8 elements", name,
           (long long)sb, (long long)sh, (long long)sn);
   return RECAP_OK;
@@ -1099,7 +1100,7 @@ int recap_qk_rotary(const void* q, const void* k, int dtype, int64_t batch, int6
                     void* stream) {
   CHECK(check_common(dtype, dim));
   REQUIRE(tokens >= 1 && tokens <= INT32_MAX, "tokens %lld outside 1..2^31-1", (long long)tokens);
-  CHECK(check_qkv("q", q, batch, q_heads, q_stride_b, q_stride_h, q_stride_n));
+  CHECK(check_qkv("q", q, batch, q_heads, q_stride_b, q_stride_h, q_stride_n, 0));
   REQUIRE(batch <= INT32_MAX / tokens, "batch * tokens exceeds 2^31-1");
   REQUIRE(q_heads <= kRotaryMaxHeads, "q_heads %lld exceeds %d", (long long)q_heads,
           kRotaryMaxHeads);
@@ -1112,7 +1113,7 @@ int recap_qk_rotary(const void* q, const void* k, int dtype, int64_t batch, int6
             q_bias, (int)q_heads};
   a.tensors = 1;
   if (k != nullptr) {
-    CHECK(check_qkv("k", k, batch, k_heads, k_stride_b, k_stride_h, k_stride_n));
+    CHECK(check_qkv("k", k, batch, k_heads, k_stride_b, k_stride_h, k_stride_n, 0));
     REQUIRE(k_heads <= kRotaryMaxHeads, "k_heads %lld exceeds %d", (long long)k_heads,
             kRotaryMaxHeads);
     CHECK(check_qk_out("k_out", k_out, batch, k_heads, tokens, dim, ko_stride_b, ko_stride_h,

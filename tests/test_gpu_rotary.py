@@ -137,6 +137,23 @@ def test_layouts(cuda, d, norm):
         run(a, axes, norm=norm, offset=off, q_out=view)
 
 
+@pytest.mark.parametrize("norm", [None, "rms_all"])
+@pytest.mark.parametrize("dim", [0, 1, 2])
+def test_expanded_inputs(cuda, dim, norm):
+    """q and k with one batch, head or token expanded to all (a stride of 0) are read in place,
+    also where another argument needs a copy."""
+    a = make(16, 2, 3, 47, 64, norm=norm)
+    axes = recap_amd.rotary_axes((2, 4, 5), CHANNELS[64], device=cuda)
+    whole = {m: v.narrow(dim, 0, 1).expand_as(v) if len(m) == 1 else v for m, v in a.items()}
+    assert whole["q"].stride(dim) == 0
+    want = run({m: v.contiguous() for m, v in whole.items()}, axes, norm=norm, offset=5)
+    got = run(whole, axes, norm=norm, offset=5)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    apart = [torch.stack((t, t), -1)[..., 0] for t in axes]
+    got = run(whole, apart, norm=norm, offset=5)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 def test_empty_and_refused(cuda):
     x = torch.zeros(0, 2, 5, 64, dtype=BF, device=cuda)
     assert K.qk_rotary(x, x)[1].shape == x.shape
