@@ -2,8 +2,9 @@
 // (token) of the residual stream at a time:
 //   r = x + gate * post(branch)                 post: none, RMS norm or LayerNorm
 //   y = norm(r) * (1 + scale) + shift           norm: none, RMS norm or LayerNorm
-// without a branch r = x.  Statistics, sums and products are fp32; r and y are each rounded
-// once, to their own type, and y is taken from the unrounded r.
+// without a branch r = x.  Sums and products are fp32 (of rows that do not fit the registers, sums
+// in 64 bits); r and y are each rounded once, to their own type, and y is taken from the
+// unrounded r.
 //
 // Bound by memory: 4 to 12 bytes and 2 to 15 flop an element, and by counters the kernels move
 // those bytes and no more.  A copy kernel that goes past the caches reaches 6.5 TB/s; here 360 MB
@@ -34,36 +35,39 @@ __device__ inline float load_one(const void* p, bool wide, int64_t i) {
 }
 
 // Sum over the workgroup, in every thread: lanes by a butterfly, waves in order.
-__device__ inline float block_sum(float v, float* part) {
-  v = wave_sum(v);
+__device__ inline double block_sum(double v, double* part) {
+  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
   __syncthreads();  // the previous sum's readers are done with `part`
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
   __syncthreads();
-  float s = part[0];
+  double s = part[0];
   for (int w = 1; w < kThreads / 64; ++w) s += part[w];
   return s;
 }
 
-struct Stats {
-  float mean, inv;
+struct RowStats {
+  double mean;
+  float inv;
 };
 
-// Mean (LayerNorm only) and reciprocal deviation of value(0 .. width - 1).
+// Mean (LayerNorm only) and reciprocal deviation of value(0 .. width - 1), in 64 bits: a thread
+// adds up to 2^16 terms in order, which in fp32 puts a row of equal values off by 8e-4, and the
+// squares of 2^24 values pass fp32's range from 4.5e15 on.
 template <class V>
-__device__ Stats row_stats(int kind, int width, float eps, float* part, V value) {
-  Stats s{0.0f, 1.0f};
+__device__ RowStats row_stats(int kind, int width, float eps, double* part, V value) {
+  RowStats s{0.0, 1.0f};
   if (kind == kNormNone) return s;
   if (kind == kNormLayer) {
-    float sum = 0.0f;
-    for (int c = threadIdx.x; c < width; c += kThreads) sum += value(c);
-    s.mean = block_sum(sum, part) / (float)width;
+    double sum = 0.0;
+    for (int c = threadIdx.x; c < width; c += kThreads) sum += (double)value(c);
+    s.mean = block_sum(sum, part) / (double)width;
   }
-  float sq = 0.0f;
+  double sq = 0.0;
   for (int c = threadIdx.x; c < width; c += kThreads) {
-    const float d = value(c) - s.mean;
-    sq = fmaf(d, d, sq);
+    const double d = (double)value(c) - s.mean;
+    sq = fma(d, d, sq);
   }
-  s.inv = 1.0f / sqrtf(block_sum(sq, part) / (float)width + eps);
+  s.inv = (float)(1.0 / sqrt(block_sum(sq, part) / (double)width + (double)eps));
   return s;
 }
 
@@ -71,33 +75,33 @@ __device__ Stats row_stats(int kind, int width, float eps, float* part, V value)
 // every pass reads the row again.
 template <class X, class T>
 __global__ __launch_bounds__(kThreads) void residual_rows_kernel(ResidualArgs a) {
-  __shared__ float part[kThreads / 64];
+  __shared__ double part[kThreads / 64];
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const int64_t b = row / a.tokens, n = row - b * a.tokens;
     const int64_t xo = b * a.x.b + n * a.x.n, bo = b * a.branch.b + n * a.branch.n,
                   go = b * a.gate.b + n * a.gate.n, so = b * a.scale.b + n * a.scale.n,
                   ho = b * a.shift.b + n * a.shift.n;
     const auto added = [&](int c) { return load_elem<T>(a.branch.p, bo + c); };
-    Stats post{0.0f, 1.0f};
+    RowStats post{0.0, 1.0f};
     if (a.branch.p) post = row_stats(a.post, a.width, a.eps, part, added);
     const auto value = [&](int c) {
       float r = load_elem<X>(a.x.p, xo + c);
       if (a.branch.p) {
-        float f = (added(c) - post.mean) * post.inv;
+        float f = (float)((double)added(c) - post.mean) * post.inv;
         if (a.branch_weight) f *= load_one<T>(a.branch_weight, a.wide_weight, c);
         if (a.branch_bias) f += load_one<T>(a.branch_bias, a.wide_weight, c);
         r = a.gate.p ? fmaf(load_one<T>(a.gate.p, a.wide_mod, go + c), f, r) : r + f;
       }
       return r;
     };
-    Stats s{0.0f, 1.0f};
+    RowStats s{0.0, 1.0f};
     if (a.y.p) s = row_stats(a.norm, a.width, a.eps, part, value);
     const int64_t ro = b * a.r.b + n * a.r.n, yo = b * a.y.b + n * a.y.n;
     __syncthreads();  // an output may be an input: the row's statistics are all taken
     for (int c = threadIdx.x; c < a.width; c += kThreads) {
       const float r = value(c);
       if (a.y.p) {
-        float y = (r - s.mean) * s.inv;
+        float y = (float)((double)r - s.mean) * s.inv;
         if (a.weight) y *= load_one<T>(a.weight, a.wide_weight, c);
         if (a.bias) y += load_one<T>(a.bias, a.wide_weight, c);
         if (a.scale.p) y *= 1.0f + load_one<T>(a.scale.p, a.wide_mod, so + c);
@@ -121,6 +125,10 @@ template <class X>
 constexpr int kChunk = X::code == 3 ? 4 : 8;  // 16 bytes of the stream
 
 enum ResidualKind { kPre, kGate, kBoth };
+
+struct Stats {
+  float mean, inv;
+};
 
 template <int CHUNKS, int N>
 __device__ Stats chunk_stats(int kind, const float (&v)[CHUNKS][N], int skip, int width, float eps,

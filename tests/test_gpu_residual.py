@@ -207,6 +207,40 @@ def test_a_large_mean(cuda):
     check_all(a, "layer", None, "large mean")
 
 
+@pytest.mark.parametrize("post", ["rms", "layer"])
+def test_the_widest_rows(cuda, post):
+    """2^24 channels, fp32, with a norm of the branch and one of the sum: rows of equal values, rows
+    of values up to 1e17, whose squares' sum is past fp32's range, and ordinary ones.  With sums in
+    64 bits an element is off by its own roundings only.  A norm has three (the difference, the root,
+    their product), the sum one more of the sum's size: 12 half steps cover them.  The second norm
+    adds its three, and the first's errors through its element, mean and deviation: 24."""
+    width = 1 << 24
+    g = torch.Generator(device="cuda").manual_seed(40)
+    x = torch.randn(1, 3, width, generator=g, device="cuda")
+    x[0, 0] = 1.1
+    x[0, 1].clamp_(-6, 6).mul_(1.6e16)
+    f = x * 1.0
+    for kind in ("rms", "layer"):
+        print(f"case {post} {kind}", flush=True)
+        r, y = K.gated_residual_norm(x, f, norm=kind, branch_norm=post)
+        y1 = K.norm_modulate(x, norm=kind)
+        for row in range(3):
+            v = x[0, row].double()
+            mean = v.mean() if kind == "layer" else v.new_zeros(())
+            dev = ((v - mean).square().mean() + 1e-6).sqrt()
+            limit = 12 * 2.0 ** -24 * (v.abs() / dev + 1)
+            assert ((y1[0, row].double() - (v - mean) / dev).abs() <= limit).all(), (kind, row)
+            m = v.mean() if post == "layer" else v.new_zeros(())
+            d = ((v - m).square().mean() + 1e-6).sqrt()
+            sizes = v.abs() + v.abs() / d + 1
+            sum_ = v + (v - m) / d
+            assert ((r[0, row].double() - sum_).abs() <= 12 * 2.0 ** -24 * sizes).all(), (kind, row)
+            mean = sum_.mean() if kind == "layer" else v.new_zeros(())
+            dev = ((sum_ - mean).square().mean() + 1e-6).sqrt()
+            limit = 24 * 2.0 ** -24 * (sizes / dev + 1)
+            assert ((y[0, row].double() - (sum_ - mean) / dev).abs() <= limit).all(), (kind, row)
+
+
 def test_one_channel_with_another_stride(cuda):
     """Rows of one channel, whose stride means nothing (transposed from [batch, 1, tokens])."""
     x = torch.randn(2, 1, 5, device=cuda).transpose(1, 2)
