@@ -122,6 +122,9 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, int64_t 
   };
   float all = 1.0f;
   if (NORM == kRotaryRmsAll) {
+    // A lane's squares are added over a power of two no smaller than the heads, which changes no
+    // bit of the mean but keeps the sum in range: up to 2^16 heads of values up to about 1e17.
+    const float down = __uint_as_float((unsigned)(127 - (32 - __clz(t.heads - 1))) << 23);
     float sq = 0.0f;
     for (int first = 0; first < steps; first += kBatch) {
       if (steps > kBatch) {
@@ -137,10 +140,10 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, int64_t 
           float part = 0.0f;
 #pragma unroll
           for (int e = 0; e < 16; ++e) part = fmaf(x[e], x[e], part);
-          sq += there(first + j) ? part : 0.0f;
+          sq = fmaf(there(first + j) ? part : 0.0f, down, sq);
         }
     }
-    all = 1.0f / sqrtf(row_sum(sq, kLanes * side, nullptr) / (float)(t.heads * D) + a.eps);
+    all = 1.0f / sqrtf(row_sum(sq, kLanes * side, nullptr) / ((float)(t.heads * D) * down) + a.eps);
   }
   for (int first = 0; first < steps; first += kBatch) {
     if (NORM != kRotaryRmsAll || steps > kBatch) fetch(first, past);

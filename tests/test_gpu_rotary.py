@@ -203,6 +203,18 @@ def test_tokens_outside_the_grid_keep_their_values(cuda, d, pairing):
     assert torch.equal(K.qk_rotary(q, pairing=pairing)[0].view(torch.int16), q.view(torch.int16))
 
 
+@pytest.mark.parametrize("norm", ["rms", "rms_all"])
+@pytest.mark.parametrize("heads", [1, 12, 65, 4099])
+def test_large_values(cuda, heads, norm):
+    """Values just inside 1e17, at their signs' random turns: a norm over all heads adds heads * d
+    squares, past fp32's range from some 270 heads of 128 on if they are added as they are."""
+    g = torch.Generator(device="cuda").manual_seed(17)
+    q = torch.randint(0, 2, (1, heads, 5, 128), generator=g, device="cuda").mul(2).sub(1).to(BF) * 9.9e16
+    q = torch.cat((q, q / 3), dim=2)
+    axes = recap_amd.rotary_axes((1, 2, 3), CHANNELS[128], device=cuda)
+    check_both({"q": q, "k": q.flip(1)}, axes, f"{heads} heads", norm=norm, offset=2)
+
+
 def test_streams_and_graph(cuda):
     axes = recap_amd.rotary_axes((3, 20, 20), CHANNELS[128], device=cuda)
     a = make(8, 1, 6, 1250, 128, norm="rms_all")
