@@ -13,6 +13,7 @@ import math
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import call
@@ -641,27 +642,34 @@ def _choice(table: dict, value, what: str) -> int:
     return table[value]
 
 
+_GRADIENT = "requires a gradient, which this call does not record: run it under torch.no_grad()"
+_TANGENT = "carries a forward-mode tangent, which this call does not propagate: unpack it first"
+
+
 def _specs(tensors) -> tuple:
     """What a call's checks look at of its tensors, hashable: everything but their addresses."""
     grad = torch.is_grad_enabled()
-    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.device,
-                                          grad and t.requires_grad) for t in tensors])
+    dual = forward_ad._current_level >= 0
+    return tuple([None if t is None else (
+        t.shape, t.stride(), t.dtype, t.device,
+        _GRADIENT if grad and t.requires_grad else
+        _TANGENT if dual and forward_ad.unpack_dual(t).tangent is not None else None)
+        for t in tensors])
 
 
 def _together(specs: dict) -> torch.device:
-    """The GPU that all tensors of a call are on.  The kernels have no backward pass, so a
-    call that would have to record one is refused."""
+    """The GPU that all tensors of a call are on.  The kernels have no derivatives, so a call that
+    would have to record or propagate one is refused."""
+    specs = {name: spec for name, spec in specs.items() if spec is not None}
+    for name, spec in specs.items():
+        if spec[4]:
+            raise ValueError(f"{name} {spec[4]}")
     device = next(iter(specs.values()))[3]
     for name, spec in specs.items():
-        if spec is None:
-            continue
         if spec[3].type != "cuda":
             raise ValueError(f"{name} must be a GPU tensor")
         if spec[3] != device:
             raise ValueError(f"{name} is on {spec[3]}, the call on {device}")
-        if spec[4]:
-            raise ValueError(f"{name} requires a gradient, which this call does not record: run it "
-                             "under torch.no_grad()")
     return device
 
 

@@ -111,6 +111,25 @@ def test_residual_refusals(call, match):
         call()
 
 
+@pytest.mark.parametrize("call", [
+    lambda x, w: K.norm_modulate(x), lambda x, w: K.norm_modulate(x.detach(), weight=w),
+    lambda x, w: K.gated_residual(x, x.detach()), lambda x, w: K.gated_residual_norm(X[:, :, :1].expand(2, 5, 64), x),
+    lambda x, w: K.qk_rotary(x.view(1, 2, 5, 64)),
+    lambda x, w: K.qk_rotary(x.detach().view(1, 2, 5, 64), norm="rms", q_weight=w)])
+def test_derivatives_are_refused(call):
+    """No call drops a derivative silently: neither a gradient it would have to record nor, also
+    under no_grad, the tangent of forward mode."""
+    from torch.autograd import forward_ad
+    x, w = torch.randn(2, 5, 64).to(BF), torch.ones(64, dtype=BF)
+    with pytest.raises(ValueError, match="gradient"):
+        call(x.clone().requires_grad_(), w.clone().requires_grad_())
+    with forward_ad.dual_level(), torch.no_grad():
+        with pytest.raises(ValueError, match="tangent"):
+            call(*(forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, w)))
+        with pytest.raises(ValueError, match="GPU"):
+            call(x, w)
+
+
 def test_output_overlap_rule():
     """An output may be the input it is named for, or take turns with inputs in rows of one
     pitch; anything else that shares memory is refused."""
