@@ -734,6 +734,12 @@ def _check_output(name: str, out: torch.Tensor, shape, dtype: torch.dtype,
             raise ValueError(f"{name} overlaps the memory of {other}")
 
 
+def _written(*outs: torch.Tensor | None) -> None:
+    """Given outputs count as changed in place, as after torch's own calls: a backward pass that
+    saved one before raises instead of using the new values."""
+    torch.autograd.graph.increment_version([out for out in outs if out is not None])
+
+
 def _weights(kind: int, extent: int, dtype: torch.dtype, specs: dict) -> set:
     """Types of the given weights and biases of a norm over `extent` channels."""
     given = {name: v for name, v in specs.items() if v is not None}
@@ -884,6 +890,7 @@ def qk_rotary(q: torch.Tensor, k: torch.Tensor | None = None, axes=None, *, offs
         if q_out is not None and k_out is not None:
             _check_output("k_out", k_out, k.shape, k.dtype, {"q_out": q_out}, "")
     strides, out_strides = plan.strides, plan.out_strides
+    given = q_out, k_out
     if q_out is not None or k_out is not None:
         out_strides = tuple(made if out is None else _row_strides(out.shape, out.stride())
                             for out, made in zip((q_out, k_out), out_strides))
@@ -904,6 +911,8 @@ def qk_rotary(q: torch.Tensor, k: torch.Tensor | None = None, axes=None, *, offs
              *((None,) * 3 if axes is None else [t.data_ptr() or None for t in axes]), plan.lengths,
              plan.pairs, int(offset), *plan.codes, *map(_p, vectors), plan.weight_code, float(eps),
              q_out.data_ptr(), *out_strides[0], _p(k_out), *out_strides[1])
+    if given[0] is not None or given[1] is not None:
+        _written(*given)
     return q_out, k_out
 
 
@@ -1013,6 +1022,8 @@ def _residual_call(name: str, names, x, dtype, branch, mods, vectors, norms, eps
     if branch is None:
         args.insert(-2, _STREAM_DTYPES[dtype])
     _call_on(plan.device, name, *args)
+    if any(given is not None for _, given, _, _ in outs):
+        _written(*(given for _, given, _, _ in outs))
     return tuple(made)
 
 

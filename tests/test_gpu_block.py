@@ -102,3 +102,25 @@ def test_block_exact_step_and_text_length(cuda):
     assert torch.equal(seen["q"], want)
     assert short[0].shape[1] == wl.tokens - 100 and torch.isfinite(short[1]).all()
     assert torch.isfinite(long[1]).all()
+
+
+@pytest.mark.parametrize("call", [
+    lambda x, b: K.norm_modulate(x, out=x), lambda x, b: K.gated_residual(x, b, out=x),
+    lambda x, b: K.gated_residual_norm(b, x, norm_out=x),
+    lambda x, b: K.gated_residual_norm(x, b[..., ::2].repeat_interleave(2, -1), b.new_zeros(1, 128)[:, ::2],
+                                       out=x),
+    lambda x, b: K.qk_rotary(x[None], None, norm="rms", q_out=x[None]),
+    lambda x, b: K.qk_rotary(b[None], x[None], norm="rms", k_out=x[None])])
+def test_in_place_is_seen_by_autograd(cuda, call):
+    """A tensor that a graph saved, then given as an output: the backward pass raises instead of
+    giving the gradient of other values.  Outputs that a call makes count no change."""
+    x, b = (torch.randn(2, 5, 64, device=cuda).to(torch.bfloat16) for _ in range(2))
+    w = torch.ones(64, dtype=torch.bfloat16, device=cuda, requires_grad=True)
+    loss = (w * x).sum()
+    with torch.no_grad():
+        call(x, b)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        call(x, b)
+    assert K.norm_modulate(x)._version == 0
