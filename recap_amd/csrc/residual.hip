@@ -135,14 +135,16 @@ __device__ Stats chunk_stats(int kind, const float (&v)[CHUNKS][N], int skip, in
                              int lanes, float* part) {
   Stats s{0.0f, 1.0f};
   if (kind == kNormNone) return s;
-  const float per = 1.0f / (float)width;
   if (kind == kNormLayer) {
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < CHUNKS; ++j)
 #pragma unroll
       for (int e = 0; e < N; ++e) sum += j < CHUNKS - 1 || e >= skip ? v[j][e] : 0.0f;
-    s.mean = row_sum(sum, lanes, part) * per;
+    // A division: the mean of equal values whose sum is exact is then that value, and the row 0.
+    // (The product with a rounded 1 / width misses it by 6e-8 of the value, which at 1000 and
+    // eps 1e-6 is a row of 0.06.)  The time is the same.
+    s.mean = row_sum(sum, lanes, part) / (float)width;
   }
   float sq = 0.0f;
 #pragma unroll
@@ -152,7 +154,7 @@ __device__ Stats chunk_stats(int kind, const float (&v)[CHUNKS][N], int skip, in
       const float d = j < CHUNKS - 1 || e >= skip ? v[j][e] - s.mean : 0.0f;
       sq = fmaf(d, d, sq);
     }
-  s.inv = 1.0f / sqrtf(row_sum(sq, lanes, part) * per + eps);
+  s.inv = 1.0f / sqrtf(row_sum(sq, lanes, part) * (1.0f / (float)width) + eps);
   return s;
 }
 

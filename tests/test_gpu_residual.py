@@ -200,6 +200,24 @@ def test_values_that_are_not_numbers(cuda, width):
     assert (y[0, 5] == 0).all()
 
 
+@pytest.mark.parametrize("width", [14, 15, 28, 61, 448, 832, 960, 1001, 1920, 3840, 7168, 8064])
+@pytest.mark.parametrize("types", [(BF, BF, BF), (FP, FP, FP), (F32, FP, FP), (F32, F32, F32)], ids=str)
+def test_rows_of_equal_values(cuda, width, types):
+    """LayerNorm of a row of equal values is 0 exactly, the shift with one.  The values have few bits,
+    so that sums are exact in fp32 in any order, and the widths are such that most of the values
+    times a rounded 1 / width miss the mean."""
+    x = torch.tensor([3.0, 1000.0, -77.0, 0.84375, 1960.0, 0.0], device=cuda)[None, :, None]
+    x = x.expand(2, 6, width).to(types[0]).contiguous()
+    shift = torch.linspace(-1, 1, width, device=cuda).to(types[2])
+    assert not K.norm_modulate(x, dtype=types[1]).any()
+    y = K.norm_modulate(x, None, shift, dtype=types[1])
+    assert torch.equal(y, shift.to(types[1]).expand_as(y))
+    branch = x.to(types[1])
+    r, y = K.gated_residual_norm(x, branch)
+    assert torch.equal(r, (2 * x.double()).to(types[0])) and not y.any()
+    assert torch.equal(K.gated_residual(x, branch, branch_norm="layer"), x)
+
+
 def test_a_large_mean(cuda):
     """A row whose mean is 1000 times its deviation: the variance is taken about the mean."""
     a = make(10, 2, 9, 2048, (F32, F32, F32), "none", affine=False)
