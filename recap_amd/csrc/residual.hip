@@ -6,7 +6,7 @@
 // in 64 bits); r and y are each rounded once, to their own type, and y is taken from the
 // unrounded r.
 //
-// Bound by memory: 4 to 12 bytes and 2 to 15 flop an element, and by counters the kernels move
+// Bound by memory: 4 to 16 bytes and 2 to 15 flop an element, and by counters the kernels move
 // those bytes and no more.  A copy kernel that goes past the caches reaches 6.5 TB/s; here 360 MB
 // of bf16 with a gate (720p, 118,800 x 1536) take 169 us, 6.5 TB/s; gate and norm (480p,
 // 32,760 x 1536) 66 us, 6.1; gate and norm with a norm of the branch (118,800 x 2048) 321 us, 6.1.
@@ -298,7 +298,12 @@ __global__ __launch_bounds__((kMaxThreads<X, ROWS, CHUNKS, KIND>)) void residual
   }
 }
 
-constexpr int kMinWidth = 8, kMaxWidth = 4 * 1024 * 4;
+// Widths that 1024 lanes of four chunks hold: up to 16,384 channels of an fp32 stream, 32,768 of a
+// 16-bit one.  There norm_modulate at 3,000 x 32,768 takes 95 us, gated_residual_norm 169; a
+// workgroup that reads the row again for each sum takes 534 and 1,134.
+constexpr int kMinWidth = 8;
+template <class X>
+constexpr int kMaxWidth = 4 * 1024 * kChunk<X>;
 constexpr int64_t kAllLanes = 256 * 2048;  // that the chip holds at once
 
 // Normalised rows of this many bytes or more go past the caches.  The chain of kStreamBytes in us,
@@ -384,7 +389,7 @@ hipError_t launch_kind(const ResidualArgs& a, hipStream_t s) {
 
 template <class X, class T>
 hipError_t launch(const ResidualArgs& a, hipStream_t s) {
-  if (a.width >= kMinWidth && a.width <= kMaxWidth) {
+  if (a.width >= kMinWidth && a.width <= kMaxWidth<X>) {
     if (!a.branch.p) return launch_kind<X, T, kPre>(a, s);
     return a.y.p ? launch_kind<X, T, kBoth>(a, s) : launch_kind<X, T, kGate>(a, s);
   }

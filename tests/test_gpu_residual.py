@@ -200,6 +200,18 @@ def test_values_that_are_not_numbers(cuda, width):
     assert (y[0, 5] == 0).all()
 
 
+@pytest.mark.parametrize("width", [16383, 16384, 16385, 20001, 24576, 24577, 32760, 32768, 32769])
+@pytest.mark.parametrize("types", [(BF, BF, F32), (FP, FP, FP), (F32, F32, F32)], ids=str)
+def test_widths_at_the_registers_end(cuda, width, types):
+    """16,384 channels of an fp32 stream and 32,768 of a 16-bit one are what 1024 lanes hold."""
+    check_all(make(33, 1, 3, width, types, "sample1"), "layer", "rms", f"width {width}")
+    a = make(34, 2, 5, width, types, "token", affine=False)
+    check_all(a, "rms", "layer", f"width {width}")
+    want, x, branch = run_both(a, "rms", "layer"), a["x"].clone(), a["branch"].clone()
+    run_both({**a, "x": x, "branch": branch}, "rms", "layer", out=x, norm_out=branch)
+    assert torch.equal(x, want[0]) and torch.equal(branch, want[1])
+
+
 @pytest.mark.parametrize("width", [14, 15, 28, 61, 448, 832, 960, 1001, 1920, 3840, 7168, 8064])
 @pytest.mark.parametrize("types", [(BF, BF, BF), (FP, FP, FP), (F32, FP, FP), (F32, F32, F32)], ids=str)
 def test_rows_of_equal_values(cuda, width, types):
