@@ -6,7 +6,7 @@ import torch
 
 import oracle as O
 import recap_amd
-from around_util import qk, residual
+from around_util import check, qk, residual
 from gpu_util import SMALL, metrics
 from recap_amd import EXACT, REFRESH, SPARSE, OperatorConfig, kernels as K
 from recap_amd.layout import Layout, SparseGeometry, hilbert_permutation
@@ -124,3 +124,32 @@ def test_in_place_is_seen_by_autograd(cuda, call):
     with torch.inference_mode():
         call(x, b)
     assert K.norm_modulate(x)._version == 0
+
+
+@pytest.mark.parametrize("name,qk_norm", [("text-first-ragged", "rms"), ("text-last-d128", "rms_all")])
+def test_block_outputs_at_another_text_length(cuda, name, qk_norm):
+    """After a prompt's text length changed, an EXACT step's outputs are its parts' one by one, and
+    those of the 64-bit definition around the same attention output."""
+    import torch.nn.functional as F
+    wl = SMALL[name]
+    block, w, mods, steps, _ = build(wl, cuda, qk_norm, torch.bfloat16, 1)
+    op = block.operator
+    op.begin_step(0, EXACT)
+    cut = wl.text_tokens // 2
+    op.layout.text_tokens -= cut
+    op.layout._gather_cache.clear()
+    x = steps[0][:, cut:] if wl.text_first else steps[0][:, :-cut]
+    scale, shift, gate, scale2, shift2 = mods
+    r, y = block(x, *mods)
+    h = K.norm_modulate(x, scale, shift, dtype=wl.dtype)
+    q, k, v = ((h @ w[n].T).unflatten(2, (wl.heads, wl.dim)).transpose(1, 2) for n in "qkv")
+    q, k = K.qk_rotary(q, k, block.axes, offset=op.layout.video_offset, norm=qk_norm,
+                       q_weight=block.q_weight, k_weight=block.k_weight)
+    branch = F.scaled_dot_product_attention(q, k, v).transpose(1, 2).flatten(2) @ w["o"].T
+    parts = K.gated_residual_norm(x, branch, gate, scale2, shift2, norm="rms", branch_norm="rms",
+                                  branch_weight=block.branch_weight)
+    assert torch.equal(r, parts[0]) and torch.equal(y, parts[1])
+    want = residual(x, branch, gate, scale2, shift2, kind="rms", post="rms",
+                    branch_weight=block.branch_weight)
+    check(r, want[0], "residual")
+    check(y, want[1], "normed")

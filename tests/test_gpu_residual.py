@@ -390,3 +390,59 @@ def test_large_calls_equal_small_ones(cuda, types, batch, tokens, width):
         assert torch.equal(got[0], whole[0][:, rows]) and torch.equal(got[1], whole[1][:, rows])
         assert torch.equal(run_pre(part, "rms", types[1]), pre[:, rows])
         assert torch.equal(run_gate(part, None), gate[:, rows])
+
+
+@pytest.mark.parametrize("types,width", [
+    ((BF, BF, F32), 256), ((BF, BF, F32), 768), ((BF, BF, F32), 1536), ((FP, FP, FP), 1155),
+    ((F32, FP, F32), 128), ((F32, FP, F32), 512), ((F32, BF, F32), 768), ((F32, BF, F32), 1024),
+    ((F32, F32, F32), 128), ((F32, F32, F32), 500), ((F32, F32, F32), 768), ((F32, F32, F32), 1001)], ids=str)
+def test_rows_past_the_caches_equal_small_calls(cuda, types, width):
+    """320 MiB of normalised rows and more are stored past the caches: every number of chunks and rows
+    a lane holds, against the same rows in calls of their own, and in place."""
+    size = 4 if types[1] == F32 else 2
+    tokens = (320 << 20) // (width * size) // 2 * 2 + 7
+    print(f"case {types} {tokens} x {width}", flush=True)
+    a = make(35, 1, tokens, width, types)
+    whole, pre = run_both(a, "layer", None), run_pre(a, "rms", types[1])
+    posted = run_both(a, "rms", "layer")
+    for rows in (slice(0, 70), slice(tokens // 2, tokens // 2 + 9), slice(tokens - 71, tokens)):
+        part = {n: v[:, rows] if v.ndim == 3 and v.shape[1] > 1 else v for n, v in a.items()}
+        for got, want in ((run_both(part, "layer", None), whole), (run_both(part, "rms", "layer"), posted)):
+            assert torch.equal(got[0], want[0][:, rows]) and torch.equal(got[1], want[1][:, rows])
+        assert torch.equal(run_pre(part, "rms", types[1]), pre[:, rows])
+    del posted, pre
+    run_both(a, "layer", None, out=a["x"], norm_out=a["branch"])
+    assert torch.equal(a["x"], whole[0]) and torch.equal(a["branch"], whole[1])
+
+
+@pytest.mark.parametrize("width", [1, 5, 7, 32769, 40001])
+@pytest.mark.parametrize("types", [(BF, BF, BF), (F32, FP, F32), (F32, F32, F32)], ids=str)
+def test_in_place_beyond_the_registers(cuda, width, types):
+    """The rows that a workgroup reads again for each sum, over their own inputs."""
+    a = make(36, 2, 33, width, types)
+    for norm, post in (("layer", "layer"), ("rms", None)):
+        want = run_both(a, norm, post)
+        x, br = a["x"].clone(), a["branch"].clone()
+        run_both({**a, "x": x, "branch": br}, norm, post, out=x, norm_out=br)
+        assert torch.equal(x, want[0]) and torch.equal(br, want[1])
+        want, x = run_gate(a, post), a["x"].clone()
+        assert torch.equal(run_gate({**a, "x": x}, post, out=x), want)
+        if types[0] == types[1]:
+            want, x = run_pre(a, norm), a["x"].clone()
+            assert torch.equal(run_pre({**a, "x": x}, norm, out=x), want)
+
+
+@pytest.mark.parametrize("width", [3, 5])
+def test_more_short_rows_than_workgroups(cuda, width):
+    """Rows under a chunk, more than a launch's 2^20 workgroups: a workgroup takes several."""
+    a = make(37, 2, (1 << 20) + 300, width, (BF, BF, F32))
+    tokens = a["x"].shape[1]
+    whole, pre = run_both(a, "layer", "rms"), run_pre(a, "rms")
+    x, br = a["x"].clone(), a["branch"].clone()
+    run_both({**a, "x": x, "branch": br}, "layer", "rms", out=x, norm_out=br)
+    assert torch.equal(x, whole[0]) and torch.equal(br, whole[1])
+    for rows in (slice(0, 40), slice(tokens - 700, tokens - 600), slice(tokens - 40, tokens)):
+        part = {n: v[:, rows] if v.ndim == 3 else v for n, v in a.items()}
+        got = run_both(part, "layer", "rms")
+        assert torch.equal(got[0], whole[0][:, rows]) and torch.equal(got[1], whole[1][:, rows])
+        assert torch.equal(run_pre(part, "rms"), pre[:, rows])

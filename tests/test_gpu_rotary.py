@@ -283,3 +283,33 @@ def test_more_tokens_than_one_launch(cuda):
     want = K.qk_rotary(tail["q"], None, axes, norm="rms", q_weight=tail["q_weight"])[0]
     got = K.qk_rotary(q, None, axes, offset=n - 40, norm="rms", q_weight=tail["q_weight"], q_out=q)[0]
     assert torch.equal(got[:, :, -40:], want) and not got[:, :, :-40].any()
+
+
+@pytest.mark.parametrize("d,heads,heads_k,tokens", [
+    (128, 48, 48, 70), (128, 48, 7, 70), (64, 130, 48, 33), (128, 41, 41, 70), (64, 80, 3, 1)])
+@pytest.mark.parametrize("pairing", ["interleaved", "halves"])
+def test_many_heads_under_one_norm(cuda, d, heads, heads_k, tokens, pairing):
+    """A norm over more heads than a wave holds at once reads them again after the sum: against the
+    definition, and in place."""
+    axes = recap_amd.rotary_axes((1, 1, tokens), CHANNELS[d], device=cuda)
+    a = make(18, 2, heads, tokens, d, norm="rms_all", heads_k=heads_k)
+    want = check_both(a, axes, f"{heads} and {heads_k} heads", norm="rms_all", pairing=pairing)
+    b = {**a, "q": a["q"].clone(), "k": a["k"].transpose(1, 2).contiguous().transpose(1, 2)}
+    run(b, axes, norm="rms_all", pairing=pairing, q_out=b["q"], k_out=b["k"])
+    assert torch.equal(b["q"], want[0]) and torch.equal(b["k"], want[1])
+
+
+@pytest.mark.parametrize("d,heads", [(128, 48), (64, 130), (128, 25)])
+def test_many_heads_past_the_caches(cuda, d, heads):
+    """The same at 192 MiB a call and more, in place, against the tokens in calls of their own."""
+    tokens = (192 << 20) // (8 * d * heads) + 9
+    print(f"case {heads} x {tokens} x {d}", flush=True)
+    a = make(19, 1, heads, tokens, d, norm="rms_all")
+    axes = recap_amd.rotary_axes((1, 1, tokens), CHANNELS[d], device=cuda)
+    whole = run(a, axes, norm="rms_all")
+    for first in (0, tokens // 2, tokens - 9):
+        part = {m: v[:, :, first:first + 9] if len(m) == 1 else v for m, v in a.items()}
+        got = run(part, (*axes[:2], axes[2][first:first + 9]), norm="rms_all")
+        assert all(torch.equal(x, y[:, :, first:first + 9]) for x, y in zip(got, whole))
+    run(a, axes, norm="rms_all", q_out=a["q"], k_out=a["k"])
+    assert torch.equal(a["q"], whole[0]) and torch.equal(a["k"], whole[1])
