@@ -51,8 +51,10 @@ class AttentionBlock:
     next_norm: str = "layer"                # before the next half
     next_weight: torch.Tensor | None = None
     next_bias: torch.Tensor | None = None
-    eps: float = 1e-6
+    eps: float = 1e-6                       # of the norm before the attention
     dtype: torch.dtype | None = None        # of the projections (an fp32 stream); None: the stream's
+    qk_eps: float | None = None             # of the queries' and keys' norm; None: eps
+    next_eps: float | None = None           # of the output's norm and the next half's; None: eps
 
     def __call__(self, x: torch.Tensor, scale: torch.Tensor | None = None,
                  shift: torch.Tensor | None = None, gate: torch.Tensor | None = None,
@@ -74,10 +76,11 @@ class AttentionBlock:
         query, key = K.qk_rotary(query, key, self.axes, offset=layout.video_offset,
                                  pairing=self.pairing, norm=self.qk_norm,
                                  q_weight=self.q_weight, k_weight=self.k_weight,
-                                 q_bias=self.q_bias, k_bias=self.k_bias, eps=self.eps)
+                                 q_bias=self.q_bias, k_bias=self.k_bias,
+                                 eps=self.eps if self.qk_eps is None else self.qk_eps)
         out = self.operator.attend(self.layer, query, key, value)
         branch = self.to_out(out.transpose(1, 2).flatten(2))
         return K.gated_residual_norm(
             x, branch, gate, next_scale, next_shift, norm=self.next_norm, weight=self.next_weight,
             bias=self.next_bias, branch_norm=self.branch_norm, branch_weight=self.branch_weight,
-            branch_bias=self.branch_bias, eps=self.eps)
+            branch_bias=self.branch_bias, eps=self.eps if self.next_eps is None else self.next_eps)

@@ -153,3 +153,23 @@ def test_block_outputs_at_another_text_length(cuda, name, qk_norm):
                     branch_weight=block.branch_weight)
     check(r, want[0], "residual")
     check(y, want[1], "normed")
+
+
+def test_block_norms_with_their_own_eps(cuda):
+    """eps, qk_eps and next_eps each reach their own norms."""
+    wl = SMALL["video-ragged-d128"]
+    block, w, mods, steps, _ = build(wl, cuda, "rms", torch.bfloat16, 1)
+    block.eps, block.qk_eps, block.next_eps = 0.3, 0.02, 0.1
+    block.operator.begin_step(0, EXACT)
+    seen, attend = {}, block.operator.attend
+    block.operator.attend = lambda layer, *qkv: seen.update(qkv=qkv, out=attend(layer, *qkv)) or seen["out"]
+    x = steps[0]
+    r, y = block(x, *mods)
+    h = K.norm_modulate(x, mods[0], mods[1], eps=0.3)
+    q, k = ((h @ w[n].T).unflatten(2, (wl.heads, wl.dim)).transpose(1, 2) for n in "qk")
+    for got, t, weight in ((seen["qkv"][0], q, block.q_weight), (seen["qkv"][1], k, block.k_weight)):
+        check(got, qk(t, block.axes, kind="rms", weight=weight, eps=0.02), "queries and keys")
+    branch = seen["out"].transpose(1, 2).flatten(2) @ w["o"].T
+    want = residual(x, branch, *mods[2:], kind="rms", post="rms", branch_weight=block.branch_weight, eps=0.1)
+    check(r, want[0], "residual")
+    check(y, want[1], "normed")
