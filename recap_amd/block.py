@@ -6,6 +6,10 @@ the queries' and keys' norm and rotation, the attention call, the output project
 gated residual with the next half's modulated norm.  The projections are the model's own
 modules; everything between them runs on the HIP kernels.  A model integration builds one per
 layer in its ``build_operator`` and calls it in the block's forward.
+
+It is a block of one stream: one set of projections, norms and modulations for the tokens of the
+whole sequence.  A block whose text tokens have their own calls the kernels itself, each stream's
+queries and keys with ``q_out`` and ``k_out`` in its part of the joint sequence.
 """
 
 from __future__ import annotations

@@ -173,3 +173,58 @@ def test_block_norms_with_their_own_eps(cuda):
     want = residual(x, branch, *mods[2:], kind="rms", post="rms", branch_weight=block.branch_weight, eps=0.1)
     check(r, want[0], "residual")
     check(y, want[1], "normed")
+
+
+@pytest.mark.parametrize("text_first", [False, True])
+@pytest.mark.parametrize("heads,d", [(3, 128), (2, 64)])
+@pytest.mark.parametrize("grid", [(3, 5, 10), (3, 15, 20)], ids=str)
+def test_two_streams_in_one_sequence(cuda, text_first, heads, d, grid):
+    """A block whose text tokens have projections and norms of their own: each stream's queries and
+    keys go into its part of the joint sequence, and its part of the attention's output into its own
+    residual stream.  A video of at most two blocks may leave rows of a sparse call without a tail,
+    which the reference's merge makes NaN: such rows stay NaN and touch no others."""
+    text, width, b = 77, 192, 2
+    video = grid[0] * grid[1] * grid[2]
+    layout = Layout.from_permutation(hilbert_permutation(grid), text_tokens=text, text_first=text_first)
+    op = recap_amd.Operator.build(OperatorConfig(head_density=0.5), SparseGeometry.build(layout, 128), n_layers=1)
+    axes = recap_amd.rotary_axes(grid, CHANNELS[d], device=cuda)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    dtype, inner = torch.bfloat16, heads * d
+    first = layout.video_offset
+    parts = {"video": slice(first, first + video),
+             "text": slice(0, text) if text_first else slice(video, video + text)}
+    streams = {n: rand(b, video if n == "video" else text, width).to(dtype) for n in parts}
+    w = {n: {m: (rand(*s) * s[1] ** -0.5).to(dtype) for m, s in
+             (("q", (inner, width)), ("k", (inner, width)), ("v", (inner, width)), ("o", (width, inner)))}
+         for n in parts}
+    norms = {n: [(1 + 0.2 * rand(d)).to(dtype) for _ in "qk"] for n in parts}
+    mods = {n: [0.3 * rand(b, 1, width) for _ in range(5)] for n in parts}
+
+    joint = [torch.full((b, video + text, heads, d), 7.0, dtype=dtype, device=cuda).transpose(1, 2)
+             for _ in "qkv"]
+    split = {}
+    for n, at in parts.items():
+        h = K.norm_modulate(streams[n], mods[n][0], mods[n][1])
+        q, k, v = ((h @ w[n][m].T).unflatten(2, (heads, d)).transpose(1, 2) for m in "qkv")
+        split[n] = q, k
+        K.qk_rotary(q, k, axes if n == "video" else None, norm="rms", q_weight=norms[n][0],
+                    k_weight=norms[n][1], q_out=joint[0][:, :, at], k_out=joint[1][:, :, at])
+        joint[2][:, :, at] = v
+    for n, at in parts.items():
+        for i in range(2):
+            check(joint[i][:, :, at], qk(split[n][i], axes if n == "video" else None, kind="rms",
+                                         weight=norms[n][i]), f"{n} {'qk'[i]}")
+    for step, kind in enumerate((REFRESH, SPARSE)):
+        print(f"case {heads} x {d} text first {text_first} {kind}", flush=True)
+        op.begin_step(step, kind)
+        out = op.attend(0, *joint).transpose(1, 2)
+        for n, at in parts.items():
+            branch = out[:, at].flatten(2) @ w[n]["o"].T
+            r, y = K.gated_residual_norm(streams[n], branch, *mods[n][2:])
+            want = residual(streams[n], branch, *mods[n][2:], kind="layer")
+            rows = ~branch.isnan().any(-1)
+            assert rows.all() or (video <= 256 and kind == SPARSE and branch[~rows].isnan().all())
+            assert r[~rows].isnan().all() and y[~rows].isnan().all()
+            for label, got, (exact, bound) in (("residual", r, want[0]), ("normed", y, want[1])):
+                check(got[rows], (exact[rows], bound[rows]), f"{n} {label}")
