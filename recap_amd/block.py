@@ -56,7 +56,7 @@ class AttentionBlock:
     next_weight: torch.Tensor | None = None
     next_bias: torch.Tensor | None = None
     eps: float = 1e-6                       # of the norm before the attention
-    dtype: torch.dtype | None = None        # of the projections (an fp32 stream); None: the stream's
+    dtype: torch.dtype | None = None        # of the projections; None: the stream's
     qk_eps: float | None = None             # of the queries' and keys' norm; None: eps
     next_eps: float | None = None           # of the output's norm and the next half's; None: eps
 

@@ -203,6 +203,8 @@ constexpr bool kWideRows = ROWS > 1 && CHUNKS == 3 && KIND == kBoth && kChunk<X>
 template <class X, int ROWS, int CHUNKS, int KIND>
 constexpr int kMaxThreads = kWideRows<X, ROWS, CHUNKS, KIND> ? kThreads : 1024;
 
+// Every level below is a kernel of its own, 300 with the types: 44 s of compiling on one core, the
+// longest of the library's sources.
 // ROWS > 1: rows of one sample (`per_sample` workgroups each) that share gate, scale and shift.
 // STREAM: 1 loads the rows past the caches, 2 also stores the normalised ones past them.
 template <class X, class T, int ROWS, int CHUNKS, int KIND, int STREAM>
@@ -308,7 +310,8 @@ constexpr int64_t kAllLanes = 256 * 2048;  // that the chip holds at once
 
 // Normalised rows of this many bytes or more go past the caches.  The chain of kStreamBytes in us,
 // through them -> past them: 101 MB of rows 583 -> 605, 201 MB 1,156 -> 1,188, 276 MB
-// 1,747 -> 1,753, 365 MB 2,250 -> 2,237; 487 MB (118,800 x 2048), the call alone, 335 -> 321.
+// 1,747 -> 1,753, 365 MB 2,317 -> 2,310, 487 MB 3,087 -> 3,049, 730 MB 4,578 -> 4,547; the call
+// alone, 487 MB (118,800 x 2048), 335 -> 321.
 constexpr int64_t kPastBytes = int64_t(320) << 20;
 
 template <class X, class T, int ROWS, int CHUNKS, int KIND>

@@ -230,6 +230,13 @@ hipError_t launch(const RotaryArgs& a, hipStream_t s) {
   }
   constexpr int kWaves = kThreads / 64;
   const int64_t blocks = (waves + kWaves - 1) / kWaves;
+  // Past the caches from kStreamBytes on, loads (of heads of 128) and stores, though Q and K are
+  // read next: what they would push out, V and the projections' other outputs, is read as well.
+  // Three projections, this call, then recap_kv_pack and recap_pool_blocks in us, heads of 128,
+  // stores through the caches -> past them: 101 MB a call 147.5 -> 150.9, 203 MB 279.1 -> 277.3,
+  // 302 MB 431.0 -> 423.9, 403 MB 519.2 -> 514.0, 2,926 MB 6,170 -> 6,118; heads of 64, 331 MB
+  // 722.8 -> 722.1, 1,109 MB 2,307 -> 2,290.  With the whole sparse call behind them the same way
+  // or even (403 MB 1,987 -> 1,975).
   for (int64_t first = 0; first < blocks; first += kMaxBlocks) {
     const dim3 grid((unsigned)std::min(blocks - first, kMaxBlocks), a.tensors);
     if (4 * D * values >= kStreamBytes) {

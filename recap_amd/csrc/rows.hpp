@@ -37,6 +37,7 @@ constexpr int64_t kMaxBlocks = 1 << 20;  // of a launch, whose threads have to b
 // 256 MB Infinity Cache beside what comes after.  A chain gated_residual_norm, two projections,
 // gated_residual_norm at width 1536 in us, loads through the caches -> past them: 100 MB a call
 // 178 -> 182, 151 MB 257 -> 258, 252 MB 385 -> 379, 302 MB 483 -> 471, 403 MB 595 -> 580.
+// Rotated queries and keys are also stored past them from there on (rotary.hip).
 constexpr int64_t kStreamBytes = int64_t(192) << 20;
 
 // 16 and 8 bytes at any address; STREAM: past the caches, for data that is used once.  (A vector
