@@ -462,7 +462,8 @@ int recap_bank_copy_async(void* dst, const void* src, int64_t bytes, void* strea
  *    v / W % H, v % W); the other tokens (text) are not rotated.  Frequency i rotates channels
  *    (2i, 2i + 1) (RECAP_PAIRS_INTERLEAVED) or (i, i + dim / 2) (RECAP_PAIRS_HALVES).  lengths
  *    and pairs (host arrays of 3) NULL: no rotation.
- *  - k may be NULL.  An output may be its own input, and overlaps nothing else.
+ *  - Inputs may be expanded (strides of 0).  k may be NULL.  An output may be its own input, and
+ *    overlaps nothing else; rows of an output that share memory are refused.
  * Statistics and products are fp32 (a norm's rows stay below about 1e17), rounded once.  Covers
  * the query/key norm and the rotary embedding before operator.attend in the model processors,
  * recap/models/hunyuan.py:79-154. */
@@ -491,8 +492,8 @@ int recap_qk_rotary(const void* q, const void* k, int dtype, int64_t batch, int6
  *  - Strides are in elements, channels have unit stride, and nothing needs more than its
  *    element's alignment.  residual_out may be x and out may be branch (for
  *    recap_norm_modulate, x); outputs overlap nothing else.
- * Statistics and products are fp32 (a norm's rows stay below about 1e17); each output is
- * rounded once.  Covers the modulated norms and gated residuals of the transformer blocks
+ * Statistics and products are fp32 or wider (a norm's rows stay below about 1e17); each output
+ * is rounded once.  Covers the modulated norms and gated residuals of the transformer blocks
  * whose processors call operator.attend, recap/models/hunyuan.py:79-154. */
 int recap_norm_modulate(const void* x, int x_dtype, int64_t batch, int64_t tokens,
                         int64_t width, int64_t x_stride_b, int64_t x_stride_n,
