@@ -72,7 +72,8 @@ __device__ RowStats row_stats(int kind, int width, float eps, double* part, V va
 }
 
 // Rows under a chunk or too wide for the registers of 1024 lanes: one workgroup per row, and
-// every pass reads the row again.
+// every pass reads the row again (norm_modulate of 2,000 rows of 40,001: 549 us, sums in fp32 541;
+// a million rows of 5: 2.5 ms).
 template <class X, class T>
 __global__ __launch_bounds__(kThreads) void residual_rows_kernel(ResidualArgs a) {
   __shared__ double part[kThreads / 64];
