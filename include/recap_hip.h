@@ -33,10 +33,11 @@
 extern "C" {
 #endif
 
-#define RECAP_ABI_VERSION 10
+#define RECAP_ABI_VERSION 11
 
 enum { RECAP_OK = 0, RECAP_EINVAL = 1, RECAP_EUNSUPPORTED = 2, RECAP_EHIP = 3 };
-enum { RECAP_F16 = 1, RECAP_BF16 = 2, RECAP_F32 = 3 };  /* F32: around the attention call only */
+enum { RECAP_F16 = 1, RECAP_BF16 = 2, RECAP_F32 = 3 };  /* F32: around the attention call and
+                                                            microscaled forms only */
 enum { RECAP_NORM_NONE = 0, RECAP_NORM_RMS = 1, RECAP_NORM_LAYER = 2, RECAP_NORM_RMS_ALL = 3 };
 enum { RECAP_PAIRS_INTERLEAVED = 0, RECAP_PAIRS_HALVES = 1 };
 enum { RECAP_CLOSURE_ROT = 1, RECAP_CLOSURE_CVK = 2, RECAP_CLOSURE_SCATTER = 4 };
@@ -522,6 +523,48 @@ int recap_gated_residual_norm(const void* x, int x_dtype, int64_t batch, int64_t
                               void* residual_out, int64_t residual_stride_b,
                               int64_t residual_stride_n, void* out, int64_t out_stride_b,
                               int64_t out_stride_n, void* stream);
+
+/* Microscaled forms --------------------------------------------------------------------- */
+
+/* Rows [rows, width] in 4 or 8 bits with one scale for every block of 32 values along the row.
+ * A block whose largest magnitude is a has the scale 2^e, held as the byte e + 127:
+ *   RECAP_MX_FP4   e the smallest, from -127 on, with a < 7 * 2^e; a value is the nearest of 0,
+ *                  0.5, 1, 1.5, 2, 3, 4 and 6 times 2^e.  A code is that list's index with the
+ *                  sign in bit 3, two to a byte, the first in the low half.  Rows are filled up
+ *                  with zeros to a multiple of 256 values.
+ *   RECAP_MX_INT8  e the smallest, from -127 on, with 64 a < 127.5 * 2^e; a code c is an integer
+ *                  of -127 .. 127, its value c * 2^(e - 6).  Rows are filled up to whole blocks.
+ * Ties go to the even code.  A block with an infinity or NaN has the byte 255 and reads as NaN.
+ * recap_mx_row_bytes and recap_mx_row_scales give the bytes of a row's codes and of its scales;
+ * rows follow one another without gaps.
+ *  - values are of dtype (RECAP_BF16, RECAP_F16 or RECAP_F32), rows row_stride elements apart
+ *    (0 reads one row again; an output's rows may not overlap), of any alignment of their type.
+ *  - codes are 16-byte aligned.  A value that dtype cannot hold reads as its rounding to dtype.
+ * No counterpart in the reference, whose refinement is fp16 (recap/operator.py:33-59). */
+enum { RECAP_MX_FP4 = 1, RECAP_MX_INT8 = 2 };
+int64_t recap_mx_row_bytes(int format, int64_t width);
+int64_t recap_mx_row_scales(int format, int64_t width);
+int recap_mx_quantise(const void* values, int dtype, int64_t rows, int64_t width,
+                      int64_t row_stride, int format, void* codes, uint8_t* scales, void* stream);
+int recap_mx_dequantise(const void* codes, const uint8_t* scales, int format, int64_t rows,
+                        int64_t width, void* values, int dtype, int64_t row_stride,
+                        void* stream);
+
+/* A projection with fp4 operands: out[m, n] = sum_k x[m, k] * weight[n, k] + bias[n], out
+ * [rows, outputs] of dtype (RECAP_BF16, RECAP_F16 or RECAP_F32), its rows out_stride elements
+ * apart.
+ *  - x_scales non-NULL: x holds fp4 codes (x_dtype and x_stride are not read).  NULL: x holds
+ *    values of x_dtype, rows x_stride elements apart, which the call brings into fp4 in the
+ *    workspace (recap_mx_linear_workspace_size bytes, 16-byte aligned; of no size, and NULL
+ *    allowed, with codes).  The workspace needs no contents and keeps none.
+ *  - bias [outputs] of bias_dtype (any of the three types) or NULL.
+ *  - Codes are 16-byte aligned, scales 8-byte aligned; width is at most 2^22.
+ * Products are exact, sums fp32, rounded once after the bias. */
+int64_t recap_mx_linear_workspace_size(int64_t rows, int64_t width, int64_t outputs, int codes);
+int recap_mx_linear(const void* x, int x_dtype, int64_t x_stride, const uint8_t* x_scales,
+                    int64_t rows, int64_t width, const void* weight, const uint8_t* weight_scales,
+                    int64_t outputs, const void* bias, int bias_dtype, void* out, int dtype,
+                    int64_t out_stride, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

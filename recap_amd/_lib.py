@@ -11,12 +11,13 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "librecap_hip.so"
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 RECAP_OK, RECAP_EINVAL, RECAP_EUNSUPPORTED, RECAP_EHIP = 0, 1, 2, 3
 RECAP_F16, RECAP_BF16, RECAP_F32 = 1, 2, 3
 NORM_NONE, NORM_RMS, NORM_LAYER, NORM_RMS_ALL = 0, 1, 2, 3
 PAIRS_INTERLEAVED, PAIRS_HALVES = 0, 1
+MX_FP4, MX_INT8 = 1, 2
 CLOSURE_ROT, CLOSURE_CVK, CLOSURE_SCATTER = 1, 2, 4
 CAPTURE_NOALLOC_MAX_PAIRS = 1 << 19  # RECAP_CAPTURE_NOALLOC_MAX_PAIRS
 PAGER_TIMING = 1  # RECAP_PAGER_TIMING
@@ -108,6 +109,13 @@ SIGNATURES: dict[str, tuple] = {
     "recap_gated_residual_norm": (_I, [_P, _I, _I64, _I64, _I64, _I64, _I64, _P, _I, _I64, _I64,
                                        *_ROWS, *_ROWS, *_ROWS, _I, _P, _P, _P, _P, _I, _I, _I, _F,
                                        *_ROWS, *_ROWS, _P]),
+    "recap_mx_row_bytes": (_I64, [_I, _I64]),
+    "recap_mx_row_scales": (_I64, [_I, _I64]),
+    "recap_mx_quantise": (_I, [_P, _I, _I64, _I64, _I64, _I, _P, _P, _P]),
+    "recap_mx_dequantise": (_I, [_P, _P, _I, _I64, _I64, _P, _I, _I64, _P]),
+    "recap_mx_linear_workspace_size": (_I64, [_I64, _I64, _I64, _I]),
+    "recap_mx_linear": (_I, [_P, _I, _I64, _P, _I64, _I64, _P, _P, _I64, _P, _I, _P, _I, _I64, _P,
+                             _I64, _P]),
 }
 
 _lock = threading.Lock()

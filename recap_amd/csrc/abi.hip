@@ -11,6 +11,7 @@
 
 #include <cmath>
 #include "kernels.hpp"
+#include "microscale.hpp"
 
 using namespace recap;
 
@@ -1313,6 +1314,115 @@ int recap_gated_residual_norm(const void* x, int x_dtype, int64_t batch, int64_t
   a.eps = eps;
   return residual(a, "gated_residual_norm", x_dtype, dtype, mod_dtype, weight_dtype, batch,
                   tokens, width, stream);
+}
+
+namespace {
+
+int check_mx(const char* what, int format, int dtype, int64_t rows, int64_t width) {
+  static_assert(RECAP_MX_FP4 == kMxFp4 && RECAP_MX_INT8 == kMxInt8, "format codes");
+  REQUIRE(format == RECAP_MX_FP4 || format == RECAP_MX_INT8, "%s: unknown format %d", what, format);
+  REQUIRE(stream_dtype(dtype), "%s: unknown dtype %d", what, dtype);
+  REQUIRE(rows >= 1 && width >= 1, "%s: sizes must be positive", what);
+  REQUIRE(rows <= INT32_MAX && width <= (1 << 24), "%s: %lld rows of %lld exceed 2^31-1 or 2^24",
+          what, (long long)rows, (long long)width);
+  return RECAP_OK;
+}
+
+int check_mx_rows(const char* what, const void* values, int dtype, int64_t rows, int64_t width,
+                  int64_t stride, bool output, const void* codes, const void* scales) {
+  REQUIRE(values && codes && scales, "%s: NULL pointer", what);
+  REQUIRE((reinterpret_cast<uintptr_t>(values) & (dtype == RECAP_F32 ? 3 : 1)) == 0,
+          "%s: values are misaligned for their type", what);
+  REQUIRE(stride >= 0, "%s: row stride %lld must be non-negative", what, (long long)stride);
+  REQUIRE(!output || rows == 1 || stride >= width, "%s: row stride %lld lets rows of %lld overlap",
+          what, (long long)stride, (long long)width);
+  REQUIRE(aligned16(codes), "%s: codes must be 16-byte aligned", what);
+  return RECAP_OK;
+}
+
+constexpr int64_t kMaxLinearWidth = int64_t(1) << 22;
+
+}  // namespace
+
+int64_t recap_mx_row_bytes(int format, int64_t width) {
+  return (format == RECAP_MX_FP4 || format == RECAP_MX_INT8) && width >= 1
+             ? mx_row_bytes(format, width) : -1;
+}
+
+int64_t recap_mx_row_scales(int format, int64_t width) {
+  return (format == RECAP_MX_FP4 || format == RECAP_MX_INT8) && width >= 1
+             ? mx_row_scales(format, width) : -1;
+}
+
+int recap_mx_quantise(const void* values, int dtype, int64_t rows, int64_t width,
+                      int64_t row_stride, int format, void* codes, uint8_t* scales,
+                      void* stream) {
+  CHECK(check_mx("mx_quantise", format, dtype, rows, width));
+  CHECK(check_mx_rows("mx_quantise", values, dtype, rows, width, row_stride, false, codes, scales));
+  return hip_status(run_mx_quantise({const_cast<void*>(values), rows, width, row_stride, codes,
+                                     scales}, dtype, format, as_stream(stream)), "mx_quantise launch");
+}
+
+int recap_mx_dequantise(const void* codes, const uint8_t* scales, int format, int64_t rows,
+                        int64_t width, void* values, int dtype, int64_t row_stride,
+                        void* stream) {
+  CHECK(check_mx("mx_dequantise", format, dtype, rows, width));
+  CHECK(check_mx_rows("mx_dequantise", values, dtype, rows, width, row_stride, true, codes, scales));
+  return hip_status(run_mx_dequantise({values, rows, width, row_stride, const_cast<void*>(codes),
+                                       const_cast<uint8_t*>(scales)}, dtype, format,
+                                      as_stream(stream)), "mx_dequantise launch");
+}
+
+int64_t recap_mx_linear_workspace_size(int64_t rows, int64_t width, int64_t outputs, int codes) {
+  if (rows < 1 || width < 1 || outputs < 1 || rows > INT32_MAX || outputs > INT32_MAX ||
+      width > kMaxLinearWidth)
+    return -1;
+  return codes ? 0 : rows * (mx_row_bytes(kMxFp4, width) + mx_row_scales(kMxFp4, width));
+}
+
+int recap_mx_linear(const void* x, int x_dtype, int64_t x_stride, const uint8_t* x_scales,
+                    int64_t rows, int64_t width, const void* weight, const uint8_t* weight_scales,
+                    int64_t outputs, const void* bias, int bias_dtype, void* out, int dtype,
+                    int64_t out_stride, void* workspace, int64_t workspace_bytes, void* stream) {
+  CHECK(check_mx("mx_linear", RECAP_MX_FP4, dtype, rows, width));
+  REQUIRE(outputs >= 1 && outputs <= INT32_MAX, "mx_linear: outputs %lld outside 1..2^31-1",
+          (long long)outputs);
+  REQUIRE(width <= kMaxLinearWidth, "mx_linear: width %lld exceeds 2^22", (long long)width);
+  REQUIRE(x && weight && weight_scales && out, "mx_linear: NULL pointer");
+  const auto aligned8 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; };
+  REQUIRE(aligned16(weight) && aligned8(weight_scales),
+          "mx_linear: the weight's codes must be 16-byte and its scales 8-byte aligned");
+  REQUIRE(bias == nullptr || stream_dtype(bias_dtype), "mx_linear: unknown bias dtype %d", bias_dtype);
+  REQUIRE((reinterpret_cast<uintptr_t>(bias) & (bias_dtype == RECAP_F32 ? 3 : 1)) == 0,
+          "mx_linear: the bias is misaligned for its type");
+  REQUIRE((reinterpret_cast<uintptr_t>(out) & (dtype == RECAP_F32 ? 3 : 1)) == 0,
+          "mx_linear: out is misaligned for its type");
+  REQUIRE(rows == 1 || out_stride >= outputs, "mx_linear: row stride %lld lets rows of %lld overlap",
+          (long long)out_stride, (long long)outputs);
+  hipStream_t s = as_stream(stream);
+  const uint8_t* codes = static_cast<const uint8_t*>(x);
+  const uint8_t* scales = x_scales;
+  if (x_scales != nullptr) {
+    REQUIRE(aligned16(x) && aligned8(x_scales),
+            "mx_linear: x's codes must be 16-byte and its scales 8-byte aligned");
+  } else {
+    const int64_t need = recap_mx_linear_workspace_size(rows, width, outputs, 0);
+    REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= need,
+            "mx_linear: workspace of %lld bytes, need %lld, 16-byte aligned",
+            (long long)workspace_bytes, (long long)need);
+    CHECK(check_mx("mx_linear", RECAP_MX_FP4, x_dtype, rows, width));
+    uint8_t* space = static_cast<uint8_t*>(workspace);
+    uint8_t* space_scales = space + rows * mx_row_bytes(kMxFp4, width);
+    CHECK(check_mx_rows("mx_linear", x, x_dtype, rows, width, x_stride, false, space, space_scales));
+    CHECK(hip_status(run_mx_quantise({const_cast<void*>(x), rows, width, x_stride, space,
+                                      space_scales}, x_dtype, kMxFp4, s), "mx_quantise launch"));
+    codes = space;
+    scales = space_scales;
+  }
+  const MxProductArgs a{codes, scales, static_cast<const uint8_t*>(weight), weight_scales, bias,
+                        bias_dtype, out, out_stride, (int)rows, (int)outputs,
+                        (int)(mx_filled(kMxFp4, width) / mx_fill(kMxFp4))};
+  return hip_status(run_mx_product(a, dtype, s), "mx_linear launch");
 }
 
 }  // extern "C"

@@ -200,6 +200,26 @@ struct RotaryArgs {
 };
 hipError_t run_rotary(const RotaryArgs& a, int dtype, int dim, hipStream_t s);
 
+// Microscaled rows (microscale.hip; formats in microscale.hpp).
+struct MxRowsArgs {
+  void* values;                                  // rows [rows][width], `stride` elements apart
+  int64_t rows, width, stride;
+  void* codes; uint8_t* scales;                  // without gaps between rows
+  int64_t chunks = 0;                            // of 8 values a filled row, set at launch
+};
+hipError_t run_mx_quantise(const MxRowsArgs& a, int dtype, int format, hipStream_t s);
+hipError_t run_mx_dequantise(const MxRowsArgs& a, int dtype, int format, hipStream_t s);
+
+// Product of fp4 rows, out[m][n] = sum_k x[m][k] w[n][k] + bias[n] (mx_linear.hip).
+struct MxProductArgs {
+  const uint8_t* x; const uint8_t* x_scales;     // [rows] of `steps` 128-byte steps of 256 values
+  const uint8_t* w; const uint8_t* w_scales;     // [outputs] likewise; 8 scale bytes a step
+  const void* bias; int bias_dtype;              // [outputs], or null
+  void* out; int64_t stride;
+  int rows, outputs, steps;
+};
+hipError_t run_mx_product(const MxProductArgs& a, int dtype, hipStream_t s);
+
 // Host-bank pager (pager.hip): pinned host banks, device slots, prefetch and write-back
 // streams.  Slot and key indices are checked by the caller (abi.hip).
 struct Pager;

@@ -1077,6 +1077,295 @@ def gated_residual_norm(x: torch.Tensor, branch: torch.Tensor, gate: torch.Tenso
                           [("out", out, x.dtype, "x"), ("norm_out", norm_out, branch.dtype, "branch")])
 
 
+# -- microscaled forms ----------------------------------------------------------------------
+
+MX_BLOCK = 32  # values along a row that share a scale
+_MX_FORMATS = {"fp4": _lib.MX_FP4, "int8": _lib.MX_INT8}
+_MX_FILL = {"fp4": 256, "int8": MX_BLOCK}
+_MX_CODES = {"fp4": torch.uint8, "int8": torch.int8}
+
+
+@dataclass(frozen=True)
+class Microscaled:
+    """Rows ``[..., width]`` in 4 or 8 bits, with a power of two for every 32 values along a row.
+
+    ``format`` ``"fp4"``: values 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives times the scale, two
+    codes to a byte of ``codes`` (uint8 ``[..., bytes]``); rows are filled up to 256 values.
+    ``"int8"``: integers up to 127 times the scale / 64 (int8 ``[..., values]``); rows are filled up
+    to 32 values.  ``scales`` (uint8 ``[..., blocks]``) holds each scale's exponent + 127; 255 marks
+    a block that held an infinity or NaN and reads as NaN.  Both tensors are contiguous."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    format: str
+    width: int
+
+    @property
+    def shape(self) -> torch.Size:
+        return torch.Size((*self.codes.shape[:-1], self.width))
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.codes, self.scales))
+
+    @classmethod
+    def empty(cls, shape, format: str, device=None) -> "Microscaled":
+        """Room for rows of this shape, not yet written."""
+        _choice(_MX_FORMATS, format, "format")
+        *lead, width = (int(n) for n in shape)
+        if width < 1:
+            raise ValueError(f"rows of {width} values")
+        filled = -(-width // _MX_FILL[format]) * _MX_FILL[format]
+        return cls(torch.empty(*lead, filled // 2 if format == "fp4" else filled,
+                               dtype=_MX_CODES[format], device=device),
+                   torch.empty(*lead, filled // MX_BLOCK, dtype=torch.uint8, device=device),
+                   format, width)
+
+
+def _check_microscaled(name: str, format: str, width: int, codes, scales) -> int:
+    """Checks a Microscaled's specs; returns its number of rows."""
+    _choice(_MX_FORMATS, format, "format")
+    if width < 1:
+        raise ValueError(f"{name} has rows of {width} values")
+    filled = -(-width // _MX_FILL[format]) * _MX_FILL[format]
+    lead = tuple(codes[0][:-1])
+    for part, spec, dtype, size in (
+            ("codes", codes, _MX_CODES[format], filled // 2 if format == "fp4" else filled),
+            ("scales", scales, torch.uint8, filled // MX_BLOCK)):
+        if spec[2] != dtype or len(spec[0]) < 1 or tuple(spec[0]) != (*lead, size):
+            raise ValueError(f"{name}: {part} of {format} rows of {width} are {dtype} "
+                             f"{(*lead, size)}, got {spec[2]} {tuple(spec[0])}")
+        step = 1
+        for n, stride in zip(reversed(spec[0]), reversed(spec[1])):
+            if n > 1 and stride != step and 0 not in lead:
+                raise ValueError(f"{name}: {part} must be contiguous")
+            step *= n
+    return math.prod(lead)
+
+
+def _even_rows(spec) -> int | None:
+    """Stride of the rows of a tensor ``[..., width]``, where one reaches them all."""
+    step = size = None
+    shape, strides = spec[:2]
+    if shape[-1] > 1 and strides[-1] != 1:
+        return None
+    for n, stride in zip(reversed(shape[:-1]), reversed(strides[:-1])):
+        if n == 1:
+            continue
+        if step is None:
+            step, size = stride, n
+        elif stride != step * size:
+            return None
+        else:
+            size *= n
+    return shape[-1] if step is None else step
+
+
+def _mx_values(name: str, spec) -> None:
+    if len(spec[0]) < 1 or spec[0][-1] < 1:
+        raise ValueError(f"{name} must be [..., width], got {tuple(spec[0])}")
+    if spec[2] not in _STREAM_DTYPES:
+        raise ValueError(f"unsupported dtype {spec[2]} of {name}; use bfloat16, float16 or float32")
+
+
+@functools.lru_cache(maxsize=1024)
+def _mx_rows_plan(name: str, values, format: str, width: int, codes, scales):
+    """(device, number of rows, row stride or None) of values [..., width] and their form."""
+    _mx_values(name, values)
+    lead = tuple(values[0][:-1])
+    rows = math.prod(lead)
+    if codes is not None:
+        _check_microscaled("the microscaled form", format, width, codes, scales)
+        if (*lead, width) != (*codes[0][:-1], values[0][-1]):
+            raise ValueError(f"{name} is {tuple(values[0])}, the microscaled form "
+                             f"{(*codes[0][:-1], width)}")
+    device = _together({name: values, "codes": codes, "scales": scales})
+    return device, rows, _even_rows(values)
+
+
+def _aligned(t: torch.Tensor, to: int) -> torch.Tensor:
+    return t if t.data_ptr() % to == 0 else t.clone()
+
+
+def mx_quantise(x: torch.Tensor, format: str = "fp4", *,
+                out: Microscaled | None = None) -> Microscaled:
+    """Rows ``[..., width]`` of bfloat16, float16 or float32 in their microscaled form.  Each block of
+    32 values along a row gets the smallest power of two with which its largest magnitude still
+    rounds to a code, and every value its nearest code (ties to the even one).  Rows an even step
+    apart (a slice of a wider projection, an expanded row) are read in place, others laid out first.
+    ``out`` is written in place: a bank that is kept."""
+    _choice(_MX_FORMATS, format, "format")
+    specs = _specs((x,) if out is None else (x, out.codes, out.scales))
+    if out is not None and out.format != format:
+        raise ValueError(f"out is {out.format}, the call's format {format}")
+    width = x.shape[-1] if x.ndim else 0
+    device, rows, stride = _mx_rows_plan("x", specs[0], format, width if out is None else out.width,
+                                         *(specs[1:] or (None, None)))
+    given = out
+    if out is None:
+        out = Microscaled.empty(x.shape, format, device)
+    else:
+        if out.codes.data_ptr() % 16:
+            raise ValueError("out must have 16-byte aligned codes")
+        for name, t in (("codes", out.codes), ("scales", out.scales)):
+            _apart(f"out's {name}", t, {"x": x})
+        _apart("out's codes", out.codes, {"its scales": out.scales})
+    if rows == 0:
+        return out
+    if stride is None:
+        x = x.contiguous()
+        stride = width
+    _call_on(device, "recap_mx_quantise", x.data_ptr(), _STREAM_DTYPES[x.dtype], rows, width, stride,
+             _MX_FORMATS[format], out.codes.data_ptr(), out.scales.data_ptr())
+    if given is not None:
+        _written(given.codes, given.scales)
+    return out
+
+
+def _apart(name: str, out: torch.Tensor, inputs: dict[str, torch.Tensor | None]) -> None:
+    if out.numel() == 0:
+        return
+    lo, hi = _span(out)
+    for other, t in inputs.items():
+        if t is not None and t.numel():
+            start, end = _span(t)
+            if start < hi and lo < end and not _interleaved(out, t):
+                raise ValueError(f"{name} overlaps the memory of {other}")
+
+
+def mx_dequantise(m: Microscaled, dtype: torch.dtype = torch.bfloat16, *,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """The values ``[..., width]`` of a microscaled tensor, as ``dtype`` (exact in bfloat16 and
+    float32, and in float16 within its range).  ``out``: rows an even step apart."""
+    specs = _specs((m.codes, m.scales) if out is None else (m.codes, m.scales, out))
+    if out is None:
+        if dtype not in _STREAM_DTYPES:
+            raise ValueError(f"unsupported dtype {dtype}; use bfloat16, float16 or float32")
+        rows = _check_microscaled("m", m.format, m.width, *specs)
+        device, stride = _together({"codes": specs[0], "scales": specs[1]}), m.width
+        given, out = None, torch.empty(m.shape, dtype=dtype, device=device)
+    else:
+        given = out
+        device, rows, stride = _mx_rows_plan("out", specs[2], m.format, m.width, *specs[:2])
+        _check_output("out", out, m.shape, dtype, {"codes": m.codes, "scales": m.scales}, "")
+        if stride is None:
+            raise ValueError("out must have rows an even step apart")
+    if rows == 0:
+        return out
+    codes = _aligned(m.codes, 16)
+    _call_on(device, "recap_mx_dequantise", codes.data_ptr(), m.scales.data_ptr(),
+             _MX_FORMATS[m.format], rows, m.width, out.data_ptr(), _STREAM_DTYPES[out.dtype], stride)
+    if given is not None:
+        _written(given)
+    return out
+
+
+@dataclass(frozen=True)
+class _LinearPlan:
+    """What an mx_linear call of given shapes and types passes besides addresses."""
+
+    device: torch.device
+    shape: tuple            # of the result
+    rows: int
+    width: int
+    outputs: int
+    stride: int | None      # of x's rows; None: x is first laid out
+    dtype: torch.dtype      # of the result
+    bias_code: int
+    workspace: int
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear_plan(x, x_scales, x_form, weight, weight_scales, w_form, bias, dtype) -> _LinearPlan:
+    """Checks of an mx_linear call, from its tensors' specs and (format, width) of those in fp4."""
+    for name, form in (("x", x_form), ("weight", w_form)):
+        if form is not None and form[0] != "fp4":
+            raise ValueError(f"{name} is {form[0]}; the product takes fp4 codes")
+    outputs = _check_microscaled("weight", *w_form, weight, weight_scales)
+    width = w_form[1]
+    if len(weight[0]) != 2 or outputs < 1:
+        raise ValueError(f"weight must be [outputs, width], got {(*weight[0][:-1], width)}")
+    if x_form is not None:
+        _check_microscaled("x", *x_form, x, x_scales)
+        shape, stride = (*x[0][:-1], x_form[1]), x_form[1]
+        dtype = dtype or torch.bfloat16
+    else:
+        _mx_values("x", x)
+        shape, stride = tuple(x[0]), _even_rows(x)
+        dtype = dtype or x[2]
+    if shape[-1] != width:
+        raise ValueError(f"x is {shape}, the weight takes rows of {width}")
+    if dtype not in _STREAM_DTYPES:
+        raise ValueError(f"unsupported dtype {dtype}; use bfloat16, float16 or float32")
+    bias_code = _STREAM_DTYPES[dtype]
+    if bias is not None:
+        if tuple(bias[0]) != (outputs,):
+            raise ValueError(f"bias is {tuple(bias[0])}, expected ({outputs},)")
+        if bias[2] not in _STREAM_DTYPES:
+            raise ValueError(f"unsupported dtype {bias[2]} of bias")
+        bias_code = _STREAM_DTYPES[bias[2]]
+    rows = math.prod(shape[:-1])
+    device = _together({"x": x, "x's scales": x_scales, "weight": weight,
+                        "the weight's scales": weight_scales, "bias": bias})
+    size = 0 if rows == 0 else int(_lib.load().recap_mx_linear_workspace_size(
+        rows, width, outputs, int(x_form is not None)))
+    if size < 0:
+        raise ValueError(f"mx_linear: {rows} rows of {width} to {outputs} outputs are too many")
+    return _LinearPlan(device, (*shape[:-1], outputs), rows, width, outputs, stride, dtype, bias_code,
+                       size)
+
+
+def mx_linear(x: torch.Tensor | Microscaled, weight: Microscaled,
+              bias: torch.Tensor | None = None, *, dtype: torch.dtype | None = None,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """``x @ weight.T + bias`` in 4 bits: ``weight`` is fp4 ``[outputs, width]`` (mx_quantise of a
+    projection's weight, once), ``x`` ``[..., width]`` is fp4 too, or a bfloat16, float16 or float32
+    tensor that the call brings into fp4.  Several projections of the same rows quantise them once
+    and pass the Microscaled.  Products are exact and sums fp32; the result has ``dtype`` (x's own,
+    bfloat16 for codes), rounded once after the bias.  ``out`` may be rows an even step apart (a
+    part of a wider tensor)."""
+    micro = isinstance(x, Microscaled)
+    tensors = (x.codes, x.scales) if micro else (x, None)
+    specs = _specs((*tensors, weight.codes, weight.scales, bias))
+    plan = _linear_plan(specs[0], specs[1], (x.format, x.width) if micro else None, specs[2],
+                        specs[3], (weight.format, weight.width), specs[4], dtype)
+    given, stride = out, plan.outputs
+    if out is None:
+        out = torch.empty(plan.shape, dtype=plan.dtype, device=plan.device)
+    else:
+        spec = _specs((out,))[0]
+        _together({"weight": specs[2], "out": spec})
+        _check_output("out", out, plan.shape, plan.dtype,
+                      {"x": tensors[0], "x's scales": tensors[1], "weight": weight.codes,
+                       "the weight's scales": weight.scales, "bias": bias}, "")
+        stride = _even_rows(spec)
+        if stride is None:
+            raise ValueError("out must have rows an even step apart")
+    if plan.rows == 0:
+        return out
+    codes, scales, x_code, x_stride, work = tensors[0], tensors[1], 0, 0, None
+    if micro:
+        codes, scales = _aligned(codes, 16), _aligned(scales, 8)
+    else:
+        x_stride = plan.stride
+        if x_stride is None:
+            codes, x_stride = x.contiguous(), plan.width
+        x_code = _STREAM_DTYPES[x.dtype]
+        work = torch.empty(plan.workspace, dtype=torch.uint8, device=plan.device)
+    w, w_scales = _aligned(weight.codes, 16), _aligned(weight.scales, 8)
+    bias = _unit(bias)
+    _call_on(plan.device, "recap_mx_linear", codes.data_ptr(), x_code, x_stride, _p(scales),
+             plan.rows, plan.width, w.data_ptr(), w_scales.data_ptr(), plan.outputs, _p(bias),
+             plan.bias_code, out.data_ptr(),
+             _STREAM_DTYPES[plan.dtype], stride, _p(work), plan.workspace)
+    if given is not None:
+        _written(given)
+    return out
+
+
 def bank_copy_async(dst: torch.Tensor, src: torch.Tensor, stream=None) -> None:
     """Asynchronous device <-> pinned-host copy of a whole bank tensor on ``stream``."""
     if dst.numel() * dst.element_size() != src.numel() * src.element_size():
