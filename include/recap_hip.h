@@ -550,6 +550,43 @@ int recap_mx_dequantise(const void* codes, const uint8_t* scales, int format, in
                         int64_t width, void* values, int dtype, int64_t row_stride,
                         void* stream);
 
+/* recap_sparse_merge_attn_ws, recap_sparse_call and recap_refresh_capture with the refinement in
+ * RECAP_MX_INT8: det holds the codes [banks, R, dim] (16-byte aligned), det_scale the scale bytes
+ * [banks, R, dim / 32] (4-byte aligned).  A capture rounds once, from fp32 to the codes (and takes
+ * the mass the head leaves, 1 - ratio, without cancellation); a merge reads them in place.  Other
+ * arguments and results are those of the calls named. */
+int recap_sparse_merge_attn_mx(const void* q, int dtype, int64_t batch, int64_t heads,
+                               int64_t dim, int64_t stride_b, int64_t stride_h,
+                               int64_t stride_n, const void* k_tiles, const void* vt_tiles,
+                               const int32_t* rowmap, const uint8_t* kernel_mask,
+                               int64_t n_tokens, int64_t n_video, float scale, const void* go,
+                               const float* gl, const void* det, const uint8_t* det_scale,
+                               const float* dl, const float* glref, const float* center,
+                               float alpha_override, void* out, int64_t out_stride_b,
+                               int64_t out_stride_h, int64_t out_stride_n, int64_t split,
+                               int balance, void* workspace, int64_t workspace_bytes,
+                               void* stream);
+int recap_sparse_call_mx(const void* q, const void* k, const void* v, int dtype, int64_t batch,
+                         int64_t heads, int64_t dim, int64_t q_stride_b, int64_t q_stride_h,
+                         int64_t q_stride_n, int64_t k_stride_b, int64_t k_stride_h,
+                         int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_h,
+                         int64_t v_stride_n, const int32_t* rowmap, int64_t n_tokens,
+                         int64_t n_video, float scale, float theta, int64_t rank, int64_t group,
+                         int64_t parts, const void* u_hi_t, const void* u_lo_t, const void* u_t,
+                         const uint8_t* partition, const uint8_t* kernel_mask, const void* det,
+                         const uint8_t* det_scale, const float* dl, const float* glref,
+                         float alpha_override, void* out, int64_t out_stride_b,
+                         int64_t out_stride_h, int64_t out_stride_n, int64_t split,
+                         void* const* stage_events, void* workspace, int64_t workspace_bytes,
+                         void* stream);
+int recap_refresh_capture_mx(const void* dense_out, int dtype, int64_t batch, int64_t heads,
+                             int64_t dim, int64_t out_stride_b, int64_t out_stride_h,
+                             int64_t out_stride_n, const float* dense_lse, const void* head_out,
+                             const float* head_lse, const void* go, const float* gl,
+                             const int32_t* rowmap, int64_t n_tokens, int64_t n_video, void* det,
+                             uint8_t* det_scale, float* dl, const float* glref,
+                             const float* center, float* stat_partial, float* stats, void* stream);
+
 /* A projection with fp4 operands: out[m, n] = sum_k x[m, k] * weight[n, k] + bias[n], out
  * [rows, outputs] of dtype (RECAP_BF16, RECAP_F16 or RECAP_F32), its rows out_stride elements
  * apart.

@@ -23,7 +23,9 @@ from .config import (OperatingPoint, OperatorConfig, RecapConfig, config_from_di
                      load_config)
 from .controller import Controller
 from .host_banks import HostBankOperator
+from .kernels import Microscaled
 from .layout import Layout, SparseGeometry, hilbert_permutation
+from .microscale import MicroscaledLinear
 from .operator import EXACT, REFRESH, SPARSE, DetailBank, Operator, SparseAttention
 from .rotary import rotary_axes
 from .session import REUSE, RecapSession
@@ -33,7 +35,7 @@ __all__ = [
     "EXACT", "REFRESH", "REUSE", "SPARSE", "AttentionBlock", "AttentionBranch", "BlockSummary",
     "ClosureBank",
     "Controller", "DetailBank", "HostBankOperator",
-    "Layout", "OperatingPoint", "Operator", "OperatorConfig", "RecapConfig", "RecapSession",
+    "Layout", "Microscaled", "MicroscaledLinear", "OperatingPoint", "Operator", "OperatorConfig", "RecapConfig", "RecapSession",
     "SparseAttention", "SparseGeometry", "config_from_dict", "hilbert_permutation", "install",
     "load_config", "register_builder", "rotary_axes",
 ]

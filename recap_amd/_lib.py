@@ -113,6 +113,14 @@ SIGNATURES: dict[str, tuple] = {
     "recap_mx_row_scales": (_I64, [_I, _I64]),
     "recap_mx_quantise": (_I, [_P, _I, _I64, _I64, _I64, _I, _P, _P, _P]),
     "recap_mx_dequantise": (_I, [_P, _P, _I, _I64, _I64, _P, _I, _I64, _P]),
+    "recap_sparse_merge_attn_mx": (_I, [_P, _I, _I64, _I64, _I64, *_STRIDES, _P, _P, _P, _P,
+                                        _I64, _I64, _F, _P, _P, _P, _P, _P, _P, _P, _F, _P,
+                                        *_STRIDES, _I64, _I, _P, _I64, _P]),
+    "recap_sparse_call_mx": (_I, [_P, _P, _P, _I, _I64, _I64, _I64, *_STRIDES, *_STRIDES, *_STRIDES,
+                                  _P, _I64, _I64, _F, _F, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P,
+                                  _P, _P, _P, _F, _P, *_STRIDES, _I64, _P, _P, _I64, _P]),
+    "recap_refresh_capture_mx": (_I, [_P, _I, _I64, _I64, _I64, *_STRIDES, _P, _P, _P, _P, _P, _P,
+                                      _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P]),
     "recap_mx_linear_workspace_size": (_I64, [_I64, _I64, _I64, _I]),
     "recap_mx_linear": (_I, [_P, _I, _I64, _P, _I64, _I64, _P, _P, _I64, _P, _I, _P, _I, _I64, _P,
                              _I64, _P]),

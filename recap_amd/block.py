@@ -4,7 +4,7 @@ What the reference's processors and the blocks around them do with torch modules
 (recap/models/hunyuan.py:79-154): the modulated norm of the residual stream, the projections,
 the queries' and keys' norm and rotation, the attention call, the output projection, and the
 gated residual with the next half's modulated norm.  The projections are the model's own
-modules; everything between them runs on the HIP kernels.  A model integration builds one per
+modules, or ``MicroscaledLinear``s in 4 bits; everything between them runs on the HIP kernels.  A model integration builds one per
 layer in its ``build_operator`` and calls it in the block's forward.
 
 It is a block of one stream: one set of projections, norms and modulations for the tokens of the
@@ -21,6 +21,7 @@ from typing import Callable
 import torch
 
 from . import kernels as K
+from .microscale import MicroscaledLinear
 from .operator import Operator
 
 Projection = Callable[[torch.Tensor], torch.Tensor]
@@ -75,8 +76,13 @@ class AttentionBlock:
                                  f"{layout.video_tokens} video tokens")
         y = K.norm_modulate(x, scale, shift, norm=self.norm, weight=self.weight, bias=self.bias,
                             eps=self.eps, dtype=self.dtype)
-        query, key, value = (p(y).unflatten(-1, (self.heads, -1)).transpose(1, 2)
-                             for p in (self.to_q, self.to_k, self.to_v))
+        projections = self.to_q, self.to_k, self.to_v
+        if all(isinstance(p, MicroscaledLinear) for p in projections):
+            rows = K.mx_quantise(y)     # once for the three
+            parts = [p(rows, dtype=p.dtype or y.dtype) for p in projections]
+        else:
+            parts = [p(y) for p in projections]
+        query, key, value = (t.unflatten(-1, (self.heads, -1)).transpose(1, 2) for t in parts)
         query, key = K.qk_rotary(query, key, self.axes, offset=layout.video_offset,
                                  pairing=self.pairing, norm=self.qk_norm,
                                  q_weight=self.q_weight, k_weight=self.k_weight,

@@ -594,27 +594,36 @@ static int merge_args(const void* q, int dtype, int64_t batch, int64_t heads, in
                       int64_t stride_b, int64_t stride_h, int64_t stride_n, const void* k_tiles,
                       const void* vt_tiles, const int32_t* rowmap, const uint8_t* kernel_mask,
                       int64_t n_tokens, int64_t n_video, float scale, const void* go,
-                      const float* gl, const void* det, const float* dl, const float* glref,
-                      const float* center, float alpha_override, void* out,
-                      int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_n,
-                      AttnArgs& a) {
+                      const float* gl, const void* det, const uint8_t* det_scale,
+                      const float* dl, const float* glref, const float* center,
+                      float alpha_override, void* out, int64_t out_stride_b,
+                      int64_t out_stride_h, int64_t out_stride_n, AttnArgs& a) {
   CHECK(attn_common(q, dtype, batch, heads, dim, stride_b, stride_h, stride_n, k_tiles, vt_tiles,
                     rowmap, n_tokens, n_video, a));
   CHECK(check_qkv("out", out, batch, heads, out_stride_b, out_stride_h, out_stride_n));
   REQUIRE(kernel_mask != nullptr, "kernel_mask is NULL");
   if (a.rows > 0) {
     REQUIRE(go && gl && det && dl && aligned16(go) && aligned16(det), "merge inputs go/gl/det/dl");
+    REQUIRE((reinterpret_cast<uintptr_t>(det_scale) & 3) == 0, "det_scale must be 4-byte aligned");
     REQUIRE(alpha_override >= 0.0f || (glref && (center || a.drift_part)),
             "drift weight needs glref and center");
   }
   a.kmask = kernel_mask;
   CHECK(set_scale(a, scale));
   a.out = static_cast<uint16_t*>(out); a.osB = out_stride_b; a.osH = out_stride_h; a.osN = out_stride_n;
-  a.go = static_cast<const uint16_t*>(go); a.gl = gl; a.det = static_cast<const uint16_t*>(det);
+  a.go = static_cast<const uint16_t*>(go); a.gl = gl; a.det = det; a.det_scale = det_scale;
   a.dl = dl; a.glref = glref; a.center = center;
   a.use_override = alpha_override >= 0.0f ? 1 : 0;
   a.alpha_override = alpha_override;
   return RECAP_OK;
+}
+
+// The launch of a merge: the refinement is in int8 where it has scales.  (Without refined rows both
+// modes are one.)
+static int merge_launch(const AttnArgs& a, int dtype, int64_t dim, hipStream_t s) {
+  return hip_status(run_attention(a, dtype, (int)dim,
+                                  a.det_scale != nullptr ? kModeMergeInt8 : kModeMerge, s),
+                    "attention launch");
 }
 
 int recap_sparse_merge_attn(const void* q, int dtype, int64_t batch, int64_t heads,
@@ -628,10 +637,27 @@ int recap_sparse_merge_attn(const void* q, int dtype, int64_t batch, int64_t hea
                             void* stream) {
   AttnArgs a{};
   CHECK(merge_args(q, dtype, batch, heads, dim, stride_b, stride_h, stride_n, k_tiles, vt_tiles,
-                   rowmap, kernel_mask, n_tokens, n_video, scale, go, gl, det, dl, glref, center,
-                   alpha_override, out, out_stride_b, out_stride_h, out_stride_n, a));
+                   rowmap, kernel_mask, n_tokens, n_video, scale, go, gl, det, nullptr, dl, glref,
+                   center, alpha_override, out, out_stride_b, out_stride_h, out_stride_n, a));
   CHECK(set_queue(a, work_queue, as_stream(stream)));
-  return hip_status(run_attention(a, dtype, (int)dim, kModeMerge, as_stream(stream)), "attention launch");
+  return merge_launch(a, dtype, dim, as_stream(stream));
+}
+
+static int merge_ws(const void* q, int dtype, int64_t batch, int64_t heads, int64_t dim,
+                    int64_t stride_b, int64_t stride_h, int64_t stride_n, const void* k_tiles,
+                    const void* vt_tiles, const int32_t* rowmap, const uint8_t* kernel_mask,
+                    int64_t n_tokens, int64_t n_video, float scale, const void* go,
+                    const float* gl, const void* det, const uint8_t* det_scale, const float* dl,
+                    const float* glref, const float* center, float alpha_override, void* out,
+                    int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_n,
+                    int64_t split, int balance, void* workspace, int64_t workspace_bytes,
+                    void* stream) {
+  AttnArgs a{};
+  CHECK(merge_args(q, dtype, batch, heads, dim, stride_b, stride_h, stride_n, k_tiles, vt_tiles,
+                   rowmap, kernel_mask, n_tokens, n_video, scale, go, gl, det, det_scale, dl, glref,
+                   center, alpha_override, out, out_stride_b, out_stride_h, out_stride_n, a));
+  CHECK(set_workspace(a, dim, split, balance, workspace, workspace_bytes, as_stream(stream)));
+  return merge_launch(a, dtype, dim, as_stream(stream));
 }
 
 int recap_sparse_merge_attn_ws(const void* q, int dtype, int64_t batch, int64_t heads,
@@ -644,12 +670,28 @@ int recap_sparse_merge_attn_ws(const void* q, int dtype, int64_t batch, int64_t 
                                void* out, int64_t out_stride_b, int64_t out_stride_h,
                                int64_t out_stride_n, int64_t split, int balance,
                                void* workspace, int64_t workspace_bytes, void* stream) {
-  AttnArgs a{};
-  CHECK(merge_args(q, dtype, batch, heads, dim, stride_b, stride_h, stride_n, k_tiles, vt_tiles,
-                   rowmap, kernel_mask, n_tokens, n_video, scale, go, gl, det, dl, glref, center,
-                   alpha_override, out, out_stride_b, out_stride_h, out_stride_n, a));
-  CHECK(set_workspace(a, dim, split, balance, workspace, workspace_bytes, as_stream(stream)));
-  return hip_status(run_attention(a, dtype, (int)dim, kModeMerge, as_stream(stream)), "attention launch");
+  return merge_ws(q, dtype, batch, heads, dim, stride_b, stride_h, stride_n, k_tiles, vt_tiles,
+                  rowmap, kernel_mask, n_tokens, n_video, scale, go, gl, det, nullptr, dl, glref,
+                  center, alpha_override, out, out_stride_b, out_stride_h, out_stride_n, split,
+                  balance, workspace, workspace_bytes, stream);
+}
+
+int recap_sparse_merge_attn_mx(const void* q, int dtype, int64_t batch, int64_t heads,
+                               int64_t dim, int64_t stride_b, int64_t stride_h,
+                               int64_t stride_n, const void* k_tiles, const void* vt_tiles,
+                               const int32_t* rowmap, const uint8_t* kernel_mask,
+                               int64_t n_tokens, int64_t n_video, float scale, const void* go,
+                               const float* gl, const void* det, const uint8_t* det_scale,
+                               const float* dl, const float* glref, const float* center,
+                               float alpha_override, void* out, int64_t out_stride_b,
+                               int64_t out_stride_h, int64_t out_stride_n, int64_t split,
+                               int balance, void* workspace, int64_t workspace_bytes,
+                               void* stream) {
+  REQUIRE(det_scale || n_video < kBlock, "sparse_merge_attn_mx: det_scale is NULL");
+  return merge_ws(q, dtype, batch, heads, dim, stride_b, stride_h, stride_n, k_tiles, vt_tiles,
+                  rowmap, kernel_mask, n_tokens, n_video, scale, go, gl, det, det_scale, dl, glref,
+                  center, alpha_override, out, out_stride_b, out_stride_h, out_stride_n, split,
+                  balance, workspace, workspace_bytes, stream);
 }
 
 static int64_t cvk_partials(int64_t banks, int64_t nb, ClosureSpan span) {
@@ -763,18 +805,19 @@ int64_t recap_sparse_call_workspace_size(int dtype, int64_t banks, int64_t dim, 
                       {(int)group, (int)parts}, rank, split).bytes;
 }
 
-int recap_sparse_call(const void* q, const void* k, const void* v, int dtype, int64_t batch,
-                      int64_t heads, int64_t dim, int64_t q_stride_b, int64_t q_stride_h,
-                      int64_t q_stride_n, int64_t k_stride_b, int64_t k_stride_h,
-                      int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_h,
-                      int64_t v_stride_n, const int32_t* rowmap, int64_t n_tokens,
-                      int64_t n_video, float scale, float theta, int64_t rank, int64_t group,
-                      int64_t parts, const void* u_hi_t, const void* u_lo_t, const void* u_t,
-                      const uint8_t* partition, const uint8_t* kernel_mask, const void* det,
-                      const float* dl, const float* glref, float alpha_override, void* out,
-                      int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_n,
-                      int64_t split, void* const* stage_events, void* workspace,
-                      int64_t workspace_bytes, void* stream) {
+static int sparse_call(const void* q, const void* k, const void* v, int dtype, int64_t batch,
+                       int64_t heads, int64_t dim, int64_t q_stride_b, int64_t q_stride_h,
+                       int64_t q_stride_n, int64_t k_stride_b, int64_t k_stride_h,
+                       int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_h,
+                       int64_t v_stride_n, const int32_t* rowmap, int64_t n_tokens,
+                       int64_t n_video, float scale, float theta, int64_t rank, int64_t group,
+                       int64_t parts, const void* u_hi_t, const void* u_lo_t, const void* u_t,
+                       const uint8_t* partition, const uint8_t* kernel_mask, const void* det,
+                       const uint8_t* det_scale, const float* dl, const float* glref,
+                       float alpha_override, void* out, int64_t out_stride_b,
+                       int64_t out_stride_h, int64_t out_stride_n, int64_t split,
+                       void* const* stage_events, void* workspace, int64_t workspace_bytes,
+                       void* stream) {
   // Every check of the five launches is made before the first of them.
   CHECK(check_common(dtype, dim));
   CHECK(check_tokens(n_tokens, n_video));
@@ -802,8 +845,8 @@ int recap_sparse_call(const void* q, const void* k, const void* v, int dtype, in
   a.drift_part = f32(w.drift);
   CHECK(merge_args(q, dtype, batch, heads, dim, q_stride_b, q_stride_h, q_stride_n, base + w.kt,
                    base + w.vt, rowmap, kernel_mask, n_tokens, n_video, scale, base + w.go,
-                   f32(w.gl), det, dl, glref, nullptr, alpha_override, out, out_stride_b,
-                   out_stride_h, out_stride_n, a));
+                   f32(w.gl), det, det_scale, dl, glref, nullptr, alpha_override, out,
+                   out_stride_b, out_stride_h, out_stride_n, a));
   unsigned* words = reinterpret_cast<unsigned*>(base + w.attn);
   const AttnSpace space = attn_space(banks, dim, a.tb - a.ds, split);
   a.queue = words;
@@ -830,8 +873,50 @@ int recap_sparse_call(const void* q, const void* k, const void* v, int dtype, in
                           n_tokens, n_video, scale, theta, rank, glref, base + w.go, f32(w.gl),
                           f32(w.drift), stream));
   CHECK(mark(3));
-  CHECK(hip_status(run_attention(a, dtype, (int)dim, kModeMerge, s), "attention launch"));
+  CHECK(merge_launch(a, dtype, dim, s));
   return mark(4);
+}
+
+int recap_sparse_call(const void* q, const void* k, const void* v, int dtype, int64_t batch,
+                      int64_t heads, int64_t dim, int64_t q_stride_b, int64_t q_stride_h,
+                      int64_t q_stride_n, int64_t k_stride_b, int64_t k_stride_h,
+                      int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_h,
+                      int64_t v_stride_n, const int32_t* rowmap, int64_t n_tokens,
+                      int64_t n_video, float scale, float theta, int64_t rank, int64_t group,
+                      int64_t parts, const void* u_hi_t, const void* u_lo_t, const void* u_t,
+                      const uint8_t* partition, const uint8_t* kernel_mask, const void* det,
+                      const float* dl, const float* glref, float alpha_override, void* out,
+                      int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_n,
+                      int64_t split, void* const* stage_events, void* workspace,
+                      int64_t workspace_bytes, void* stream) {
+  return sparse_call(q, k, v, dtype, batch, heads, dim, q_stride_b, q_stride_h, q_stride_n,
+                     k_stride_b, k_stride_h, k_stride_n, v_stride_b, v_stride_h, v_stride_n, rowmap, n_tokens,
+                     n_video, scale, theta, rank, group, parts, u_hi_t, u_lo_t, u_t, partition,
+                     kernel_mask, det, nullptr, dl, glref, alpha_override, out, out_stride_b,
+                     out_stride_h, out_stride_n, split, stage_events, workspace, workspace_bytes,
+                     stream);
+}
+
+int recap_sparse_call_mx(const void* q, const void* k, const void* v, int dtype, int64_t batch,
+                         int64_t heads, int64_t dim, int64_t q_stride_b, int64_t q_stride_h,
+                         int64_t q_stride_n, int64_t k_stride_b, int64_t k_stride_h,
+                         int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_h,
+                         int64_t v_stride_n, const int32_t* rowmap, int64_t n_tokens,
+                         int64_t n_video, float scale, float theta, int64_t rank, int64_t group,
+                         int64_t parts, const void* u_hi_t, const void* u_lo_t, const void* u_t,
+                         const uint8_t* partition, const uint8_t* kernel_mask, const void* det,
+                         const uint8_t* det_scale, const float* dl, const float* glref,
+                         float alpha_override, void* out, int64_t out_stride_b,
+                         int64_t out_stride_h, int64_t out_stride_n, int64_t split,
+                         void* const* stage_events, void* workspace, int64_t workspace_bytes,
+                         void* stream) {
+  REQUIRE(det_scale || n_video < kBlock, "sparse_call_mx: det_scale is NULL");
+  return sparse_call(q, k, v, dtype, batch, heads, dim, q_stride_b, q_stride_h, q_stride_n,
+                     k_stride_b, k_stride_h, k_stride_n, v_stride_b, v_stride_h, v_stride_n, rowmap, n_tokens,
+                     n_video, scale, theta, rank, group, parts, u_hi_t, u_lo_t, u_t, partition,
+                     kernel_mask, det, det_scale, dl, glref, alpha_override, out, out_stride_b,
+                     out_stride_h, out_stride_n, split, stage_events, workspace, workspace_bytes,
+                     stream);
 }
 
 int64_t recap_attn_queue_words(void) { return kQueueWords; }
@@ -856,8 +941,8 @@ static int capture_args(const void* dense_out, int dtype, int64_t batch, int64_t
                         int64_t out_stride_n, const float* dense_lse, const void* head_out,
                         const float* head_lse, const void* go, const float* gl,
                         const int32_t* rowmap, int64_t n_tokens, int64_t n_video, void* det,
-                        float* dl, const float* glref, const float* center, float* stats,
-                        CaptureArgs& a, bool& work) {
+                        uint8_t* det_scale, float* dl, const float* glref, const float* center,
+                        float* stats, CaptureArgs& a, bool& work) {
   CHECK(check_common(dtype, dim));
   CHECK(check_tokens(n_tokens, n_video));
   CHECK(check_qkv("dense_out", dense_out, batch, heads, out_stride_b, out_stride_h, out_stride_n));
@@ -876,23 +961,23 @@ static int capture_args(const void* dense_out, int dtype, int64_t batch, int64_t
   a.go = static_cast<const uint16_t*>(go); a.gl = gl; a.rowmap = rowmap;
   a.heads = (int)heads; a.banks = (int)(batch * heads); a.n_tokens = (int)n_tokens;
   a.rows = (int)g.rows;
-  a.det = static_cast<uint16_t*>(det); a.dl = dl;
+  a.det = det; a.det_scale = det_scale; a.dl = dl;
   a.glref = glref; a.center = center;
   return RECAP_OK;
 }
 
-int recap_refresh_capture(const void* dense_out, int dtype, int64_t batch, int64_t heads,
-                          int64_t dim, int64_t out_stride_b, int64_t out_stride_h,
-                          int64_t out_stride_n, const float* dense_lse, const void* head_out,
-                          const float* head_lse, const void* go, const float* gl,
-                          const int32_t* rowmap, int64_t n_tokens, int64_t n_video, void* det,
-                          float* dl, const float* glref, const float* center,
-                          float* stat_partial, float* stats, void* stream) {
+static int refresh_capture(const void* dense_out, int dtype, int64_t batch, int64_t heads,
+                           int64_t dim, int64_t out_stride_b, int64_t out_stride_h,
+                           int64_t out_stride_n, const float* dense_lse, const void* head_out,
+                           const float* head_lse, const void* go, const float* gl,
+                           const int32_t* rowmap, int64_t n_tokens, int64_t n_video, void* det,
+                           uint8_t* det_scale, float* dl, const float* glref,
+                           const float* center, float* stat_partial, float* stats, void* stream) {
   CaptureArgs a{};
   bool work = false;
   CHECK(capture_args(dense_out, dtype, batch, heads, dim, out_stride_b, out_stride_h,
                      out_stride_n, dense_lse, head_out, head_lse, go, gl, rowmap, n_tokens,
-                     n_video, det, dl, glref, center, stats, a, work));
+                     n_video, det, det_scale, dl, glref, center, stats, a, work));
   const bool validate = glref != nullptr;
   REQUIRE(!validate || stat_partial, "validation needs stat_partial");
   REQUIRE(!validate || (reinterpret_cast<uintptr_t>(stat_partial) & 7) == 0,
@@ -904,6 +989,31 @@ int recap_refresh_capture(const void* dense_out, int dtype, int64_t batch, int64
   CHECK(hip_status(run_capture(a, dtype, (int)dim, &blocks, s), "capture launch"));
   if (validate) CHECK(hip_status(run_sum_pairs(stat_partial, a.banks * blocks, stats, s), "sum_pairs launch"));
   return RECAP_OK;
+}
+
+int recap_refresh_capture(const void* dense_out, int dtype, int64_t batch, int64_t heads,
+                          int64_t dim, int64_t out_stride_b, int64_t out_stride_h,
+                          int64_t out_stride_n, const float* dense_lse, const void* head_out,
+                          const float* head_lse, const void* go, const float* gl,
+                          const int32_t* rowmap, int64_t n_tokens, int64_t n_video, void* det,
+                          float* dl, const float* glref, const float* center,
+                          float* stat_partial, float* stats, void* stream) {
+  return refresh_capture(dense_out, dtype, batch, heads, dim, out_stride_b, out_stride_h,
+                         out_stride_n, dense_lse, head_out, head_lse, go, gl, rowmap, n_tokens, n_video, det,
+                         nullptr, dl, glref, center, stat_partial, stats, stream);
+}
+
+int recap_refresh_capture_mx(const void* dense_out, int dtype, int64_t batch, int64_t heads,
+                             int64_t dim, int64_t out_stride_b, int64_t out_stride_h,
+                             int64_t out_stride_n, const float* dense_lse, const void* head_out,
+                             const float* head_lse, const void* go, const float* gl,
+                             const int32_t* rowmap, int64_t n_tokens, int64_t n_video, void* det,
+                             uint8_t* det_scale, float* dl, const float* glref,
+                             const float* center, float* stat_partial, float* stats, void* stream) {
+  REQUIRE(det_scale || n_video < kBlock, "refresh_capture_mx: det_scale is NULL");
+  return refresh_capture(dense_out, dtype, batch, heads, dim, out_stride_b, out_stride_h,
+                         out_stride_n, dense_lse, head_out, head_lse, go, gl, rowmap, n_tokens, n_video, det,
+                         det_scale, dl, glref, center, stat_partial, stats, stream);
 }
 
 int recap_refresh_capture_noalloc(const void* dense_out, int dtype, int64_t batch,
@@ -918,7 +1028,7 @@ int recap_refresh_capture_noalloc(const void* dense_out, int dtype, int64_t batc
   bool work = false;
   CHECK(capture_args(dense_out, dtype, batch, heads, dim, out_stride_b, out_stride_h,
                      out_stride_n, dense_lse, head_out, head_lse, go, gl, rowmap, n_tokens,
-                     n_video, det, dl, glref, center, stats, a, work));
+                     n_video, det, nullptr, dl, glref, center, stats, a, work));
   const bool validate = glref != nullptr;
   if (validate) {
     const int64_t pairs = recap_capture_partials(batch * heads, dim, n_video);

@@ -35,6 +35,7 @@
 #include <type_traits>
 
 #include "kernels.hpp"
+#include "microscale.hpp"
 
 namespace recap {
 
@@ -154,8 +155,17 @@ __device__ inline void store_rows(const AttnArgs& a, int bank, int b, int h, int
   if (r < a.rows) {
     const int64_t ri = (int64_t)bank * a.rows + r;
     const uint16_t* gorow = a.go + ri * D;
-    const uint16_t* drow = a.det + ri * D;
-    u32x4 gv[NV], dv[NV];
+    // The refinement: fp16, or int8 codes with a unit for every 32 columns.
+    constexpr bool kInt8 = MODE == kModeMergeInt8;
+    const auto* drow = static_cast<const std::conditional_t<kInt8, int8_t, uint16_t>*>(a.det) + ri * D;
+    using Det = std::conditional_t<kInt8, u32x2, u32x4>;  // 8 of them
+    u32x4 gv[NV];
+    Det dv[NV];
+    unsigned units = 0;
+    if constexpr (kInt8) {
+      const uint8_t* at = a.det_scale + ri * (D / kMxBlock);
+      units = D == 128 ? *reinterpret_cast<const unsigned*>(at) : *reinterpret_cast<const uint16_t*>(at);
+    }
     const float glv = a.gl[ri], dlv = a.dl[ri];
     float move = 0.0f;
     if (!a.use_override) {
@@ -169,7 +179,7 @@ __device__ inline void store_rows(const AttnArgs& a, int bank, int b, int h, int
 #pragma unroll
     for (int i = 0; i < NV; ++i) gv[i] = *reinterpret_cast<const u32x4*>(gorow + col(i));
 #pragma unroll
-    for (int i = 0; i < NV; ++i) dv[i] = *reinterpret_cast<const u32x4*>(drow + col(i));
+    for (int i = 0; i < NV; ++i) dv[i] = *reinterpret_cast<const Det*>(drow + col(i));
     asm volatile("" ::: "memory");  // all of them before the first store
     const float admit = a.use_override ? a.alpha_override : expf(-fabsf(move));
     const float cl = glv + dlv;
@@ -188,16 +198,23 @@ __device__ inline void store_rows(const AttnArgs& a, int bank, int b, int h, int
     for (int i = 0; i < NV; ++i) {
       const u32x4 hv = packed(i);
       u32x4 v;
+      const float unit = kInt8 ? mx_int8_unit(units >> (8 * (i / 2)) & 0xff) : 1.0f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         float res[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float gov = T::to_f((uint16_t)(e ? gv[i][w] >> 16 : gv[i][w] & 0xffff));
-          const float detv = f16_to_f((uint16_t)(e ? dv[i][w] >> 16 : dv[i][w] & 0xffff));
+          float detv;
+          if constexpr (kInt8) {
+            detv = mx_int8_code(dv[i], 2 * w + e) * unit;
+          } else {
+            detv = f16_to_f((uint16_t)(e ? dv[i][w] >> 16 : dv[i][w] & 0xffff));
+          }
           const float ohv = T::to_f((uint16_t)(e ? hv[w] >> 16 : hv[w] & 0xffff));
-          const float to = (gov * sm + (gov + detv) * cm) * rden;
-          res[e] = (ohv * wh + to * wt) * rden2;
+          // Written as fmas, so that both forms of the refinement round alike.
+          const float to = fmaf(gov + detv, cm, gov * sm) * rden;
+          res[e] = fmaf(to, wt, ohv * wh) * rden2;
         }
         v[w] = pack2<T>(res[0], res[1]);
       }
@@ -336,7 +353,7 @@ void attention_kernel(AttnArgs a) {
     asm volatile("" : "+s"(args));
     return *(const AttnArgs*)args;
   };
-  constexpr bool kSplits = MODE == kModeHead || MODE == kModeMerge;
+  constexpr bool kSplits = MODE == kModeHead || MODE == kModeMerge || MODE == kModeMergeInt8;
   const int split = kSplits ? a.split : 1;
   const int nlong = a.tb - a.ds, nshort = a.ds;
   const int n_long_items = a.banks * nlong * split;
@@ -909,13 +926,14 @@ static int persistent_grid(int items) {
 
 template <class T, int D>
 static hipError_t launch_attention(const AttnArgs& a, int mode, hipStream_t s) {
-  const bool splits = mode == kModeHead || mode == kModeMerge;
+  const bool splits = mode == kModeHead || mode == kModeMerge || mode == kModeMergeInt8;
   const int items = a.banks * (a.ds + (a.tb - a.ds) * (splits ? a.split : 1));
   const dim3 grid((unsigned)(a.queue != nullptr ? persistent_grid(items) : items)), block(kThreads);
   switch (mode) {
     case kModeHead: hipLaunchKernelGGL((attention_kernel<T, D, kModeHead>), grid, block, 0, s, a); break;
     case kModeDense: hipLaunchKernelGGL((attention_kernel<T, D, kModeDense>), grid, block, 0, s, a); break;
     case kModeDenseHead: hipLaunchKernelGGL((attention_kernel<T, D, kModeDenseHead>), grid, block, 0, s, a); break;
+    case kModeMergeInt8: hipLaunchKernelGGL((attention_kernel<T, D, kModeMergeInt8>), grid, block, 0, s, a); break;
     default: hipLaunchKernelGGL((attention_kernel<T, D, kModeMerge>), grid, block, 0, s, a); break;
   }
   return hipGetLastError();

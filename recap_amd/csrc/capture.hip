@@ -8,13 +8,20 @@
 // (drift weight included) and accumulates sum (old - of)^2 and sum of^2.  The reference
 // adds them with float atomics; here each workgroup writes a partial pair and sum_pairs
 // adds them in a fixed order.  Elementwise, HBM-bound, 16-byte accesses.
+//
+// The refinement is kept as fp16 or as int8 with a scale for every 32 channels (microscale.hpp): the
+// four lanes that hold a block take its largest magnitude and D is rounded once, from fp32, to its
+// codes.  There 1 - ratio is -expm1(lh - lf) and DL = (lf - gl) + ln(1 - ratio), which keep the
+// digits that the difference of two near values in fp32 loses (a row whose head holds all but
+// 4e-4 of the mass: 1.5e-4 off against 1e-7).
 #include <mutex>
 
 #include "kernels.hpp"
+#include "microscale.hpp"
 
 namespace recap {
 
-template <class T, int D>
+template <class T, int D, bool MX>
 __global__ __launch_bounds__(256) void capture_kernel(CaptureArgs a) {
   constexpr int TPR = D / 8, RPB = 256 / TPR;
   __shared__ float red[2][4];
@@ -30,7 +37,7 @@ __global__ __launch_bounds__(256) void capture_kernel(CaptureArgs a) {
   const float glv = a.gl[ri];
   float ratio = expf(fminf(lh - lf, 0.0f));
   ratio = fminf(ratio, 1.0f - 1.0e-6f);
-  const float den = 1.0f - ratio;
+  const float den = MX ? fmaxf(-expm1f(lh - lf), 1.0e-6f) : 1.0f - ratio;
 
   const u32x4 ofw = *reinterpret_cast<const u32x4*>(a.of + b * a.osB + h * a.osH + (int64_t)nat * a.osN + 8 * c);
   const u32x4 ohw = *reinterpret_cast<const u32x4*>(a.oh + ((int64_t)bank * a.n_tokens + r) * D + 8 * c);
@@ -47,7 +54,13 @@ __global__ __launch_bounds__(256) void capture_kernel(CaptureArgs a) {
   const bool validate = a.glref != nullptr;
   float err2 = 0.0f, ref2 = 0.0f;
   if (validate) {
-    const u32x4 dw = *reinterpret_cast<const u32x4*>(a.det + ri * D + 8 * c);
+    float before[8];
+    if constexpr (MX) {
+      mx_int8_values(static_cast<const u32x2*>(a.det)[ri * TPR + c], a.det_scale[(ri * TPR + c) >> 2],
+                     before);
+    } else {
+      load_chunk<F16>(static_cast<const uint16_t*>(a.det) + ri * D, 8 * c, before);
+    }
     const float old_dl = a.dl[ri];
     const float admit = expf(-fabsf(glv - a.glref[ri] - a.center[bank]));
     const float cl = glv + old_dl;
@@ -61,8 +74,7 @@ __global__ __launch_bounds__(256) void capture_kernel(CaptureArgs a) {
     const float mden = fmaxf(wh + wt, 1.0e-30f);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float det = f16_to_f((uint16_t)(dw[e >> 1] >> ((e & 1) * 16)));
-      const float to = (go[e] * sm + (go[e] + det) * cm) / tden;
+      const float to = (go[e] * sm + (go[e] + before[e]) * cm) / tden;
       const float old = (oh[e] * wh + to * wt) / mden;
       err2 += (old - of[e]) * (old - of[e]);
       ref2 += of[e] * of[e];
@@ -70,20 +82,24 @@ __global__ __launch_bounds__(256) void capture_kernel(CaptureArgs a) {
     __syncthreads();  // every old value of this block's rows is read before any write
   }
 
-  unsigned w[4];
+  float v[8];
 #pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    float v[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const float tail = (of[e + u] - ratio * oh[e + u]) / den;
-      float cached = fmaxf(fminf(tail - go[e + u], 6.0e4f), -6.0e4f);
-      v[u] = ratio > 1.0f - 1.0e-3f ? 0.0f : cached;
-    }
-    w[e >> 1] = (unsigned)f_to_f16(v[0]) | ((unsigned)f_to_f16(v[1]) << 16);
+  for (int e = 0; e < 8; ++e) {
+    const float tail = (of[e] - ratio * oh[e]) / den;
+    const float cached = fmaxf(fminf(tail - go[e], 6.0e4f), -6.0e4f);
+    v[e] = ratio > 1.0f - 1.0e-3f ? 0.0f : cached;
   }
-  *reinterpret_cast<u32x4*>(a.det + ri * D + 8 * c) = u32x4{w[0], w[1], w[2], w[3]};
-  if (c == 0) a.dl[ri] = fmaxf(fminf(lf + logf(den) - glv, 30.0f), -30.0f);
+  if constexpr (MX) {
+    const unsigned s = mx_scale<kMxInt8>(quad_max(magnitude_bits(v)));
+    static_cast<u32x2*>(a.det)[ri * TPR + c] = mx_int8_codes(v, s);
+    if ((c & 3) == 0) a.det_scale[(ri * TPR + c) >> 2] = (uint8_t)s;
+  } else {
+    Rounded<F16, 8> r;
+    r.set(v);
+    r.template store<false>(static_cast<uint16_t*>(a.det) + ri * D, 8 * c, 0);
+  }
+  const float mass = MX ? (lf - glv) + logf(den) : lf + logf(den) - glv;
+  if (c == 0) a.dl[ri] = fmaxf(fminf(mass, 30.0f), -30.0f);
 
   if (validate) {
     err2 = wave_sum(err2);
@@ -103,7 +119,12 @@ template <class T, int D>
 static hipError_t launch_capture(const CaptureArgs& a, int* blocks_per_bank, hipStream_t s) {
   constexpr int RPB = 256 / (D / 8);
   *blocks_per_bank = a.rows / RPB;
-  hipLaunchKernelGGL((capture_kernel<T, D>), dim3((unsigned)(a.banks * (a.rows / RPB))), dim3(256), 0, s, a);
+  const dim3 grid((unsigned)(a.banks * (a.rows / RPB)));
+  if (a.det_scale != nullptr) {
+    capture_kernel<T, D, true><<<grid, dim3(256), 0, s>>>(a);
+  } else {
+    capture_kernel<T, D, false><<<grid, dim3(256), 0, s>>>(a);
+  }
   return hipGetLastError();
 }
 

@@ -108,7 +108,8 @@ struct CoarseArgs {
 hipError_t run_coarse(const CoarseArgs& a, int dtype, int dim, hipStream_t s);
 
 // Block-sparse attention (attention.hip).
-enum AttnMode { kModeHead = 0, kModeDense = 1, kModeMerge = 2, kModeDenseHead = 3 };
+// kModeMergeInt8: a merge whose refinement is in int8.
+enum AttnMode { kModeHead = 0, kModeDense = 1, kModeMerge = 2, kModeDenseHead = 3, kModeMergeInt8 = 4 };
 struct AttnArgs {
   const uint16_t* q; int64_t qsB, qsH, qsN;
   const uint16_t* kp; const uint16_t* vp;
@@ -120,7 +121,8 @@ struct AttnArgs {
                                                  // head_out in the query type
   uint16_t* out; int64_t osB, osH, osN;          // dense / dense-head / merge, native order
   float* lse_native;                             // dense / dense-head [bank][N]
-  int rows; const uint16_t* go; const float* gl; const uint16_t* det; const float* dl;
+  int rows; const uint16_t* go; const float* gl; const float* dl;
+  const void* det; const uint8_t* det_scale;     // fp16 values, or int8 codes and their scales
   const float* glref; const float* center; float alpha_override; int use_override;
   // With center null: the coarse tail's partial sums of gl - glref, [bank][rows / 128], from
   // which every wave takes its row's drift centre (the sum of drift_center).
@@ -148,7 +150,8 @@ struct CaptureArgs {
   const uint16_t* go; const float* gl;           // coarse branch [bank][rows](D)
   const int32_t* rowmap;
   int heads, banks, n_tokens, rows;
-  uint16_t* det; float* dl;                      // refinement (fp16 values), in place
+  void* det; float* dl;                          // refinement, in place: fp16 values, or with
+  uint8_t* det_scale;                            // scales int8 codes (microscale.hpp)
   const float* glref; const float* center;       // validation inputs, null = no validation
   float* stat_part;                              // [bank][blocks][2]
 };

@@ -98,13 +98,18 @@ __device__ inline void mx_fp4_values(unsigned w, unsigned s, float (&v)[8]) {
   for (int e = 0; e < 8; ++e) v[e] = s == 255 ? mx_nan() : x[e];
 }
 
+// Code e (0 .. 7, memory order) of eight, and what a code of a block with scale s is worth.
+__device__ inline float mx_int8_code(u32x2 w, int e) {
+  return (float)((int)(w[e >> 2] << (24 - 8 * (e & 3))) >> 24);
+}
+__device__ inline float mx_int8_unit(unsigned s) {
+  return s == 255 ? mx_nan() : ldexpf(1.0f, (int)s - 133);
+}
+
 __device__ inline void mx_int8_values(u32x2 w, unsigned s, float (&v)[8]) {
-  const int down = (int)s - 133;
+  const float unit = mx_int8_unit(s);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int c = (int)(w[e >> 2] << (24 - 8 * (e & 3))) >> 24;
-    v[e] = s == 255 ? mx_nan() : ldexpf((float)c, down);
-  }
+  for (int e = 0; e < 8; ++e) v[e] = mx_int8_code(w, e) * unit;
 }
 
 }  // namespace recap

@@ -1,7 +1,7 @@
 """Refinement banks in pinned host memory, paged to the GPU layer by layer
 (recap/host_banks.py), over the native pager of librecap_hip.so (``recap_pager_*``).
 
-Every (stream, layer) key's bank -- the fp16 refinement, its log-mass, the partition, the
+Every (stream, layer) key's bank -- the fp16 or int8 refinement, its log-mass, the partition, the
 kernel mask and the drift reference, i.e. everything a sparse call of that layer reads --
 lives in pinned host memory the pager allocates.  Device slots (two with prefetch, one
 without) hold the bank of the layer that runs: the pager stages it in on the compute
@@ -17,11 +17,14 @@ import ctypes
 import torch
 
 from . import _lib
+from . import kernels as K
 from .operator import REFRESH, SPARSE, Operator
 
-# The paged fields, in the pager's field order; the last three are the layer's split state.
+# The paged fields, in the pager's field order; the last three are the layer's split state.  An
+# int8 refinement has a sixth.
 FIELDS = ("value", "log_mass", "partition", "head_kernel_mask", "coarse_lse")
 SPLIT = FIELDS[2:]
+SCALE = "value_scale"
 
 
 class _Pager:
@@ -79,6 +82,10 @@ class HostBankOperator(Operator):
 
     # -- geometry of a bank --------------------------------------------------------------
 
+    @property
+    def _fields(self) -> tuple[str, ...]:
+        return FIELDS + (SCALE,) if self.bank_format == "int8" else FIELDS
+
     def _field_specs(self, banks: int, dim: int) -> dict[str, tuple]:
         """Shape and dtype of each paged field (the partition is kept per bank here and
         viewed [B, H, nb, nb] when a layer runs)."""
@@ -86,11 +93,15 @@ class HostBankOperator(Operator):
         n_video = self.layout.video_tokens
         rows, nb = (n_video // block) * block, -(-n_video // block)
         tb = -(-self.layout.tokens // block)
-        return {"value": ((banks, rows, dim), torch.float16),
-                "log_mass": ((banks, rows), torch.float32),
-                "partition": ((banks, nb, nb), torch.bool),
-                "head_kernel_mask": ((banks, tb, tb), torch.bool),
-                "coarse_lse": ((banks, rows), torch.float32)}
+        int8 = self.bank_format == "int8"
+        specs = {"value": ((banks, rows, dim), torch.int8 if int8 else torch.float16),
+                 "log_mass": ((banks, rows), torch.float32),
+                 "partition": ((banks, nb, nb), torch.bool),
+                 "head_kernel_mask": ((banks, tb, tb), torch.bool),
+                 "coarse_lse": ((banks, rows), torch.float32)}
+        if int8:
+            specs[SCALE] = ((banks, rows, dim // K.MX_BLOCK), torch.uint8)
+        return specs
 
     def _setup(self, banks: int, dim: int, device) -> None:
         """A pager and device slots for banks of this geometry.  The geometry is every
@@ -117,7 +128,7 @@ class HostBankOperator(Operator):
                 old = tensors.get(name)
                 if old is None or tuple(old.shape) != tuple(shape) or old.dtype != dtype:
                     tensors[name] = torch.empty(shape, dtype=dtype, device=device)
-            ptrs = (ctypes.c_void_p * len(FIELDS))(*(tensors[n].data_ptr() for n in FIELDS))
+            ptrs = (ctypes.c_void_p * len(specs))(*(tensors[n].data_ptr() for n in specs))
             self._pager("bind", slot, ctypes.cast(ptrs, ctypes.c_void_p))
         self._specs = specs
         self._turn = 0
@@ -167,6 +178,7 @@ class HostBankOperator(Operator):
         nb = slot_tensors["partition"].shape[-1]
         views = dict(slot_tensors, partition=slot_tensors["partition"].view(b, h, nb, nb))
         bank.value, bank.log_mass = views["value"], views["log_mass"]
+        bank.value_scale = views.get(SCALE)
         if load:
             for name in SPLIT:
                 setattr(bank, name, views[name])
@@ -187,7 +199,7 @@ class HostBankOperator(Operator):
                     self._prefetch_next(layer_index, stored_only=True)
         finally:
             self._pager("release", slot, compute)
-            for name in FIELDS:
+            for name in self._fields:
                 setattr(bank, name, None)
         return out
 

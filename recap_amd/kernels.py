@@ -488,22 +488,40 @@ def sparse_merge_attn(q: torch.Tensor, kv: PackedKV, rowmap: torch.Tensor,
                       glref, center, alpha_override: float | None = None,
                       out: torch.Tensor | None = None, balance: bool = True) -> torch.Tensor:
     """Corrected sparse output [B, H, N, d] in native order (one fused kernel); `balance` as
-    for dense_head_attn."""
+    for dense_head_attn.  ``det`` is fp16 [banks, R, d], or an int8 Microscaled of that shape, read
+    in place."""
     _same_type(q, kv)
     b, h, n, d = q.shape
     kernel_mask = kernel_mask.contiguous()
-    if any(t is not None and not t.is_contiguous() for t in (go, gl, det, dl, glref, center)):
+    name, det_args = _refinement("recap_sparse_merge_attn", det, b * h * geo.rows, d, "_ws")
+    if any(t is not None and not t.is_contiguous()
+           for t in (go, gl, None if name.endswith("_mx") else det, dl, glref, center)):
         raise ValueError("merge inputs must be contiguous")
     if out is None:
         out = torch.empty(b, h, n, d, dtype=q.dtype, device=q.device)
     alpha = -1.0 if alpha_override is None else float(alpha_override)
     split, work = _attn_workspace(q, geo)
-    call("recap_sparse_merge_attn_ws", *_qkv_args(q), kv.k_tiles.data_ptr(),
+    call(name, *_qkv_args(q), kv.k_tiles.data_ptr(),
          kv.vt_tiles.data_ptr(), rowmap.data_ptr(), kernel_mask.data_ptr(), n, geo.n_video,
-         float(scale), _p(go), _p(gl), _p(det), _p(dl), _p(glref), _p(center), alpha,
+         float(scale), _p(go), _p(gl), *det_args, _p(dl), _p(glref), _p(center), alpha,
          out.data_ptr(), out.stride(0), out.stride(1), out.stride(2), split, int(balance),
          work.data_ptr(), work.numel(), _stream())
     return out
+
+
+def _refinement(name: str, det, rows: int, dim: int, plain: str = "") -> tuple[str, tuple]:
+    """(entry point, its refinement arguments): fp16 values as they are given, or the codes and
+    scales of an int8 Microscaled with `rows` rows of `dim`."""
+    if not isinstance(det, Microscaled):
+        return name + plain, (_p(det),)
+    if det.format != "int8" or det.width != dim:
+        raise ValueError(f"a refinement is int8 rows of {dim}, got {det.format} rows of {det.width}")
+    specs = _specs((det.codes, det.scales))
+    if _check_microscaled("the refinement", "int8", dim, *specs) != rows:
+        raise ValueError(f"the refinement has {tuple(det.shape)} values, expected {rows} rows of "
+                         f"{dim}")
+    _together({"the refinement's codes": specs[0], "the refinement's scales": specs[1]})
+    return name + "_mx", (det.codes.data_ptr(), det.scales.data_ptr())
 
 
 _MASKS, _HALF, _FLOAT = (torch.bool, torch.uint8), (torch.float16,), (torch.float32,)
@@ -516,12 +534,12 @@ def _sparse_call_bytes(*sizes: int) -> int:
 
 def sparse_call(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rowmap: torch.Tensor,
                 geo: Geometry, scale: float, theta: float, rank: int, tables: BasisTables,
-                partition: torch.Tensor, kernel_mask: torch.Tensor, det: torch.Tensor,
-                dl: torch.Tensor, glref: torch.Tensor, alpha_override: float | None = None,
+                partition: torch.Tensor, kernel_mask: torch.Tensor,
+                det: "torch.Tensor | Microscaled", dl: torch.Tensor, glref: torch.Tensor, alpha_override: float | None = None,
                 out: torch.Tensor | None = None, events=None) -> torch.Tensor:
     """A whole corrected sparse call with a frozen basis in one library call and one
     workspace: kv_pack, closure_tables, coarse_tail and sparse_merge_attn with
-    their outputs bit for bit, in five launches.  ``events``: five timing events recorded
+    their outputs bit for bit, in five launches.  ``det`` as in sparse_merge_attn.  ``events``: five timing events recorded
     before the first stage and after pack, closure (with the tables), coarse and attention."""
     if not q.shape == k.shape == v.shape or not q.dtype == k.dtype == v.dtype:
         raise ValueError("Q, K and V must have the same shape and dtype")
@@ -536,15 +554,17 @@ def sparse_call(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rowmap: torch
         if table.numel() != banks * d * d:
             raise ValueError(f"table {name} has {table.numel()} elements, expected {banks * d * d}")
     rows = banks * geo.rows
+    entry, det_args = _refinement("recap_sparse_call", det, rows, d)
+    half = None if isinstance(det, Microscaled) else det
     for name, t, size, types in (("partition", partition, banks * geo.nb ** 2, _MASKS),
                                  ("kernel_mask", kernel_mask, banks * geo.tb ** 2, _MASKS),
-                                 ("det", det, rows * d, _HALF), ("dl", dl, rows, _FLOAT),
+                                 ("det", half, rows * d, _HALF), ("dl", dl, rows, _FLOAT),
                                  ("glref", glref, rows, _FLOAT)):
-        if t.numel() != size or t.dtype not in types:
+        if t is not None and (t.numel() != size or t.dtype not in types):
             raise ValueError(f"{name} has {t.numel()} {t.dtype} elements, expected {size} of "
                              f"{types[0]}")
     partition, kernel_mask = partition.contiguous(), kernel_mask.contiguous()
-    if not (det.is_contiguous() and dl.is_contiguous() and glref.is_contiguous()):
+    if not all(t is None or t.is_contiguous() for t in (half, dl, glref)):
         raise ValueError("merge inputs must be contiguous")
     if out is None:
         out = torch.empty(b, h, n, d, dtype=q.dtype, device=q.device)
@@ -561,11 +581,11 @@ def sparse_call(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rowmap: torch
         for event in events:
             event.record()   # creates the event; the call records it again at its stage
         handles = (ctypes.c_void_p * 5)(*(event.cuda_event for event in events))
-    call("recap_sparse_call", q.data_ptr(), k.data_ptr(), v.data_ptr(), code, b, h, d,
+    call(entry, q.data_ptr(), k.data_ptr(), v.data_ptr(), code, b, h, d,
          *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], rowmap.data_ptr(), n, geo.n_video,
          float(scale), float(theta), rank, group, parts, tables.u_hi_t.data_ptr(),
          tables.u_lo_t.data_ptr(), tables.u_t.data_ptr(), partition.data_ptr(),
-         kernel_mask.data_ptr(), det.data_ptr(), dl.data_ptr(), glref.data_ptr(),
+         kernel_mask.data_ptr(), *det_args, dl.data_ptr(), glref.data_ptr(),
          -1.0 if alpha_override is None else float(alpha_override), out.data_ptr(),
          *out.stride()[:3], split, handles, work.data_ptr(), size, _stream())
     return out
@@ -577,32 +597,38 @@ def sparse_call(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rowmap: torch
 def _check_capture(dense_out, dense_lse, head_out, head_lse, go, gl, det, dl, glref, center):
     """Argument checks shared by both capture entry points: the kernels read the head and
     coarse outputs as 16-bit values of the dense output's type and the refinement as fp16."""
-    if not all(t.is_contiguous() for t in (dense_lse, head_out, head_lse, go, gl, det, dl)):
+    micro = isinstance(det, Microscaled)
+    if not all(t.is_contiguous() for t in (dense_lse, head_out, head_lse, go, gl, dl)) or not (
+            micro or det.is_contiguous()):
         raise ValueError("capture inputs must be contiguous")
     if head_out.dtype != dense_out.dtype or go.dtype != dense_out.dtype:
         raise ValueError("capture: head and coarse outputs must have the dense output's dtype")
-    if det.dtype != torch.float16 or dl.dtype != torch.float32:
-        raise ValueError("capture: the refinement is fp16 values and fp32 log-masses")
+    if not micro and det.dtype != torch.float16 or dl.dtype != torch.float32:
+        raise ValueError("capture: the refinement is fp16 values (or int8 microscaled ones) and fp32 "
+                         "log-masses")
     if (glref is None) != (center is None):
         raise ValueError("capture: validation needs both glref and center")
 
 
 def refresh_capture(dense_out: torch.Tensor, dense_lse: torch.Tensor, head_out: torch.Tensor,
                     head_lse: torch.Tensor, go: torch.Tensor, gl: torch.Tensor,
-                    rowmap: torch.Tensor, geo: Geometry, det: torch.Tensor, dl: torch.Tensor,
-                    glref: torch.Tensor | None = None, center: torch.Tensor | None = None):
-    """Write the refinement in place; with (glref, center) return the validation pair."""
+                    rowmap: torch.Tensor, geo: Geometry, det: "torch.Tensor | Microscaled",
+                    dl: torch.Tensor, glref: torch.Tensor | None = None,
+                    center: torch.Tensor | None = None):
+    """Write the refinement in place; with (glref, center) return the validation pair.  ``det`` is
+    fp16 [banks, R, d], or an int8 Microscaled of that shape."""
     b, h, n, d = dense_out.shape
     _check_capture(dense_out, dense_lse, head_out, head_lse, go, gl, det, dl, glref, center)
+    name, det_args = _refinement("recap_refresh_capture", det, b * h * geo.rows, d)
     stats = part = None
     if glref is not None:
         npart = int(_lib.load().recap_capture_partials(b * h, d, geo.n_video))
         part = torch.empty(max(1, npart), 2, dtype=torch.float32, device=dense_out.device)
         stats = torch.empty(2, dtype=torch.float32, device=dense_out.device)
-    call("recap_refresh_capture", dense_out.data_ptr(), dtype_code(dense_out.dtype), b, h, d,
+    call(name, dense_out.data_ptr(), dtype_code(dense_out.dtype), b, h, d,
          dense_out.stride(0), dense_out.stride(1), dense_out.stride(2), dense_lse.data_ptr(),
          head_out.data_ptr(), head_lse.data_ptr(), go.data_ptr(), gl.data_ptr(),
-         rowmap.data_ptr(), n, geo.n_video, det.data_ptr(), dl.data_ptr(), _p(glref),
+         rowmap.data_ptr(), n, geo.n_video, *det_args, dl.data_ptr(), _p(glref),
          _p(center), _p(part), _p(stats), _stream())
     return stats
 
@@ -617,6 +643,8 @@ def refresh_capture_noalloc(dense_out: torch.Tensor, dense_lse: torch.Tensor,
     (its validation partials live in a static 4 MiB device array); the caller passes the
     validation pair's output ``stats`` ([2] fp32) when validating."""
     b, h, n, d = dense_out.shape
+    if isinstance(det, Microscaled):
+        raise ValueError("capture: microscaled refinements need refresh_capture")
     _check_capture(dense_out, dense_lse, head_out, head_lse, go, gl, det, dl, glref, center)
     if glref is not None and stats is None:
         raise ValueError("capture: a validating call (glref given) needs the stats output")

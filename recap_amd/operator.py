@@ -105,13 +105,20 @@ class DetailBank:
 
     head_kernel_mask: torch.Tensor | None = None  # [banks, tb, tb] bool
     partition: torch.Tensor | None = None         # [B, H, nb, nb] bool
-    value: torch.Tensor | None = None             # [banks, rows, dim] fp16
+    value: torch.Tensor | None = None             # [banks, rows, dim] fp16, or int8 codes
     log_mass: torch.Tensor | None = None          # [banks, rows] fp32
     coarse_lse: torch.Tensor | None = None        # [banks, rows] fp32
     valid: bool = False
     refreshed_at: int = 0
     pending_stats: torch.Tensor | None = None     # [2] fp32: sum sq error, sum sq output
     pending_age: int | None = None
+    value_scale: torch.Tensor | None = None       # [banks, rows, dim / 32]: of int8 codes
+
+    def refinement(self) -> "torch.Tensor | K.Microscaled | None":
+        """The refinement values as the kernels take them: fp16, or int8 with their scales."""
+        if self.value is None or self.value_scale is None:
+            return self.value
+        return K.Microscaled(self.value, self.value_scale, "int8", self.value.shape[-1])
 
     def release(self) -> None:
         """Forget the refinement: every field back to its declared default."""
@@ -125,11 +132,12 @@ class DetailBank:
         return None if stats is None or age is None else (stats, int(age))
 
     def refinement_bytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.value, self.log_mass)
-                   if t is not None)
+        return sum(t.numel() * t.element_size()
+                   for t in (self.value, self.value_scale, self.log_mass) if t is not None)
 
 
-_BANK_TENSORS = ("head_kernel_mask", "partition", "value", "log_mass", "coarse_lse")
+_BANK_TENSORS = ("head_kernel_mask", "partition", "value", "value_scale", "log_mass", "coarse_lse")
+BANK_FORMATS = ("fp16", "int8")
 
 
 @dataclass(frozen=True)
@@ -222,6 +230,9 @@ class Operator:
     _chunk_states: dict = field(default_factory=dict)
     _forced_partition: torch.Tensor | None = None
     _forced_rerank: bool | None = None
+    #: how a refresh keeps its refinement: "fp16", as the reference does, or "int8", microscaled
+    #: (half the memory, the paging and the reading; each value within half a step of its block)
+    bank_format: str = "fp16"
 
     # The per-(stream, layer) state is a grid of cells: the sparse state in ``layers`` and
     # the refinement in ``banks``, both indexed [stream][layer] (the reference's indexing,
@@ -232,17 +243,19 @@ class Operator:
         rows = self.layers
         if not rows or not all(isinstance(row, (list, tuple)) and row for row in rows):
             raise TypeError("Operator.layers must be indexed [stream][layer]")
+        if self.bank_format not in BANK_FORMATS:
+            raise ValueError(f"unknown bank_format {self.bank_format!r}; use one of {BANK_FORMATS}")
         self.banks = [[DetailBank() for _ in row] for row in rows]
 
     @classmethod
     def build(cls, config: OperatorConfig, geometry: SparseGeometry, *, n_layers: int,
-              n_streams: int = 1) -> "Operator":
+              n_streams: int = 1, bank_format: str = "fp16") -> "Operator":
         """A fresh sparse state in every cell (recap/operator.py:176-191)."""
         if min(n_layers, n_streams) < 1:
             raise ValueError("n_layers and n_streams must be positive")
         grid = [[SparseAttention(geometry, config) for _ in range(n_layers)]
                 for _ in range(n_streams)]
-        return cls(config, geometry.layout, grid)
+        return cls(config, geometry.layout, grid, bank_format=bank_format)
 
     @property
     def n_streams(self) -> int:
@@ -424,11 +437,15 @@ class Operator:
         go, gl, drift_part = layer.coarse_tail_apply(q, rowmap, context, flat_part, geo, scale,
                                                      glref=old_lse)
         if bank.value is None:
-            bank.value = torch.empty(banks, geo.rows, d, dtype=torch.float16, device=q.device)
+            if self.bank_format == "int8":
+                made = K.Microscaled.empty((banks, geo.rows, d), "int8", q.device)
+                bank.value, bank.value_scale = made.codes, made.scales
+            else:
+                bank.value = torch.empty(banks, geo.rows, d, dtype=torch.float16, device=q.device)
             bank.log_mass = torch.empty(banks, geo.rows, dtype=torch.float32, device=q.device)
         center = K.drift_center(drift_part, geo) if old_lse is not None else None
         stats = K.refresh_capture(full_output, full_lse, head_out, head_lse, go, gl, rowmap, geo,
-                                  bank.value, bank.log_mass, glref=old_lse, center=center)
+                                  bank.refinement(), bank.log_mass, glref=old_lse, center=center)
         if stats is not None:
             bank.pending_stats = stats
             bank.pending_age = self.step - bank.refreshed_at
@@ -457,7 +474,7 @@ class Operator:
             go, gl, _ = layer.coarse_tail_apply(
                 q, rowmap, context, bank.partition.reshape(banks, geo.nb, geo.nb), geo, scale)
             K.refresh_capture(full_output, full_lse, head_out, head_lse, go, gl, rowmap, geo,
-                              bank.value, bank.log_mass)
+                              bank.refinement(), bank.log_mass)
         bank.coarse_lse = gl.clone()
         bank.refreshed_at = self.step
         bank.valid = True
@@ -484,8 +501,8 @@ class Operator:
             return K.sparse_call(
                 q, k, v, rowmap, geo, scale, self.config.closure_gate_theta,
                 int(self.config.closure_rank), layer.tables,
-                bank.partition.reshape(banks, geo.nb, geo.nb), bank.head_kernel_mask, bank.value,
-                bank.log_mass, bank.coarse_lse, self.alpha_override, out, events)
+                bank.partition.reshape(banks, geo.nb, geo.nb), bank.head_kernel_mask,
+                bank.refinement(), bank.log_mass, bank.coarse_lse, self.alpha_override, out, events)
 
         # No basis yet (a bank that was handed in): stage by stage, the basis from these keys.
         def mark(stage: str) -> None:
@@ -504,7 +521,7 @@ class Operator:
         center = K.drift_center(drift_part, geo) if geo.rows else None
         mark("coarse")
         out = K.sparse_merge_attn(q, kv, rowmap, bank.head_kernel_mask, geo, scale, go, gl,
-                                  bank.value, bank.log_mass, old_lse, center,
+                                  bank.refinement(), bank.log_mass, old_lse, center,
                                   alpha_override=self.alpha_override, out=out)
         mark("attention")
         return out

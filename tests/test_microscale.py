@@ -137,3 +137,35 @@ def test_the_definition(format):
     codes = M.pack(index, negative, format)
     assert all(torch.equal(a, b) for a, b in zip(M.unpack(codes, format), (
         index, negative if format == "fp4" else negative & (index > 0))))
+
+
+@pytest.mark.parametrize("name,args,match", [
+    ("recap_refresh_capture_mx", [64, 2, 1, 2, 64, 64, 64, 64, *[64] * 6, 256, 256, 64, None, 64,
+                                  *[None] * 5], "det_scale is NULL"),
+    ("recap_refresh_capture_mx", [64, 2, 1, 2, 64, 64, 64, 64, *[64] * 6, 256, 256, 72, 64, 64,
+                                  *[None] * 5], "alignment"),
+    ("recap_sparse_merge_attn_mx", [64, 2, 1, 2, 64, 64, 64, 64, *[64] * 4, 256, 256, 0.125, 64, 64,
+                                    64, None, 64, 64, 64, -1.0, 64, 64, 64, 64, 1, 1, 64, 1 << 30,
+                                    None], "det_scale is NULL"),
+    ("recap_sparse_merge_attn_mx", [64, 2, 1, 2, 64, 64, 64, 64, *[64] * 4, 256, 256, 0.125, 64, 64,
+                                    64, 66, 64, 64, 64, -1.0, 64, 64, 64, 64, 1, 1, 64, 1 << 30,
+                                    None], "4-byte aligned"),
+    ("recap_sparse_call_mx", [64, 64, 64, 2, 1, 2, 64, *[64] * 9, 64, 256, 256, 0.125, 2.0, 4, 8, 1,
+                              *[64] * 6, None, 64, 64, -1.0, 64, 64, 64, 64, 1, None, 64, 1 << 30,
+                              None], "det_scale is NULL")])
+def test_c_refinement_refusals(name, args, match):
+    with pytest.raises(ValueError, match=match):
+        _lib.call(name, *args)
+
+
+def test_bank_format_is_checked():
+    from recap_amd import HostBankOperator, Operator, OperatorConfig
+    from recap_amd.layout import Layout, SparseGeometry, hilbert_permutation
+
+    geometry = SparseGeometry.build(Layout.from_permutation(hilbert_permutation((2, 8, 16)),
+                                                            text_tokens=0, text_first=False), 128)
+    for cls in (Operator, HostBankOperator):
+        assert cls.build(OperatorConfig(), geometry, n_layers=1).bank_format == "fp16"
+        assert cls.build(OperatorConfig(), geometry, n_layers=1, bank_format="int8").bank_format == "int8"
+        with pytest.raises(ValueError, match="bank_format"):
+            cls.build(OperatorConfig(), geometry, n_layers=1, bank_format="fp4")
