@@ -5,6 +5,11 @@
 // bytes of row l % 32, block l / 32, and that block's scale byte, which the instruction applies to
 // the block's sum.  Products of codes are exact; sums are fp32 and rounded once, after the bias.
 // Weight rows are the A operand, so that a lane ends with consecutive outputs of one row of x.
+//
+// Bound by power, then by the copies: from registers the instruction reaches 6.5 PFLOP/s on random
+// codes (10.0 on zeros); 8,192^3 takes 278 us, 3.95 PFLOP/s, and 215 us, 5.1, without the copies into
+// LDS.  118,800 x 2,048 to 8,192 outputs: 1,188 us, 3.36 PFLOP/s, of which a seventh goes to the tiles'
+// starts and stores.  (A library's bf16 product of 8,192^3: 1.2 PFLOP/s.)
 #include <algorithm>
 
 #include "kernels.hpp"
@@ -34,6 +39,19 @@ __device__ inline void step_barrier() {
   asm volatile("" ::: "memory");
 }
 
+// Copies 16 bytes a lane (4: copy_to_lds4) of a buffer of `bytes` bytes, from `at` (of the lane) +
+// `offset` on, into LDS from `dst` on, lane after lane.
+__device__ inline void copy_to_lds(const uint8_t* base, int bytes, char* dst, int at, int offset) {
+  const __amdgpu_buffer_rsrc_t r =
+      __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes, kBufferRsrcWord3);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)dst, 16, at, offset, 0, 0);
+}
+__device__ inline void copy_to_lds4(const uint8_t* base, int bytes, char* dst, int at, int offset) {
+  const __amdgpu_buffer_rsrc_t r =
+      __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes, kBufferRsrcWord3);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)dst, 4, at, offset, 0, 0);
+}
+
 __device__ inline float load_bias(const MxProductArgs& a, int n) {
   if (a.bias_dtype == F32::code) return load_elem<F32>(a.bias, n);
   return a.bias_dtype == BF16::code ? load_elem<BF16>(a.bias, n) : load_elem<F16>(a.bias, n);
@@ -49,133 +67,217 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(MxProductArgs a, 
   __shared__ __attribute__((aligned(16))) char x1[BM * kStepBytes];
   __shared__ __attribute__((aligned(16))) char w0[BN * kStepBytes];
   __shared__ __attribute__((aligned(16))) char w1[BN * kStepBytes];
-  __shared__ __attribute__((aligned(16))) char xs0[BM * kStepScales];
-  __shared__ __attribute__((aligned(16))) char xs1[BM * kStepScales];
-  __shared__ __attribute__((aligned(16))) char ws0[BN * kStepScales];
-  __shared__ __attribute__((aligned(16))) char ws1[BN * kStepScales];
+  __shared__ __attribute__((aligned(16))) char s0[(BM + BN) * kStepScales];  // of x, then of w
+  __shared__ __attribute__((aligned(16))) char s1[(BM + BN) * kStepScales];
+  __shared__ __attribute__((aligned(16))) float bias[BN];
 
   const int t = threadIdx.x, lane = t & 63, g = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int wm = wave % WM, wn = wave / WM;
+  // An XCD's workgroups take neighbouring tiles, kBand rows of tiles deep: those in flight on it read
+  // few distinct rows of either operand, which its L2 holds.
+  constexpr int kBand = 8;
   const int item = xcd_linear(blockIdx.x, tiles_m * tiles_n);
-  const int tn = item % tiles_n, tm = item / tiles_n;
+  const int band = item / (kBand * tiles_n), place = item - band * kBand * tiles_n;
+  const int deep = min(kBand, tiles_m - band * kBand);
+  const int tn = place / deep, tm = band * kBand + place - tn * deep;
   const int m0 = tm * BM, n0 = tn * BN;
   const int pitch = a.steps * kStepBytes, spitch = a.steps * kStepScales;
 
-  // Copies into LDS go 16 bytes a lane (4 for scales) in lane order; rows are 8 chunks whose order
-  // is exchanged by row, so that the lanes of a fragment read distinct banks.
-  const auto resource = [](const uint8_t* base, int64_t row, int rows, int pitch) {
-    return __builtin_amdgcn_make_buffer_rsrc((void*)(base + row * pitch), 0, rows * pitch,
-                                             kBufferRsrcWord3);
-  };
+  for (int i = t; i < BN; i += kThreads)
+    bias[i] = a.bias != nullptr && n0 + i < a.outputs ? load_bias(a, n0 + i) : 0.0f;
+
+  // Copies into LDS go 16 bytes a lane (4 for scales) in lane order, 8 rows (32) an instruction.  A
+  // row's 8 chunks are exchanged by row, so that the lanes of a fragment read distinct banks.  Rows
+  // past the last are copies of it and not stored.
+  constexpr int kWaves = kThreads / 64, CX = BM / 8 / kWaves, CW = BN / 8 / kWaves;
+  static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0 && kWaves % 2 == 0, "tile");
   const int mrows = min(BM, a.rows - m0), nrows = min(BN, a.outputs - n0);
-  const __amdgpu_buffer_rsrc_t xr = resource(a.x, m0, mrows, pitch);
-  const __amdgpu_buffer_rsrc_t wr = resource(a.w, n0, nrows, pitch);
-  const __amdgpu_buffer_rsrc_t xsr = resource(a.x_scales, m0, mrows, spitch);
-  const __amdgpu_buffer_rsrc_t wsr = resource(a.w_scales, n0, nrows, spitch);
-
-  const auto copy = [&](const __amdgpu_buffer_rsrc_t& r, char* dst, int rows, int live, int step) {
-    for (int i = wave; i < rows / 8; i += kThreads / 64) {
-      const int row = 8 * i + (lane >> 3);
-      const int chunk = (lane & 7) ^ TileGeom<64>::swz(row, 8);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(dst + i * 1024), 16,
-                                               min(row, live - 1) * pitch + chunk * 16,
-                                               step * kStepBytes, 0, 0);
-    }
-  };
-  const auto copy_scales = [&](const __amdgpu_buffer_rsrc_t& r, char* dst, int rows, int live,
-                               int step) {
-    for (int i = wave; i < rows / 32; i += kThreads / 64) {
-      const int row = 32 * i + (lane >> 1);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(dst + i * 256), 4,
-                                               min(row, live - 1) * spitch + (lane & 1) * 4,
-                                               step * kStepScales, 0, 0);
-    }
-  };
-
-  f32x16 acc[FN][FM] = {};
-  const auto multiply = [&](const char* x, const char* w, const char* xs, const char* ws) {
-    unsigned sx[FM], sw[FN];
+  const int first = 8 * wave + (lane >> 3), chunk = 16 * ((lane & 7) ^ TileGeom<64>::swz(first, 8));
+  int x_at[CX], w_at[CW];
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
-      sx[i] = *reinterpret_cast<const unsigned*>(xs + ((wm * FM + i) * 32 + l32) * kStepScales + 4 * g);
+  for (int i = 0; i < CX; ++i) x_at[i] = min(first + 8 * kWaves * i, mrows - 1) * pitch + chunk;
 #pragma unroll
-    for (int j = 0; j < FN; ++j)
-      sw[j] = *reinterpret_cast<const unsigned*>(ws + ((wn * FN + j) * 32 + l32) * kStepScales + 4 * g);
-    const auto fragment = [&](const char* base, int first, int s) {
-      const int row = first + l32;
-      return lds_load16(base, row * kStepBytes + (((4 * g + s) ^ TileGeom<64>::swz(row, 8)) << 4));
-    };
-    const auto block = [&](auto s) {
-      constexpr int S = decltype(s)::value;
-      u32x4 fx[FM], fw[FN];
+  for (int i = 0; i < CW; ++i) w_at[i] = min(first + 8 * kWaves * i, nrows - 1) * pitch + chunk;
+  const uint8_t* const xb = a.x + (int64_t)m0 * pitch;
+  const uint8_t* const wb = a.w + (int64_t)n0 * pitch;
+  const uint8_t* const xsb = a.x_scales + (int64_t)m0 * spitch;
+  const uint8_t* const wsb = a.w_scales + (int64_t)n0 * spitch;
+  const auto fetch = [&](char* x, char* w, char* scales, int step) {
 #pragma unroll
-      for (int j = 0; j < FN; ++j) fw[j] = fragment(w, (wn * FN + j) * 32, S);
+    for (int i = 0; i < CX; ++i)
+      copy_to_lds(xb, mrows * pitch, x + 1024 * (wave + kWaves * i), x_at[i], step * kStepBytes);
 #pragma unroll
-      for (int i = 0; i < FM; ++i) fx[i] = fragment(x, (wm * FM + i) * 32, S);
+    for (int i = 0; i < CW; ++i)
+      copy_to_lds(wb, nrows * pitch, w + 1024 * (wave + kWaves * i), w_at[i], step * kStepBytes);
 #pragma unroll
-      for (int j = 0; j < FN; ++j)
-#pragma unroll
-        for (int i = 0; i < FM; ++i) acc[j][i] = mfma_fp4<S>(fw[j], fx[i], acc[j][i], sw[j], sx[i]);
-    };
-    block(std::integral_constant<int, 0>());
-    block(std::integral_constant<int, 1>());
-    block(std::integral_constant<int, 2>());
-    block(std::integral_constant<int, 3>());
-  };
-  const auto fetch0 = [&](int step) {
-    copy(xr, x0, BM, mrows, step);
-    copy(wr, w0, BN, nrows, step);
-    copy_scales(xsr, xs0, BM, mrows, step);
-    copy_scales(wsr, ws0, BN, nrows, step);
-  };
-  const auto fetch1 = [&](int step) {
-    copy(xr, x1, BM, mrows, step);
-    copy(wr, w1, BN, nrows, step);
-    copy_scales(xsr, xs1, BM, mrows, step);
-    copy_scales(wsr, ws1, BN, nrows, step);
-  };
-
-  fetch0(0);
-  for (int step = 0; step < a.steps; step += 2) {
-    step_barrier();
-    if (step + 1 < a.steps) fetch1(step + 1);
-    multiply(x0, w0, xs0, ws0);
-    if (step + 1 >= a.steps) break;
-    step_barrier();
-    if (step + 2 < a.steps) fetch0(step + 2);
-    multiply(x1, w1, xs1, ws1);
-  }
-
-  // Lane (g, l32) of fragment (j, i) holds outputs 8 q + 4 g .. + 3 of row l32.
-#pragma unroll
-  for (int j = 0; j < FN; ++j)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int n = n0 + (wn * FN + j) * 32 + 8 * q + 4 * g;
-      float b[4] = {};
-      if (a.bias != nullptr)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) b[e] = n + e < a.outputs ? load_bias(a, n + e) : 0.0f;
-#pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        const int m = m0 + (wm * FM + i) * 32 + l32;
-        if (m >= a.rows) continue;
-        const int64_t to = m * a.stride + n;
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[j][i][4 * q + e] + b[e];
-        if (n + 4 <= a.outputs) {
-          Rounded<O, 4> r;
-          r.set(v);
-          r.template store<false>(const_cast<void*>(row_of<O>(a.out, to)), 0, 0);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < a.outputs) store_elem<O>(a.out, to + e, v[e]);
-        }
+    for (int i = 0; i < (BM + BN) / 32; i += kWaves) {
+      const int at = i + wave;  // 32 rows of scales
+      if (at < (BM + BN) / 32) {
+        const bool of_x = at < BM / 32;
+        const int rows = of_x ? mrows : nrows;
+        const int row = min(32 * (of_x ? at : at - BM / 32) + (lane >> 1), rows - 1);
+        copy_to_lds4(of_x ? xsb : wsb, rows * spitch, scales + 256 * at,
+                     row * spitch + (lane & 1) * 4, step * kStepScales);
       }
     }
+  };
+
+  // The reduction goes block pair by block pair, four a step; the fragments of the next pair are read
+  // from LDS while this one's are multiplied, over the barrier between two steps too.
+  f32x16 acc[FN][FM];
+  u32x4 fx[2][FM], fw[2][FN];
+  unsigned sx[2][FM], sw[2][FN];
+  const int row_x = wm * FM * 32 + l32, row_w = wn * FN * 32 + l32;
+  const int swz = TileGeom<64>::swz(l32, 8);
+  const auto read = [&](int set, const char* x, const char* w, int s) {
+    const int at = ((4 * g + s) ^ swz) << 4;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) fw[set][j] = lds_load16(w, (row_w + 32 * j) * kStepBytes + at);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) fx[set][i] = lds_load16(x, (row_x + 32 * i) * kStepBytes + at);
+  };
+  const auto read_scales = [&](int set, const char* scales) {
+    const auto word = [&](int row) {
+      return *reinterpret_cast<const unsigned*>(scales + row * kStepScales + 4 * g);
+    };
+#pragma unroll
+    for (int j = 0; j < FN; ++j) sw[set][j] = word(BM + row_w + 32 * j);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) sx[set][i] = word(row_x + 32 * i);
+  };
+  const auto multiply = [&](auto s, int scales) {
+    constexpr int S = decltype(s)::value;
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+        acc[j][i] = mfma_fp4<S>(fw[S & 1][j], fx[S & 1][i], acc[j][i], sw[scales][j], sx[scales][i]);
+  };
+  // One step from the buffers (x, w), its first pair already read; then the next step's is.  The
+  // scheduler would put a pair's reads behind the products they are to run beside.
+  const auto advance = [&](char* x, char* w, char* scales, const char* next_x, const char* next_w,
+                           const char* next_scales, int set, int step) {
+    const auto pair = [&](auto s) {
+      read(1 - (decltype(s)::value & 1), x, w, decltype(s)::value + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(s, set);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    pair(std::integral_constant<int, 0>());
+    pair(std::integral_constant<int, 1>());
+    pair(std::integral_constant<int, 2>());
+    // Opaque: the compiler otherwise moves all products behind the branch below, their fragments
+    // kept in registers until then.
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int i = 0; i < FM; ++i) asm volatile("" : "+v"(acc[j][i]));
+    step_barrier();
+    read_scales(1 - set, next_scales);
+    read(0, next_x, next_w, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    if (step + 2 < a.steps) fetch(x, w, scales, step + 2);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(std::integral_constant<int, 3>(), set);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  // The sums start from the bias.
+  const auto start = [&]() {
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 b = *reinterpret_cast<const f32x4*>(bias + (wn * FN + j) * 32 + 8 * q + 4 * g);
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][i][4 * q + e] = b[e];
+      }
+  };
+
+  // An odd step comes first, through the second buffer: behind the loop its sums would need
+  // registers of their own.
+  const int odd = a.steps & 1;
+  if (odd) {
+    fetch(x1, w1, s1, 0);
+    step_barrier();
+    start();
+    if (a.steps > 1) fetch(x0, w0, s0, 1);
+    read_scales(1, s1);
+    read(0, x1, w1, 0);
+    advance(x1, w1, s1, x0, w0, s0, 1, 0);
+  } else {
+    fetch(x0, w0, s0, 0);
+    step_barrier();
+    start();
+    fetch(x1, w1, s1, 1);
+    read_scales(0, s0);
+    read(0, x0, w0, 0);
+  }
+  for (int step = odd; step < a.steps; step += 2) {
+    advance(x0, w0, s0, x1, w1, s1, 0, step);
+    advance(x1, w1, s1, x0, w0, s0, 1, step + 1);
+  }
+
+  // Lane (g, l32) of fragment (j, i) holds outputs 8 q + 4 g .. + 3 of row l32: stored from there, a
+  // line of memory would be written in eight parts.  The wave passes its part of the tile, 128 bytes
+  // of every row at a time, through LDS of its own (its chunks exchanged by row as above), and stores
+  // whole lines.
+  constexpr int kSize = kBytes<O>, kFrags = 4 / kSize;  // fragments in 128 bytes
+  static_assert(FN % kFrags == 0, "passes");
+  constexpr int kRegion = FM * 32 * 128;
+  constexpr int kInX = BM * kStepBytes / kRegion, kInW = BN * kStepBytes / kRegion;
+  static_assert(2 * (kInX + kInW) >= kWaves, "room");
+  char* const region = wave < kInX            ? x0 + wave * kRegion
+                       : wave < 2 * kInX      ? x1 + (wave - kInX) * kRegion
+                       : wave < 2 * kInX + kInW ? w0 + (wave - 2 * kInX) * kRegion
+                                              : w1 + (wave - 2 * kInX - kInW) * kRegion;
+#pragma unroll
+  for (int pass = 0; pass < FN / kFrags; ++pass) {
+#pragma unroll
+    for (int f = 0; f < kFrags; ++f)
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x16& v = acc[pass * kFrags + f][i];
+          const int row = 32 * i + l32;
+          if constexpr (kSize == 2) {
+            const int at = row * 128 + (((4 * f + q) ^ swz) << 4) + 8 * g;
+            *reinterpret_cast<u32x2*>(region + at) = u32x2{
+                pack2<O>(v[4 * q], v[4 * q + 1]), pack2<O>(v[4 * q + 2], v[4 * q + 3])};
+          } else {
+            const int at = row * 128 + (((2 * q + g) ^ swz) << 4);
+            *reinterpret_cast<f32x4*>(region + at) =
+                f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+          }
+        }
+    asm volatile("" ::: "memory");
+    const int n = n0 + (wn * FN + pass * kFrags) * 32 + (lane & 7) * (16 / kSize);
+#pragma unroll
+    for (int r = 0; r < FM * 32; r += 8) {
+      const int row = r + (lane >> 3), m = m0 + wm * FM * 32 + row;
+      const u32x4 v = lds_load16(region, row * 128 + (((lane & 7) ^ TileGeom<64>::swz(row, 8)) << 4));
+      if (m >= a.rows || n >= a.outputs) continue;
+      const int64_t to = m * a.stride + n;
+      if (n + 16 / kSize <= a.outputs) {
+        store_words4<false>(const_cast<void*>(row_of<O>(a.out, to)), v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16 / kSize; ++e)
+          if (n + e < a.outputs) {
+            if constexpr (kSize == 2) {
+              static_cast<uint16_t*>(a.out)[to + e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+            } else {
+              static_cast<unsigned*>(a.out)[to + e] = v[e];
+            }
+          }
+      }
+    }
+    asm volatile("" ::: "memory");
+  }
 }
 
 template <class O, int BM, int BN, int WM, int WN>
@@ -186,9 +288,21 @@ hipError_t launch(const MxProductArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
+// The largest tile whose rounds over the 256 CUs are worth its size.  A tile of 256 x 256 takes as
+// long as 2.9 of 128 x 128 (two of which a CU holds at once) where it would take four by its work;
+// us at 8 steps, rows x outputs, 256 / 128 / 64 wide: 118,800 x 8,192 1,188 / 1,560 / -;
+// 4,600 x 2,048 (144 tiles of 256) 18.4 / 21.1 / 26.7; 19,200 x 1,024 (300) 35.8 / 33.8 / 45.5;
+// 3,000 x 2,048 (96) 17.0 / 13.6 / 18.1; 1,500 x 2,048 15.9 / 9.3 / 10.1; 256 x 2,048
+// 15.0 / 7.3 / 6.3; 512 x 2,048 at 32 steps 49.7 / 30.2 / 20.7.
 template <class O>
 hipError_t launch_type(const MxProductArgs& a, hipStream_t s) {
-  return launch<O, 128, 128, 2, 2>(a, s);
+  const auto tiles = [&](int64_t side) {
+    return ((a.rows + side - 1) / side) * ((a.outputs + side - 1) / side);
+  };
+  const auto rounds = [&](int64_t side) { return (double)((tiles(side) + 255) / 256); };
+  if (a.rows <= 64 || a.outputs <= 64 || tiles(64) <= 512) return launch<O, 64, 64, 2, 1>(a, s);
+  if (2.9 * rounds(256) < rounds(128) + 0.4) return launch<O, 256, 256, 4, 2>(a, s);
+  return launch<O, 128, 128, 4, 2>(a, s);
 }
 
 }  // namespace

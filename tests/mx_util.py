@@ -80,12 +80,13 @@ def check_product(got, x, w, bias, label: str) -> None:
     of the magnitudes."""
     want, size = x @ w.T, x.abs() @ w.abs().T
     if bias is not None:
-        want, size = want + bias.cpu().double(), size + bias.cpu().double().abs()
+        bias = bias.to(want.device).double()
+        want, size = want + bias, size + bias.abs()
     limit = (x.shape[-1] + 1) * 2.0 ** -23 * size
     info = torch.finfo(got.dtype)
     limit = limit + ((want.abs() + limit) * (info.eps / 2)).clamp_min(info.smallest_normal * info.eps / 2)
     assert got.shape == want.shape, label
-    got = got.cpu().double()
+    got = got.to(want.device).double()
     assert torch.equal(torch.isnan(got), torch.isnan(want)), f"{label}: NaN"
     ok = ~torch.isnan(want)
     off = ((got - want).abs() / limit)[ok]

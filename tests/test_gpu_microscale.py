@@ -166,6 +166,29 @@ def test_products(cuda, rows, width, outputs, dtype, out):
     M.check_product(plain, xq, wq, None, "no bias")
 
 
+# Sizes that take tiles of 128 and of 256, with one, an odd and an even number of steps of the sum.
+@pytest.mark.parametrize("rows,width,outputs", [
+    (2300, 200, 1100), (2301, 700, 1129), (2304, 1024, 1152), (1999, 1793, 1283), (8193, 256, 1030),
+    (8200, 513, 1001), (4099, 1000, 2111), (12288, 2048, 1024), (16400, 1155, 999), (70, 2100, 70000)])
+@pytest.mark.parametrize("out", [BF, FP, F32], ids=str)
+def test_large_products(cuda, rows, width, outputs, out):
+    print(f"case {rows} {width} {outputs}", flush=True)
+    x = make(20, rows, width, dtype=out, spread=0.5)
+    weight = K.mx_quantise(make(21, outputs, width, dtype=F32, spread=0.5) / width ** 0.5)
+    bias, kept = make(22, outputs, dtype=out), K.mx_quantise(x)
+    got = K.mx_linear(kept, weight, bias, dtype=out)
+    values = [K.mx_dequantise(m, F32).double() for m in (kept, weight)]
+    for first in range(0, rows, 4096):
+        part = slice(first, first + 4096)
+        M.check_product(got[part], values[0][part], values[1], bias, f"rows from {first}")
+    assert torch.equal(K.mx_linear(x, weight, bias), got)
+    # in place of another tensor's columns, whose neighbours stay
+    frame = torch.full((rows, outputs + 21), 5.0, dtype=out, device="cuda")
+    K.mx_linear(kept, weight, bias, dtype=out, out=frame[:, 11:11 + outputs])
+    assert torch.equal(frame[:, 11:11 + outputs], got)
+    assert (frame[:, :11] == 5).all() and (frame[:, 11 + outputs:] == 5).all()
+
+
 @pytest.mark.parametrize("rows,width,outputs", [(1, 512, 512), (40, 300, 90), (300, 512, 300)])
 def test_products_of_scales(cuda, rows, width, outputs):
     """Blocks far apart in size, and NaN rows that stay in their row or column."""
