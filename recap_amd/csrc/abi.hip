@@ -1510,8 +1510,9 @@ int recap_mx_linear(const void* x, int x_dtype, int64_t x_stride, const uint8_t*
   REQUIRE(rows == 1 || out_stride >= outputs, "mx_linear: row stride %lld lets rows of %lld overlap",
           (long long)out_stride, (long long)outputs);
   hipStream_t s = as_stream(stream);
-  const uint8_t* codes = static_cast<const uint8_t*>(x);
-  const uint8_t* scales = x_scales;
+  MxProductArgs a{static_cast<const uint8_t*>(x), x_scales, static_cast<const uint8_t*>(weight),
+                  weight_scales, bias, bias_dtype, out, out_stride, (int)rows, (int)outputs,
+                  (int)(mx_filled(kMxFp4, width) / mx_fill(kMxFp4))};
   if (x_scales != nullptr) {
     REQUIRE(aligned16(x) && aligned8(x_scales),
             "mx_linear: x's codes must be 16-byte and its scales 8-byte aligned");
@@ -1524,14 +1525,14 @@ int recap_mx_linear(const void* x, int x_dtype, int64_t x_stride, const uint8_t*
     uint8_t* space = static_cast<uint8_t*>(workspace);
     uint8_t* space_scales = space + rows * mx_row_bytes(kMxFp4, width);
     CHECK(check_mx_rows("mx_linear", x, x_dtype, rows, width, x_stride, false, space, space_scales));
+    if (mx_product_takes_values(a, width))
+      return hip_status(run_mx_product_values(a, dtype, x, x_dtype, x_stride, width, s),
+                        "mx_linear launch");
     CHECK(hip_status(run_mx_quantise({const_cast<void*>(x), rows, width, x_stride, space,
                                       space_scales}, x_dtype, kMxFp4, s), "mx_quantise launch"));
-    codes = space;
-    scales = space_scales;
+    a.x = space;
+    a.x_scales = space_scales;
   }
-  const MxProductArgs a{codes, scales, static_cast<const uint8_t*>(weight), weight_scales, bias,
-                        bias_dtype, out, out_stride, (int)rows, (int)outputs,
-                        (int)(mx_filled(kMxFp4, width) / mx_fill(kMxFp4))};
   return hip_status(run_mx_product(a, dtype, s), "mx_linear launch");
 }
 

@@ -222,6 +222,10 @@ struct MxProductArgs {
   int rows, outputs, steps;
 };
 hipError_t run_mx_product(const MxProductArgs& a, int dtype, hipStream_t s);
+// Whether a call of few rows takes x as values (rows of `width`, `stride` elements apart) at once.
+bool mx_product_takes_values(const MxProductArgs& a, int64_t width);
+hipError_t run_mx_product_values(const MxProductArgs& a, int dtype, const void* x, int x_dtype,
+                                 int64_t stride, int64_t width, hipStream_t s);
 
 // Host-bank pager (pager.hip): pinned host banks, device slots, prefetch and write-back
 // streams.  Slot and key indices are checked by the caller (abi.hip).

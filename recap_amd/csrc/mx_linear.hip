@@ -11,6 +11,7 @@
 // LDS.  118,800 x 2,048 to 8,192 outputs: 1,188 us, 3.36 PFLOP/s, of which a seventh goes to the tiles'
 // starts and stores.  (A library's bf16 product of 8,192^3: 1.2 PFLOP/s.)
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.hpp"
 #include "microscale.hpp"
@@ -280,6 +281,137 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(MxProductArgs a, 
   }
 }
 
+// ---------------------------------------------------------------------------------------
+// A few rows of x (a token, a timestep): the weight is read once, straight into registers, and
+// that is what takes the time.  A workgroup computes 32 outputs of every row; its waves take the
+// steps of the sum in turn, and their parts are added in that order.  x is brought into LDS by every
+// workgroup, as codes or, of few values, from the values themselves (X not Codes), which saves the
+// launch that would make its codes.
+constexpr int kFewRows = 16, kFewWaves = 8, kFewThreads = 64 * kFewWaves;
+constexpr int kBatch = 4;        // steps a wave requests before it uses the first
+constexpr int kPartPitch = 36;   // floats of a row of a wave's part
+constexpr int kFewLds = 64 * 1024;
+__host__ __device__ constexpr int few_code_pitch(int steps) { return steps * kStepBytes + 16; }
+__host__ __device__ constexpr int few_scale_pitch(int steps) { return steps * kStepScales + 4; }
+__host__ __device__ constexpr int64_t few_bytes(int64_t rows, int64_t steps) {
+  return rows * (few_code_pitch((int)steps) + few_scale_pitch((int)steps));
+}
+
+struct Codes {};
+
+template <class O, class X>
+__global__ __launch_bounds__(kFewThreads) void few_rows_kernel(MxProductArgs a, const void* values,
+                                                               int64_t value_stride, int width) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int t = threadIdx.x, lane = t & 63, g = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int n0 = blockIdx.x * 32, n = min(n0 + l32, a.outputs - 1);
+  const uint8_t* wrow = a.w + (int64_t)n * a.steps * kStepBytes + 64 * g;
+  const uint8_t* wscale = a.w_scales + (int64_t)n * a.steps * kStepScales + 4 * g;
+  u32x4 fw[kBatch][4];
+  unsigned sw[kBatch];
+  const auto request = [&](int first) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int step = first + kFewWaves * i;
+      if (step >= a.steps) continue;
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        fw[i][s] = *reinterpret_cast<const u32x4*>(wrow + step * kStepBytes + 16 * s);
+      sw[i] = *reinterpret_cast<const unsigned*>(wscale + step * kStepScales);
+    }
+  };
+  request(wave);
+
+  const int pitch = few_code_pitch(a.steps), spitch = few_scale_pitch(a.steps);
+  char* const scales = lds + a.rows * pitch;
+  const unsigned words = (unsigned)a.steps * (kStepBytes / 4);  // 8 values each
+  for (unsigned c = t; c < a.rows * words; c += kFewThreads) {
+    const unsigned row = c / words, word = c - row * words;
+    unsigned code, scale = 0;
+    if constexpr (std::is_same_v<X, Codes>) {
+      code = reinterpret_cast<const unsigned*>(a.x)[c];
+      if ((word & 3) == 0) scale = a.x_scales[c >> 2];
+    } else {
+      const int at = 8 * word, left = width - at;
+      const int64_t from = row * value_stride + at;
+      float v[8];
+      if (left >= 8) {
+        load_chunk<X>(row_of<X>(values, from), 0, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < left ? load_elem<X>(values, from + e) : 0.0f;
+      }
+      scale = mx_scale<kMxFp4>(quad_max(magnitude_bits(v)));
+      code = mx_fp4_codes(v, scale);
+    }
+    *reinterpret_cast<unsigned*>(lds + row * pitch + 4 * word) = code;
+    if ((word & 3) == 0) scales[row * spitch + (word >> 2)] = (char)scale;
+  }
+  __syncthreads();
+
+  f32x16 acc = {};
+  const char* xrow = lds + min(l32, a.rows - 1) * pitch + 64 * g;
+  const char* xscale = scales + min(l32, a.rows - 1) * spitch + 4 * g;
+  for (int first = wave; first < a.steps; first += kFewWaves * kBatch) {
+    if (first != wave) request(first);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int step = first + kFewWaves * i;
+      if (step >= a.steps) continue;
+      const unsigned sx = *reinterpret_cast<const unsigned*>(xscale + step * kStepScales);
+      const auto pair = [&](auto s) {
+        constexpr int S = decltype(s)::value;
+        acc = mfma_fp4<S>(fw[i][S], lds_load16(xrow, step * kStepBytes + 16 * S), acc, sw[i], sx);
+      };
+      pair(std::integral_constant<int, 0>());
+      pair(std::integral_constant<int, 1>());
+      pair(std::integral_constant<int, 2>());
+      pair(std::integral_constant<int, 3>());
+    }
+  }
+  __syncthreads();  // x is read: its room takes the waves' parts
+
+  float* const part = reinterpret_cast<float*>(lds);
+  if (l32 < a.rows)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<f32x4*>(part + (wave * kFewRows + l32) * kPartPitch + 8 * q + 4 * g) =
+          f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+  __syncthreads();
+  const int m = t >> 3, at = n0 + 4 * (t & 7);
+  if (m >= a.rows || at >= a.outputs) return;
+  f32x4 sum = {};
+  for (int w = 0; w < min(kFewWaves, a.steps); ++w) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(part + (w * kFewRows + m) * kPartPitch + 4 * (t & 7));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += v[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (at + e < a.outputs)
+      store_elem<O>(a.out, m * a.stride + at + e,
+                    sum[e] + (a.bias != nullptr ? load_bias(a, at + e) : 0.0f));
+}
+
+template <class O, class X>
+hipError_t launch_few(const MxProductArgs& a, const void* values, int64_t value_stride, int width,
+                      hipStream_t s) {
+  const int64_t bytes = std::max<int64_t>(few_bytes(a.rows, a.steps),
+                                          kFewWaves * kFewRows * kPartPitch * 4);
+  few_rows_kernel<O, X><<<dim3((unsigned)((a.outputs + 31) / 32)), dim3(kFewThreads), (size_t)bytes,
+                          s>>>(a, values, value_stride, width);
+  return hipGetLastError();
+}
+
+// Where that beats tiles of 64, us: 1 row x 9,216 outputs at 6 steps 4.8 (tiles 5.1), 8 rows 5.3 (5.1),
+// 32 rows 7.6 (5.3); 1 x 8,192 at 8 steps 4.4 (5.9) and at 32 10.3 (18.4); 16 x 2,048 at 28 12.9
+// (14.4); but 1 x 40,000 at 8 13.9 (9.3): x is brought into LDS too often.
+bool few(const MxProductArgs& a) {
+  return a.rows <= (a.steps >= 16 ? 16 : 8) && a.outputs <= 320 * 32 &&
+         few_bytes(a.rows, a.steps) <= kFewLds;
+}
+
 template <class O, int BM, int BN, int WM, int WN>
 hipError_t launch(const MxProductArgs& a, hipStream_t s) {
   const int64_t tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.outputs + BN - 1) / BN;
@@ -296,6 +428,7 @@ hipError_t launch(const MxProductArgs& a, hipStream_t s) {
 // 15.0 / 7.3 / 6.3; 512 x 2,048 at 32 steps 49.7 / 30.2 / 20.7.
 template <class O>
 hipError_t launch_type(const MxProductArgs& a, hipStream_t s) {
+  if (few(a)) return launch_few<O, Codes>(a, nullptr, 0, 0, s);
   const auto tiles = [&](int64_t side) {
     return ((a.rows + side - 1) / side) * ((a.outputs + side - 1) / side);
   };
@@ -310,6 +443,27 @@ hipError_t launch_type(const MxProductArgs& a, hipStream_t s) {
 hipError_t run_mx_product(const MxProductArgs& a, int dtype, hipStream_t s) {
   if (dtype == F32::code) return launch_type<F32>(a, s);
   return dtype == BF16::code ? launch_type<BF16>(a, s) : launch_type<F16>(a, s);
+}
+
+// Every workgroup makes the codes of x anew, which for up to 16 chunks of 8 values a thread saves the
+// launch that would (2 x 1,536 to 9,216, a call among others: 13.1 -> 10.6 us).
+bool mx_product_takes_values(const MxProductArgs& a, int64_t width) {
+  return few(a) && a.rows * width <= 16 * 8 * kFewThreads;
+}
+
+template <class O>
+static hipError_t few_values(const MxProductArgs& a, const void* x, int x_dtype, int64_t stride,
+                             int width, hipStream_t s) {
+  if (x_dtype == F32::code) return launch_few<O, F32>(a, x, stride, width, s);
+  return x_dtype == BF16::code ? launch_few<O, BF16>(a, x, stride, width, s)
+                               : launch_few<O, F16>(a, x, stride, width, s);
+}
+
+hipError_t run_mx_product_values(const MxProductArgs& a, int dtype, const void* x, int x_dtype,
+                                 int64_t stride, int64_t width, hipStream_t s) {
+  if (dtype == F32::code) return few_values<F32>(a, x, x_dtype, stride, (int)width, s);
+  return dtype == BF16::code ? few_values<BF16>(a, x, x_dtype, stride, (int)width, s)
+                             : few_values<F16>(a, x, x_dtype, stride, (int)width, s);
 }
 
 }  // namespace recap

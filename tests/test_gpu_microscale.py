@@ -145,7 +145,8 @@ PRODUCTS = [(1, 1, 1), (1, 32, 1), (2, 64, 3), (1, 256, 64), (3, 257, 5), (5, 10
             (17, 512, 31), (31, 300, 64), (33, 1024, 65), (64, 768, 127), (65, 256, 128), (127, 520, 129),
             (128, 1536, 128), (129, 300, 257), (200, 2048, 96), (255, 1155, 256), (257, 64, 255),
             (300, 1300, 520), (1000, 512, 300), (4, 4096, 1000), (8, 8192, 70), (1, 8192, 2000),
-            (520, 2500, 1030)]
+            (520, 2500, 1030), (16, 4200, 70), (16, 8192, 40), (9, 5000, 33), (7, 20001, 65),
+            (8, 65, 10300), (16, 3841, 32)]
 
 
 @pytest.mark.parametrize("rows,width,outputs", PRODUCTS)
