@@ -592,10 +592,11 @@ int recap_refresh_capture_mx(const void* dense_out, int dtype, int64_t batch, in
  * apart.
  *  - x_scales non-NULL: x holds fp4 codes (x_dtype and x_stride are not read).  NULL: x holds
  *    values of x_dtype, rows x_stride elements apart, which the call brings into fp4 in the
- *    workspace (recap_mx_linear_workspace_size bytes, 16-byte aligned; of no size, and NULL
- *    allowed, with codes).  The workspace needs no contents and keeps none.
+ *    workspace (recap_mx_linear_workspace_size bytes, 16-byte aligned; none, and NULL allowed,
+ *    where that is 0: with codes, and for a few rows).  It needs no contents and keeps none.
  *  - bias [outputs] of bias_dtype (any of the three types) or NULL.
- *  - Codes are 16-byte aligned, scales 8-byte aligned; width is at most 2^22.
+ *  - Codes are 16-byte aligned, scales 8-byte aligned; width is at most 2^22, rows and outputs
+ *    2^29 each and rows * outputs 2^37.
  * Products are exact, sums fp32, rounded once after the bias. */
 int64_t recap_mx_linear_workspace_size(int64_t rows, int64_t width, int64_t outputs, int codes);
 int recap_mx_linear(const void* x, int x_dtype, int64_t x_stride, const uint8_t* x_scales,

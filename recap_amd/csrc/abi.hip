@@ -1438,19 +1438,33 @@ int check_mx(const char* what, int format, int dtype, int64_t rows, int64_t widt
   return RECAP_OK;
 }
 
-int check_mx_rows(const char* what, const void* values, int dtype, int64_t rows, int64_t width,
-                  int64_t stride, bool output, const void* codes, const void* scales) {
-  REQUIRE(values && codes && scales, "%s: NULL pointer", what);
+int check_mx_values(const char* what, const void* values, int dtype, int64_t rows, int64_t width,
+                    int64_t stride, bool output) {
+  REQUIRE(values, "%s: NULL pointer", what);
   REQUIRE((reinterpret_cast<uintptr_t>(values) & (dtype == RECAP_F32 ? 3 : 1)) == 0,
           "%s: values are misaligned for their type", what);
   REQUIRE(stride >= 0, "%s: row stride %lld must be non-negative", what, (long long)stride);
   REQUIRE(!output || rows == 1 || stride >= width, "%s: row stride %lld lets rows of %lld overlap",
           what, (long long)stride, (long long)width);
+  return RECAP_OK;
+}
+
+int check_mx_codes(const char* what, const void* codes, const void* scales) {
+  REQUIRE(codes && scales, "%s: NULL pointer", what);
   REQUIRE(aligned16(codes), "%s: codes must be 16-byte aligned", what);
   return RECAP_OK;
 }
 
-constexpr int64_t kMaxLinearWidth = int64_t(1) << 22;
+// Of a product: its launch's threads stay under 2^32, its tiles' bytes under 2^31.
+constexpr int64_t kMaxLinearWidth = int64_t(1) << 22, kMaxLinearRows = int64_t(1) << 29,
+                  kMaxLinearOut = int64_t(1) << 37;
+
+bool linear_fits(int64_t rows, int64_t width, int64_t outputs) {
+  return rows >= 1 && width >= 1 && outputs >= 1 && width <= kMaxLinearWidth &&
+         rows <= kMaxLinearRows && outputs <= kMaxLinearRows && rows <= kMaxLinearOut / outputs;
+}
+
+int linear_steps(int64_t width) { return (int)(mx_filled(kMxFp4, width) / mx_fill(kMxFp4)); }
 
 }  // namespace
 
@@ -1468,7 +1482,8 @@ int recap_mx_quantise(const void* values, int dtype, int64_t rows, int64_t width
                       int64_t row_stride, int format, void* codes, uint8_t* scales,
                       void* stream) {
   CHECK(check_mx("mx_quantise", format, dtype, rows, width));
-  CHECK(check_mx_rows("mx_quantise", values, dtype, rows, width, row_stride, false, codes, scales));
+  CHECK(check_mx_values("mx_quantise", values, dtype, rows, width, row_stride, false));
+  CHECK(check_mx_codes("mx_quantise", codes, scales));
   return hip_status(run_mx_quantise({const_cast<void*>(values), rows, width, row_stride, codes,
                                      scales}, dtype, format, as_stream(stream)), "mx_quantise launch");
 }
@@ -1477,17 +1492,21 @@ int recap_mx_dequantise(const void* codes, const uint8_t* scales, int format, in
                         int64_t width, void* values, int dtype, int64_t row_stride,
                         void* stream) {
   CHECK(check_mx("mx_dequantise", format, dtype, rows, width));
-  CHECK(check_mx_rows("mx_dequantise", values, dtype, rows, width, row_stride, true, codes, scales));
+  CHECK(check_mx_values("mx_dequantise", values, dtype, rows, width, row_stride, true));
+  CHECK(check_mx_codes("mx_dequantise", codes, scales));
   return hip_status(run_mx_dequantise({values, rows, width, row_stride, const_cast<void*>(codes),
                                        const_cast<uint8_t*>(scales)}, dtype, format,
                                       as_stream(stream)), "mx_dequantise launch");
 }
 
 int64_t recap_mx_linear_workspace_size(int64_t rows, int64_t width, int64_t outputs, int codes) {
-  if (rows < 1 || width < 1 || outputs < 1 || rows > INT32_MAX || outputs > INT32_MAX ||
-      width > kMaxLinearWidth)
-    return -1;
-  return codes ? 0 : rows * (mx_row_bytes(kMxFp4, width) + mx_row_scales(kMxFp4, width));
+  if (!linear_fits(rows, width, outputs)) return -1;
+  MxProductArgs a{};
+  a.rows = (int)rows;
+  a.outputs = (int)outputs;
+  a.steps = linear_steps(width);
+  if (codes || mx_product_takes_values(a, width)) return 0;
+  return rows * (mx_row_bytes(kMxFp4, width) + mx_row_scales(kMxFp4, width));
 }
 
 int recap_mx_linear(const void* x, int x_dtype, int64_t x_stride, const uint8_t* x_scales,
@@ -1495,9 +1514,9 @@ int recap_mx_linear(const void* x, int x_dtype, int64_t x_stride, const uint8_t*
                     int64_t outputs, const void* bias, int bias_dtype, void* out, int dtype,
                     int64_t out_stride, void* workspace, int64_t workspace_bytes, void* stream) {
   CHECK(check_mx("mx_linear", RECAP_MX_FP4, dtype, rows, width));
-  REQUIRE(outputs >= 1 && outputs <= INT32_MAX, "mx_linear: outputs %lld outside 1..2^31-1",
-          (long long)outputs);
-  REQUIRE(width <= kMaxLinearWidth, "mx_linear: width %lld exceeds 2^22", (long long)width);
+  REQUIRE(linear_fits(rows, width, outputs),
+          "mx_linear: %lld rows of %lld to %lld outputs are none or too many", (long long)rows,
+          (long long)width, (long long)outputs);
   REQUIRE(x && weight && weight_scales && out, "mx_linear: NULL pointer");
   const auto aligned8 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; };
   REQUIRE(aligned16(weight) && aligned8(weight_scales),
@@ -1512,22 +1531,22 @@ int recap_mx_linear(const void* x, int x_dtype, int64_t x_stride, const uint8_t*
   hipStream_t s = as_stream(stream);
   MxProductArgs a{static_cast<const uint8_t*>(x), x_scales, static_cast<const uint8_t*>(weight),
                   weight_scales, bias, bias_dtype, out, out_stride, (int)rows, (int)outputs,
-                  (int)(mx_filled(kMxFp4, width) / mx_fill(kMxFp4))};
+                  linear_steps(width)};
   if (x_scales != nullptr) {
     REQUIRE(aligned16(x) && aligned8(x_scales),
             "mx_linear: x's codes must be 16-byte and its scales 8-byte aligned");
   } else {
+    CHECK(check_mx("mx_linear", RECAP_MX_FP4, x_dtype, rows, width));
+    CHECK(check_mx_values("mx_linear", x, x_dtype, rows, width, x_stride, false));
     const int64_t need = recap_mx_linear_workspace_size(rows, width, outputs, 0);
+    if (need == 0)
+      return hip_status(run_mx_product_values(a, dtype, x, x_dtype, x_stride, width, s),
+                        "mx_linear launch");
     REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= need,
             "mx_linear: workspace of %lld bytes, need %lld, 16-byte aligned",
             (long long)workspace_bytes, (long long)need);
-    CHECK(check_mx("mx_linear", RECAP_MX_FP4, x_dtype, rows, width));
     uint8_t* space = static_cast<uint8_t*>(workspace);
     uint8_t* space_scales = space + rows * mx_row_bytes(kMxFp4, width);
-    CHECK(check_mx_rows("mx_linear", x, x_dtype, rows, width, x_stride, false, space, space_scales));
-    if (mx_product_takes_values(a, width))
-      return hip_status(run_mx_product_values(a, dtype, x, x_dtype, x_stride, width, s),
-                        "mx_linear launch");
     CHECK(hip_status(run_mx_quantise({const_cast<void*>(x), rows, width, x_stride, space,
                                       space_scales}, x_dtype, kMxFp4, s), "mx_quantise launch"));
     a.x = space;

@@ -32,9 +32,11 @@ def test_layouts(format, width, row, scales):
 
 def test_workspace_size():
     size = _lib.load().recap_mx_linear_workspace_size
-    assert size(5, 300, 7, 0) == 5 * (256 + 16) and size(5, 300, 7, 1) == 0
+    assert size(100, 300, 7, 0) == 100 * (256 + 16) and size(100, 300, 7, 1) == 0
+    assert size(5, 300, 7, 0) == 0      # few rows: brought into fp4 where they are multiplied
     assert size(0, 300, 7, 0) == size(5, 0, 7, 0) == size(5, 300, 0, 1) == -1
-    assert size(5, (1 << 22) + 1, 7, 0) == size(1 << 31, 300, 7, 0) == -1
+    assert size(5, (1 << 22) + 1, 7, 0) == size((1 << 29) + 1, 300, 7, 0) == -1
+    assert size(5, 300, (1 << 29) + 1, 1) == size(1 << 20, 300, (1 << 17) + 1, 1) == -1
 
 
 def wide_out(strides, dtype=BF, shape=(4, 6, 40)):
@@ -92,9 +94,9 @@ def c_call(name, **change):
                                scales=64, stream=None),
         recap_mx_dequantise=dict(codes=64, scales=64, format=1, rows=4, width=96, values=64, dtype=2,
                                  stride=96, stream=None),
-        recap_mx_linear=dict(x=64, x_dtype=2, x_stride=96, x_scales=None, rows=4, width=96, w=64,
+        recap_mx_linear=dict(x=64, x_dtype=2, x_stride=96, x_scales=None, rows=40, width=96, w=64,
                              w_scales=64, outputs=40, bias=64, bias_dtype=2, out=64, dtype=2,
-                             out_stride=40, work=64, work_bytes=4 * 136, stream=None))[name]
+                             out_stride=40, work=64, work_bytes=40 * 136, stream=None))[name]
     assert set(change) <= set(base)
     return _lib.call(name, *{**base, **change}.values())
 
@@ -109,8 +111,9 @@ def c_call(name, **change):
         dict(rows=-1), dict(width=0), dict(stride=95), dict(stride=0), dict(values=65), dict(codes=72))),
     *(("recap_mx_linear", c) for c in (
         dict(x=None), dict(w=None), dict(w_scales=None), dict(out=None), dict(work=None),
-        dict(work_bytes=4 * 136 - 1), dict(work=72), dict(x_dtype=5), dict(dtype=4), dict(bias_dtype=9),
+        dict(work_bytes=40 * 136 - 1), dict(work=72), dict(x_dtype=5), dict(dtype=4), dict(bias_dtype=9),
         dict(rows=0), dict(width=0), dict(outputs=0), dict(width=(1 << 22) + 1), dict(outputs=1 << 31),
+        dict(rows=(1 << 29) + 1, x_scales=64), dict(rows=1 << 20, outputs=(1 << 17) + 1, x_scales=64),
         dict(x_stride=-96), dict(x=65), dict(out=65), dict(out=66, dtype=3), dict(bias=65),
         dict(bias=66, bias_dtype=3), dict(out_stride=39), dict(w=72), dict(w_scales=68),
         dict(x_scales=68), dict(x=72, x_scales=64)))])
