@@ -11,9 +11,9 @@
 //
 // The refinement is kept as fp16 or as int8 with a scale for every 32 channels (microscale.hpp): the
 // four lanes that hold a block take its largest magnitude and D is rounded once, from fp32, to its
-// codes.  There 1 - ratio is -expm1(lh - lf) and DL = (lf - gl) + ln(1 - ratio), which keep the
-// digits that the difference of two near values in fp32 loses (a row whose head holds all but
-// 4e-4 of the mass: 1.5e-4 off against 1e-7).
+// codes.  There 1 - ratio is -expm1(lh - lf), D = (of - oh) / (1 - ratio) + oh - go and DL =
+// (lf - gl) + ln(1 - ratio), which keep the digits that the difference of two near values in fp32
+// loses (a row whose head holds all but 4e-4 of the mass: DL 1.5e-4 off against 1e-7).
 #include <mutex>
 
 #include "kernels.hpp"
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256) void capture_kernel(CaptureArgs a) {
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float tail = (of[e] - ratio * oh[e]) / den;
+      const float tail = MX ? (of[e] - oh[e]) / den + oh[e] : (of[e] - ratio * oh[e]) / den;
       const float cached = fmaxf(fminf(tail - go[e], 6.0e4f), -6.0e4f);
       v[e] = ratio > 1.0f - 1.0e-3f ? 0.0f : cached;
     }
