@@ -175,17 +175,29 @@ hipError_t launch(MxRowsArgs a, bool read, hipStream_t s) {
     a.rows = 1;
   }
   a.chunks = mx_filled(FORMAT, a.width) / 8;
-  // The lanes a row that give the fewest workgroups, the most of those: a row of 1,155 in fp4 (160
-  // chunks) goes in five segments of 8 lanes (15,876 rows: 13.1 us; in one of 64 lanes 15.3).
+  // The lanes of a row: the fewest workgroups, weighted by what the short stretches of memory cost
+  // that few lanes reach at once.  us by 8, 16, 32, 64 and 128 lanes: 118,800 rows of 1,155 into fp4
+  // 83, 74, 87, 98, 131 and back 97, 87, 109, 72, 95; 40,000 of 2,283 57, 53, 51, 62, 56 and 64, 57,
+  // 53, 70, 49; 311,850 of 37 26, 46, 85, ... and 15, 20, 35, ...
   const auto blocks = [&](int64_t n) {
     const int64_t per_block = kThreads / n;
     return (a.rows + per_block - 1) / per_block * ((a.chunks + n * kChunks - 1) / (n * kChunks));
   };
+  const auto cost = [&](int64_t n) {
+    const double weight = read ? (n >= 64 ? 1.0 : n == 32 ? 1.2 : n == 16 ? 1.55 : n == 8 ? 1.9 : 2.6)
+                               : (n >= 32 ? 1.0 : n == 16 ? 1.15 : n == 8 ? 1.45 : 1.9);
+    return weight * (double)blocks(n);
+  };
   int lanes = kThreads;
   for (int n = kThreads / 2; n >= 4; n /= 2)
-    if (blocks(n) < blocks(lanes)) lanes = n;
+    if (cost(n) < cost(lanes)) lanes = n;
   const int64_t segments = (a.chunks + lanes * kChunks - 1) / (lanes * kChunks), all = blocks(lanes);
-  const bool past = a.rows * a.width * (kBytes<T> + 1) >= kStreamBytes;
+  // Past the caches only whole lines: fp32 values read back are stored 16 bytes of 32 at a time, and
+  // rows off 16 bytes share their ends (us through them -> past them: 118,800 x 2,048 112 -> 100,
+  // 60,000 x 2,048 of fp32 read back 111 -> 201, 118,800 x 1,155 82 -> 98).
+  const bool past = a.rows * a.width * (kBytes<T> + 1) >= kStreamBytes &&
+                    (reinterpret_cast<uintptr_t>(a.values) | a.stride * kBytes<T>) % 16 == 0 &&
+                    !(read && T::code == F32::code);
   for (int64_t first = 0; first < all; first += kMaxBlocks) {
     const dim3 grid((unsigned)std::min(all - first, kMaxBlocks));
     const auto launch = [&](auto stream) {
