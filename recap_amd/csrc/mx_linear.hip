@@ -85,9 +85,6 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(MxProductArgs a, 
   const int m0 = tm * BM, n0 = tn * BN;
   const int pitch = a.steps * kStepBytes, spitch = a.steps * kStepScales;
 
-  for (int i = t; i < BN; i += kThreads)
-    bias[i] = a.bias != nullptr && n0 + i < a.outputs ? load_bias(a, n0 + i) : 0.0f;
-
   // Copies into LDS go 16 bytes a lane (4 for scales) in lane order, 8 rows (32) an instruction.  A
   // row's 8 chunks are exchanged by row, so that the lanes of a fragment read distinct banks.  Rows
   // past the last are copies of it and not stored.
@@ -184,7 +181,11 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(MxProductArgs a, 
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  // The sums start from the bias.
+  // The sums start from the bias, fetched behind the first step, which it would hold up.
+  const auto fetch_bias = [&]() {
+    for (int i = t; i < BN; i += kThreads)
+      bias[i] = a.bias != nullptr && n0 + i < a.outputs ? load_bias(a, n0 + i) : 0.0f;
+  };
   const auto start = [&]() {
 #pragma unroll
     for (int j = 0; j < FN; ++j)
@@ -203,6 +204,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(MxProductArgs a, 
   const int odd = a.steps & 1;
   if (odd) {
     fetch(x1, w1, s1, 0);
+    fetch_bias();
     step_barrier();
     start();
     if (a.steps > 1) fetch(x0, w0, s0, 1);
@@ -211,6 +213,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(MxProductArgs a, 
     advance(x1, w1, s1, x0, w0, s0, 1, 0);
   } else {
     fetch(x0, w0, s0, 0);
+    fetch_bias();
     step_barrier();
     start();
     fetch(x1, w1, s1, 1);

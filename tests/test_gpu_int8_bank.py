@@ -229,3 +229,48 @@ def test_refusals(cuda):
         K.refresh_capture_noalloc(*p.values(), bank, mass, None)
     with pytest.raises(ValueError, match="bank_format"):
         build(Operator, SMALL["tiny"], bank_format="int4")
+
+
+def test_text_retarget_and_reset(cuda):
+    """A per-prompt text length after the banks were preallocated, and a new sample: paged banks of
+    another geometry, as the resident ones."""
+    base = SMALL["text-last-d128"]
+    wl = dataclasses.replace(base, text_tokens=16)
+    resident, paged = (build(c, wl, layers=2, bank_format="int8") for c in (Operator, HostBankOperator))
+    assert paged.preallocate_host(2, wl.heads, wl.dim) > 0
+    for text in (16, 300, 77):
+        wl = dataclasses.replace(base, text_tokens=text)
+        for op in (resident, paged):
+            op.reset()
+            op.layout.text_tokens = text
+            op.layout._gather_cache.clear()
+        for step, kind in enumerate((REFRESH, SPARSE, SPARSE, REFRESH, SPARSE)):
+            for layer in range(2):
+                qkv = inputs(wl, step + 1, cuda, seed=layer)[step]
+                outs = []
+                for op in (resident, paged):
+                    if layer == 0:
+                        op.begin_step(step, kind)
+                    outs.append(op.attend(layer, *qkv))
+                assert torch.equal(*outs), (text, step, layer)
+
+
+def test_graph_replays(cuda):
+    """A captured sparse call with the int8 bank, replayed on new inputs between eager ones."""
+    wl = SMALL["text-last-d128"]
+    calls = inputs(wl, 5, cuda)
+    op = build(Operator, wl, bank_format="int8")
+    op.begin_step(0, REFRESH)
+    op.attend(0, *calls[0])
+    op.begin_step(1, SPARSE)
+    held = tuple(x.clone() for x in calls[1])
+    op.attend(0, *held)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = op.attend(0, *held)
+    for call in calls[2:]:
+        for x, new in zip(held, call):
+            x.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, op.attend(0, *call))
