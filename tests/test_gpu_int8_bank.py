@@ -31,10 +31,12 @@ def parts(seed, batch, heads, dim, n_video, n_text, dtype=BF, spread=1.0):
     dense_lse = torch.empty_like(lse)
     dense_lse[:, rowmap.long()] = lse
     size = (spread * rand(dim)).exp()
+    far = torch.zeros(rows, device="cuda")      # masses past their limits of +-30
+    far[3::11], far[8::11] = 1, -1
     return dict(dense_out=(rand(batch, heads, n, dim) * size).to(dtype),
                 dense_lse=dense_lse.view(batch, heads, n), head_out=(rand(banks, n, dim) * size).to(dtype),
                 head_lse=lse + ratio.log(), go=(rand(banks, rows, dim) * size).to(dtype),
-                gl=4 + rand(banks, rows), rowmap=rowmap, geo=K.Geometry(n, n_video))
+                gl=4 + rand(banks, rows) + 60 * far, rowmap=rowmap, geo=K.Geometry(n, n_video))
 
 
 def empty_bank(p):
@@ -111,6 +113,23 @@ def test_validation(cuda, batch, heads, dim, n_video, n_text):
     K.refresh_capture(*q.values(), fresh, fresh_mass)
     assert torch.equal(bank.codes, fresh.codes) and torch.equal(bank.scales, fresh.scales)
     assert torch.equal(mass, fresh_mass)
+
+
+def test_capture_limits(cuda):
+    """Values past 6e4 are kept as what 6e4 rounds to, rows whose head holds all of the mass as 0."""
+    p = parts(5, 1, 1, 64, 128, 0)
+    p["dense_lse"].fill_(2.0)
+    p["head_lse"].fill_(2.0 - 0.6931472)    # half of the mass
+    p["head_lse"][:, 64:] = 3.0             # more than all
+    p["dense_out"].fill_(1.0e5)
+    p["dense_out"][..., 32:] *= -1
+    p["head_out"].zero_()
+    p["go"].zero_()
+    bank, mass = empty_bank(p)
+    K.refresh_capture(*p.values(), bank, mass)
+    got = M.read(bank)
+    assert (got[:, :64, :32] == 59904).all() and (got[:, :64, 32:] == -59904).all()
+    assert (got[:, 64:] == 0).all()
 
 
 def build(cls, wl, chunks=1, layers=1, streams=1, **more):
