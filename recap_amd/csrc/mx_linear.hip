@@ -8,7 +8,7 @@
 //
 // Bound by power, then by the copies: from registers the instruction reaches 6.5 PFLOP/s on random
 // codes (10.0 on zeros); 8,192^3 takes 278 us, 3.95 PFLOP/s, and 215 us, 5.1, without the copies into
-// LDS.  118,800 x 2,048 to 8,192 outputs: 1,188 us, 3.36 PFLOP/s, of which a seventh goes to the tiles'
+// LDS.  118,800 x 2,048 to 8,192 outputs: 1,116 us, 3.57 PFLOP/s, of which a seventh goes to the tiles'
 // starts and stores.  (A library's bf16 product of 8,192^3: 1.2 PFLOP/s.)
 #include <algorithm>
 #include <type_traits>
@@ -58,8 +58,8 @@ __device__ inline float load_bias(const MxProductArgs& a, int n) {
   return a.bias_dtype == BF16::code ? load_elem<BF16>(a.bias, n) : load_elem<F16>(a.bias, n);
 }
 
-// A workgroup computes BN outputs of BM rows, waves WN x WM of them.
-template <class O, int BM, int BN, int WM, int WN>
+// A workgroup computes BN outputs of BM rows, waves WN x WM of them.  PAST: stored past the caches.
+template <class O, int BM, int BN, int WM, int WN, bool PAST>
 __global__ __launch_bounds__(64 * WM * WN) void product_kernel(MxProductArgs a, int tiles_m,
                                                                int tiles_n) {
   constexpr int kThreads = 64 * WM * WN;
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(MxProductArgs a, 
       if (m >= a.rows || n >= a.outputs) continue;
       const int64_t to = m * a.stride + n;
       if (n + 16 / kSize <= a.outputs) {
-        store_words4<false>(const_cast<void*>(row_of<O>(a.out, to)), v);
+        store_words4<PAST>(const_cast<void*>(row_of<O>(a.out, to)), v);
       } else {
 #pragma unroll
         for (int e = 0; e < 16 / kSize; ++e)
@@ -415,17 +415,17 @@ bool few(const MxProductArgs& a) {
          few_bytes(a.rows, a.steps) <= kFewLds;
 }
 
-template <class O, int BM, int BN, int WM, int WN>
+template <class O, int BM, int BN, int WM, int WN, bool PAST = false>
 hipError_t launch(const MxProductArgs& a, hipStream_t s) {
   const int64_t tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.outputs + BN - 1) / BN;
-  product_kernel<O, BM, BN, WM, WN><<<dim3((unsigned)(tiles_m * tiles_n)), dim3(64 * WM * WN), 0, s>>>(
+  product_kernel<O, BM, BN, WM, WN, PAST><<<dim3((unsigned)(tiles_m * tiles_n)), dim3(64 * WM * WN), 0, s>>>(
       a, (int)tiles_m, (int)tiles_n);
   return hipGetLastError();
 }
 
 // The largest tile whose rounds over the 256 CUs are worth its size.  A tile of 256 x 256 takes as
 // long as 2.9 of 128 x 128 (two of which a CU holds at once) where it would take four by its work;
-// us at 8 steps, rows x outputs, 256 / 128 / 64 wide: 118,800 x 8,192 1,188 / 1,560 / -;
+// us at 8 steps, rows x outputs, 256 / 128 / 64 wide: 118,800 x 8,192 1,116 / 1,560 / -;
 // 4,600 x 2,048 (144 tiles of 256) 18.4 / 21.1 / 26.7; 19,200 x 1,024 (300) 35.8 / 33.8 / 45.5;
 // 3,000 x 2,048 (96) 17.0 / 13.6 / 18.1; 1,500 x 2,048 15.9 / 9.3 / 10.1; 256 x 2,048
 // 15.0 / 7.3 / 6.3; 512 x 2,048 at 32 steps 49.7 / 30.2 / 20.7.
@@ -437,7 +437,14 @@ hipError_t launch_type(const MxProductArgs& a, hipStream_t s) {
   };
   const auto rounds = [&](int64_t side) { return (double)((tiles(side) + 255) / 256); };
   if (a.rows <= 64 || a.outputs <= 64 || tiles(64) <= 512) return launch<O, 64, 64, 2, 1>(a, s);
-  if (2.9 * rounds(256) < rounds(128) + 0.4) return launch<O, 256, 256, 4, 2>(a, s);
+  if (2.9 * rounds(256) < rounds(128) + 0.4) {
+    // Outputs that cannot stay in the caches, in whole lines, go past them and leave them to the
+    // operands, us through -> past: 118,800 x 8,192 outputs 1,167 -> 1,116, x 2,048 329 -> 292,
+    // 60,000 x 2,048 171 -> 153; but 32,760 x 1,536 49.4 -> 50.4, and rows of 999 18.5 -> 32.
+    const bool past = a.rows * (int64_t)a.outputs * kBytes<O> >= kStreamBytes &&
+                      (reinterpret_cast<uintptr_t>(a.out) | a.stride * kBytes<O>) % 128 == 0;
+    return past ? launch<O, 256, 256, 4, 2, true>(a, s) : launch<O, 256, 256, 4, 2>(a, s);
+  }
   return launch<O, 128, 128, 4, 2>(a, s);
 }
 

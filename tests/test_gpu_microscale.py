@@ -170,7 +170,8 @@ def test_products(cuda, rows, width, outputs, dtype, out):
 # Sizes that take tiles of 128 and of 256, with one, an odd and an even number of steps of the sum.
 @pytest.mark.parametrize("rows,width,outputs", [
     (2300, 200, 1100), (2301, 700, 1129), (2304, 1024, 1152), (1999, 1793, 1283), (8193, 256, 1030),
-    (8200, 513, 1001), (4099, 1000, 2111), (12288, 2048, 1024), (16400, 1155, 999), (70, 2100, 70000)])
+    (8200, 513, 1001), (4099, 1000, 2111), (12288, 2048, 1024), (16400, 1155, 999), (70, 2100, 70000),
+    (50001, 300, 2048)])
 @pytest.mark.parametrize("out", [BF, FP, F32], ids=str)
 def test_large_products(cuda, rows, width, outputs, out):
     print(f"case {rows} {width} {outputs}", flush=True)
