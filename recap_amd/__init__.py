@@ -35,7 +35,8 @@ __all__ = [
     "EXACT", "REFRESH", "REUSE", "SPARSE", "AttentionBlock", "AttentionBranch", "BlockSummary",
     "ClosureBank",
     "Controller", "DetailBank", "HostBankOperator",
-    "Layout", "Microscaled", "MicroscaledLinear", "OperatingPoint", "Operator", "OperatorConfig", "RecapConfig", "RecapSession",
+    "Layout", "Microscaled", "MicroscaledLinear", "OperatingPoint", "Operator", "OperatorConfig",
+    "RecapConfig", "RecapSession",
     "SparseAttention", "SparseGeometry", "config_from_dict", "hilbert_permutation", "install",
     "load_config", "register_builder", "rotary_axes",
 ]

@@ -4,8 +4,8 @@ What the reference's processors and the blocks around them do with torch modules
 (recap/models/hunyuan.py:79-154): the modulated norm of the residual stream, the projections,
 the queries' and keys' norm and rotation, the attention call, the output projection, and the
 gated residual with the next half's modulated norm.  The projections are the model's own
-modules, or ``MicroscaledLinear``s in 4 bits; everything between them runs on the HIP kernels.  A model integration builds one per
-layer in its ``build_operator`` and calls it in the block's forward.
+modules, or ``MicroscaledLinear``s in 4 bits; everything between them runs on the HIP kernels.  A
+model integration builds one per layer in its ``build_operator`` and calls it in the block's forward.
 
 It is a block of one stream: one set of projections, norms and modulations for the tokens of the
 whole sequence.  A block whose text tokens have their own calls the kernels itself, each stream's

@@ -542,12 +542,14 @@ def _sparse_call_bytes(*sizes: int) -> int:
 def sparse_call(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rowmap: torch.Tensor,
                 geo: Geometry, scale: float, theta: float, rank: int, tables: BasisTables,
                 partition: torch.Tensor, kernel_mask: torch.Tensor,
-                det: "torch.Tensor | Microscaled", dl: torch.Tensor, glref: torch.Tensor, alpha_override: float | None = None,
+                det: "torch.Tensor | Microscaled", dl: torch.Tensor, glref: torch.Tensor,
+                alpha_override: float | None = None,
                 out: torch.Tensor | None = None, events=None) -> torch.Tensor:
     """A whole corrected sparse call with a frozen basis in one library call and one
     workspace: kv_pack, closure_tables, coarse_tail and sparse_merge_attn with
-    their outputs bit for bit, in five launches.  ``det`` as in sparse_merge_attn.  ``events``: five timing events recorded
-    before the first stage and after pack, closure (with the tables), coarse and attention."""
+    their outputs bit for bit, in five launches.  ``det`` as in sparse_merge_attn.  ``events``: five
+    timing events recorded before the first stage and after pack, closure (with the tables), coarse
+    and attention."""
     if not q.shape == k.shape == v.shape or not q.dtype == k.dtype == v.dtype:
         raise ValueError("Q, K and V must have the same shape and dtype")
     b, h, n, d = q.shape

@@ -72,6 +72,6 @@ def test_linear_layer(cuda):
     assert torch.equal(micro(x), want)
     wide = recap_amd.MicroscaledLinear(micro.weight, dtype=torch.float32)
     assert wide(x).dtype == torch.float32 and micro(x, dtype=torch.float16).dtype == torch.float16
-    # against the layer's own 16-bit product: fp4 operands, each value within a quarter of itself
+    # against the product of the unrounded x: its values are off by up to a fifth, or 1/14 of the block
     plain = torch.nn.functional.linear(x.float(), K.mx_dequantise(micro.weight, torch.float32))
     assert (wide(x) - plain).norm() < 0.25 * plain.norm()
