@@ -114,6 +114,28 @@ __global__ __launch_bounds__(kThreads) void quantise_kernel(MxRowsArgs a, int la
   a.scales[block] = (uint8_t)own;
 }
 
+// The 32 fp32 values of a block to memory, its four lanes side by side: each lane's own two halves would
+// leave gaps of 16 bytes in a store (us so -> side by side: fp4 4,000 x 4,096 15.7 -> 12.9, 5.8 TB/s,
+// 60,000 x 2,048 111 -> 101; int8 16.0 -> 13.7 and 125 -> 127).
+template <bool STREAM>
+__device__ inline void store_block(void* block, const float (&v)[8]) {
+  const bool odd = threadIdx.x & 1;
+  u32x4 near, far;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int lo = (int)__float_as_uint(v[e]), hi = (int)__float_as_uint(v[4 + e]);
+    const unsigned lo0 = (unsigned)__builtin_amdgcn_mov_dpp(lo, 0x50, 0xf, 0xf, false);  // lanes 0 0 1 1
+    const unsigned hi0 = (unsigned)__builtin_amdgcn_mov_dpp(hi, 0x50, 0xf, 0xf, false);
+    const unsigned lo1 = (unsigned)__builtin_amdgcn_mov_dpp(lo, 0xFA, 0xf, 0xf, false);  // 2 2 3 3
+    const unsigned hi1 = (unsigned)__builtin_amdgcn_mov_dpp(hi, 0xFA, 0xf, 0xf, false);
+    near[e] = odd ? hi0 : lo0;
+    far[e] = odd ? hi1 : lo1;
+  }
+  const int at = 4 * (threadIdx.x & 3);
+  store_words4<STREAM>(place<F32>(block, at), near);
+  store_words4<STREAM>(place<F32>(block, 16 + at), far);
+}
+
 template <class T, int FORMAT, bool STREAM>
 __global__ __launch_bounds__(kThreads) void dequantise_kernel(MxRowsArgs a, int lanes,
                                                               unsigned segments, unsigned first) {
@@ -155,6 +177,13 @@ __global__ __launch_bounds__(kThreads) void dequantise_kernel(MxRowsArgs a, int 
       mx_int8_values(w[j], s[j], v);
     }
     const int64_t to = p.row * a.stride + at;
+    if constexpr (T::code == F32::code) {
+      const int before = 8 * (threadIdx.x & 3);  // in the block
+      if (left + before >= kMxBlock) {
+        store_block<STREAM>(const_cast<void*>(row_of<T>(a.values, to - before)), v);
+        continue;
+      }
+    }
     if (left >= 8) {
       Rounded<T, 8> r;
       r.set(v);
@@ -192,9 +221,9 @@ hipError_t launch(MxRowsArgs a, bool read, hipStream_t s) {
   for (int n = kThreads / 2; n >= 4; n /= 2)
     if (cost(n) < cost(lanes)) lanes = n;
   const int64_t segments = (a.chunks + lanes * kChunks - 1) / (lanes * kChunks), all = blocks(lanes);
-  // Past the caches only whole lines: fp32 values read back are stored 16 bytes of 32 at a time, and
-  // rows off 16 bytes share their ends (us through them -> past them: 118,800 x 2,048 112 -> 100,
-  // 60,000 x 2,048 of fp32 read back 111 -> 201, 118,800 x 1,155 82 -> 98).
+  // Past the caches only whole lines: fp32 values read back are stored half a line at a time, and rows
+  // off 16 bytes share their ends (us through them -> past them: 118,800 x 2,048 112 -> 100, 60,000 x
+  // 2,048 of fp32 read back 101 -> 152, 118,800 x 1,155 82 -> 98).
   const bool past = a.rows * a.width * (kBytes<T> + 1) >= kStreamBytes &&
                     (reinterpret_cast<uintptr_t>(a.values) | a.stride * kBytes<T>) % 16 == 0 &&
                     !(read && T::code == F32::code);
