@@ -597,7 +597,8 @@ int recap_refresh_capture_mx(const void* dense_out, int dtype, int64_t batch, in
  *  - bias [outputs] of bias_dtype (any of the three types) or NULL.
  *  - Codes are 16-byte aligned, scales 8-byte aligned; width is at most 2^22, rows and outputs
  *    2^29 each and rows * outputs 2^37.
- * Products are exact, sums fp32, rounded once after the bias. */
+ * Products are exact, sums fp32; the bias is added to the whole sum in fp32 on every path, and that is
+ * rounded to dtype. */
 int64_t recap_mx_linear_workspace_size(int64_t rows, int64_t width, int64_t outputs, int codes);
 int recap_mx_linear(const void* x, int x_dtype, int64_t x_stride, const uint8_t* x_scales,
                     int64_t rows, int64_t width, const void* weight, const uint8_t* weight_scales,

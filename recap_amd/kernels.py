@@ -1369,7 +1369,7 @@ def mx_linear(x: torch.Tensor | Microscaled, weight: Microscaled,
     projection's weight, once), ``x`` ``[..., width]`` is fp4 too, or a bfloat16, float16 or float32
     tensor that the call brings into fp4.  Several projections of the same rows quantise them once
     and pass the Microscaled.  Products are exact and sums fp32; the result has ``dtype`` (x's own,
-    bfloat16 for codes), rounded once after the bias.  ``out`` may be rows an even step apart (a
+    bfloat16 for codes), rounded from fp32 after the bias.  ``out`` may be rows an even step apart (a
     part of a wider tensor)."""
     micro = isinstance(x, Microscaled)
     tensors = (x.codes, x.scales) if micro else (x, None)

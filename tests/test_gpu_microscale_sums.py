@@ -1,5 +1,5 @@
 """The fp32 sums of mx_linear on the GPU, bit for bit: operands whose sums fp32 holds exactly in any
-order, over every kernel's sizes and number of steps."""
+order, over every kernel's sizes and number of steps, and a bias far larger than the products."""
 
 import pytest
 import torch
@@ -32,3 +32,18 @@ def test_sums_are_exact(cuda, rows, width, outputs):
     for out in (F32, BF, FP):
         S.check_exact(K.mx_linear(kept, weight, dtype=out), x, w, None, f"{out}")
     S.check_exact(K.mx_linear(x, weight, dtype=F32), x, w, None, "values")
+
+@pytest.mark.parametrize("rows,width,outputs", SIZES)
+def test_large_bias(cuda, rows, width, outputs):
+    """The bias is added to the whole sum, with one rounding: 1e4 and more times the products, it takes
+    nothing from them but that."""
+    print(f"case {rows} {width} {outputs}", flush=True)
+    x, w = operands(rows, width, outputs)
+    weight = K.mx_quantise(w)
+    g = torch.Generator(device="cuda").manual_seed(width)
+    for size in (1e4, 1e8):
+        bias = size * torch.randn(outputs, generator=g, device="cuda")
+        for out in (F32, BF):
+            S.check_exact(K.mx_linear(x, weight, bias, dtype=out), x, w, bias, f"{size} {out}")
+    few = K.mx_linear(x[:1], weight, bias, dtype=F32)
+    assert torch.equal(few, K.mx_linear(x, weight, bias, dtype=F32)[:1])
