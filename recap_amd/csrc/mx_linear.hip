@@ -413,12 +413,17 @@ hipError_t launch_few(const MxProductArgs& a, const void* values, int64_t value_
   return hipGetLastError();
 }
 
-// Where that beats tiles of 64, us: 1 row x 9,216 outputs at 6 steps 4.8 (tiles 5.1), 8 rows 5.3 (5.1),
-// 32 rows 7.6 (5.3); 1 x 8,192 at 8 steps 4.4 (5.9) and at 32 10.3 (18.4); 16 x 2,048 at 28 12.9
-// (14.4); but 1 x 40,000 at 8 13.9 (9.3): x is brought into LDS too often.
+// Where that beats tiles of 64; us, few rows / tiles, the launch that makes the codes of x with both where
+// it is needed.  Values: 1 row x 1,536 to 9,216 outputs 5.1 / 8.6, 8 rows 6.6 / 8.7; 1 x 8,192 to 8,192
+// 10.7 / 29.6; 8 x 8,192 to 2,048 14.2 / 21.5; 16 x 4,096 to 2,048 11.6 / 13.8.  More than 65,536 values,
+// which have that launch here too: 8 x 14,336 to 2,048 27.7 / 33.4, 10 x 8,192 20.3 / 21.6, but 12 x 8,192
+// 22.8 / 21.7 and 16 x 5,120 18.4 / 15.3.  8 x 2,048 to 20,000 11.3 / 10.8: x is brought into LDS too
+// often.  Codes go the way of values, so that both have the same sums: 1 x 8,192 to 8,192 13.8 / 29.6,
+// 8 x 8,192 to 2,048 18.5 / 21.5, 8 x 1,536 to 9,216 8.7 / 8.7, 8 x 256 to 1,024 5.8 / 5.6, 16 x 4,096 to
+// 2,048 15.9 / 13.8; 16 x 1,536 to 1,536, 9.2 / 8.3 (values 5.7 / 8.4), is left to the tiles.
 bool few(const MxProductArgs& a) {
-  return a.rows <= (a.steps >= 16 ? 16 : 8) && a.outputs <= 320 * 32 &&
-         few_bytes(a.rows, a.steps) <= kFewLds;
+  const int most = a.steps < 16 ? 8 : a.rows * a.steps <= 256 ? kFewRows : 10;
+  return a.rows <= most && a.outputs <= 320 * 32 && few_bytes(a.rows, a.steps) <= kFewLds;
 }
 
 template <class O, int BM, int BN, int WM, int WN, bool PAST = false>
