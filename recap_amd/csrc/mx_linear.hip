@@ -422,7 +422,7 @@ hipError_t launch_few(const MxProductArgs& a, const void* values, int64_t value_
 // 8 x 8,192 to 2,048 18.5 / 21.5, 8 x 1,536 to 9,216 8.7 / 8.7, 8 x 256 to 1,024 5.8 / 5.6, 16 x 4,096 to
 // 2,048 15.9 / 13.8; 16 x 1,536 to 1,536, 9.2 / 8.3 (values 5.7 / 8.4), is left to the tiles.
 bool few(const MxProductArgs& a) {
-  const int most = a.steps < 16 ? 8 : a.rows * a.steps <= 256 ? kFewRows : 10;
+  const int most = a.steps < 16 ? 8 : a.steps * kFewRows <= 256 ? kFewRows : std::max(10, 256 / a.steps);
   return a.rows <= most && a.outputs <= 320 * 32 && few_bytes(a.rows, a.steps) <= kFewLds;
 }
 
