@@ -231,7 +231,8 @@ class Operator:
     _forced_partition: torch.Tensor | None = None
     _forced_rerank: bool | None = None
     #: how a refresh keeps its refinement: "fp16", as the reference does, or "int8", microscaled
-    #: (half the memory, the paging and the reading; each value within half a step of its block)
+    #: (half the memory, the paging and the reading; each value within half a step of its block);
+    #: fixed when the operator is built
     bank_format: str = "fp16"
 
     # The per-(stream, layer) state is a grid of cells: the sparse state in ``layers`` and
@@ -246,6 +247,12 @@ class Operator:
         if self.bank_format not in BANK_FORMATS:
             raise ValueError(f"unknown bank_format {self.bank_format!r}; use one of {BANK_FORMATS}")
         self.banks = [[DetailBank() for _ in row] for row in rows]
+
+    def __setattr__(self, name: str, value) -> None:
+        # Banks, slots and pinned memory are laid out for one format.
+        if name == "bank_format" and name in self.__dict__:
+            raise AttributeError("bank_format is fixed when the operator is built")
+        super().__setattr__(name, value)
 
     @classmethod
     def build(cls, config: OperatorConfig, geometry: SparseGeometry, *, n_layers: int,
