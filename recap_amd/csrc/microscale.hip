@@ -205,9 +205,11 @@ hipError_t launch(MxRowsArgs a, bool read, hipStream_t s) {
   }
   a.chunks = mx_filled(FORMAT, a.width) / 8;
   // The lanes of a row: the fewest workgroups, weighted by what the short stretches of memory cost
-  // that few lanes reach at once.  us by 8, 16, 32, 64 and 128 lanes: 118,800 rows of 1,155 into fp4
-  // 83, 74, 87, 98, 131 and back 97, 87, 109, 72, 95; 40,000 of 2,283 57, 53, 51, 62, 56 and 64, 57,
-  // 53, 70, 49; 311,850 of 37 26, 46, 85, ... and 15, 20, 35, ...
+  // that few lanes reach at once.  us by 8, 16, 32, 64 and 128 lanes, bf16: 118,800 rows of 1,155 into
+  // fp4 80, 72, 86, 96, 132 and back 91, 84, 116, 81, 107; 40,000 of 2,283 48, 45, 43, 54, 49 and 43,
+  // 41, 39, 45, 37; 311,850 of 37 27, 47, 87, ... and 16, 21, 36, ...  At these and five more sizes in
+  // both formats the rule's choice takes up to 7% longer than the best number; of fp32, 8% (once 14:
+  // 118,800 x 1,155 into int8 137 with 16 lanes, 120 with 128).
   const auto blocks = [&](int64_t n) {
     const int64_t per_block = kThreads / n;
     return (a.rows + per_block - 1) / per_block * ((a.chunks + n * kChunks - 1) / (n * kChunks));
@@ -221,18 +223,17 @@ hipError_t launch(MxRowsArgs a, bool read, hipStream_t s) {
   for (int n = kThreads / 2; n >= 4; n /= 2)
     if (cost(n) < cost(lanes)) lanes = n;
   const int64_t segments = (a.chunks + lanes * kChunks - 1) / (lanes * kChunks), all = blocks(lanes);
-  // Past the caches only whole lines: fp32 values read back are stored half a line at a time, and rows
-  // off 16 bytes share their ends (us through them -> past them: 118,800 x 2,048 112 -> 100, 60,000 x
-  // 2,048 of fp32 read back 101 -> 152, 118,800 x 1,155 82 -> 98).
+  // Past the caches only whole lines: fp32 values read back are stored half a line at a time and never
+  // go past them, and rows off 16 bytes share their ends (us through them -> past them: 118,800 x 2,048
+  // 112 -> 100, 60,000 x 2,048 of fp32 read back 101 -> 152, 118,800 x 1,155 82 -> 98).
   const bool past = a.rows * a.width * (kBytes<T> + 1) >= kStreamBytes &&
-                    (reinterpret_cast<uintptr_t>(a.values) | a.stride * kBytes<T>) % 16 == 0 &&
-                    !(read && T::code == F32::code);
+                    (reinterpret_cast<uintptr_t>(a.values) | a.stride * kBytes<T>) % 16 == 0;
   for (int64_t first = 0; first < all; first += kMaxBlocks) {
     const dim3 grid((unsigned)std::min(all - first, kMaxBlocks));
     const auto launch = [&](auto stream) {
       constexpr bool STREAM = decltype(stream)::value;
       if (read) {
-        dequantise_kernel<T, FORMAT, STREAM>
+        dequantise_kernel<T, FORMAT, STREAM && T::code != F32::code>
             <<<grid, dim3(kThreads), 0, s>>>(a, lanes, (unsigned)segments, (unsigned)first);
       } else {
         quantise_kernel<T, FORMAT, STREAM>
