@@ -533,7 +533,9 @@ int recap_gated_residual_norm(const void* x, int x_dtype, int64_t batch, int64_t
  *                  sign in bit 3, two to a byte, the first in the low half.  Rows are filled up
  *                  with zeros to a multiple of 256 values.
  *   RECAP_MX_INT8  e the smallest, from -127 on, with 64 a < 127.5 * 2^e; a code c is an integer
- *                  of -127 .. 127, its value c * 2^(e - 6).  Rows are filled up to whole blocks.
+ *                  of -127 .. 127, its value c * 2^(e - 6).  e is 127 at most: magnitudes from
+ *                  127.5 * 2^121 on (fp32 only) read as 127 * 2^121.  Rows are filled up to whole
+ *                  blocks.
  * Ties go to the even code.  A block with an infinity or NaN has the byte 255 and reads as NaN.
  * recap_mx_row_bytes and recap_mx_row_scales give the bytes of a row's codes and of its scales;
  * rows follow one another without gaps.

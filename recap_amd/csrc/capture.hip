@@ -23,6 +23,10 @@ namespace recap {
 
 // Rows of a thread, all of whose loads are sent out first.  At 24 heads x 118,800 x 128 the int8
 // capture takes 516 us with one row through the caches, 489 past them and 447 with two (5.8 TB/s).
+// It goes past the caches at every size.  us past / through them, alone in a loop, and between the three
+// writes of its inputs and a reading back of the bank: 4 MB in all 3.7 / 3.7 and 13.5 / 13.1, 63 MB
+// 14.1 / 15.7 and 42.7 / 42.2, 127 MB 25.7 / 26.0 and 78 / 85, 335 MB 63 / 67 and 200 / 210, 2.4 GB
+// 447 / 476 and 1,440 / 1,508.
 template <bool MX>
 constexpr int kRowsEach = MX ? 2 : 1;
 

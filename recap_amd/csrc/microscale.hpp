@@ -5,7 +5,8 @@
 //   fp4   e the smallest with a < 7 * 2^e: the largest value then rounds to at most 6, the largest
 //         code, and every value is within half a step of its own.  Codes are sign, two exponent and
 //         one mantissa bits (0, 0.5, 1, 1.5, 2, 3, 4, 6); two to a byte, the first in the low half.
-//   int8  e the smallest with 64 a < 127.5 * 2^e; integers up to 127, each worth 2^(e - 6).
+//   int8  e the smallest with 64 a < 127.5 * 2^e; integers up to 127, each worth 2^(e - 6).  e stops at
+//         127: from 127.5 * 2^121 on (1.992 * 2^127, of fp32 alone) values are cut off at 127 * 2^121.
 // Both round to nearest, ties to the even code.  s = 255 marks a block that held an infinity or NaN:
 // all of it reads as NaN.  Scales and products with them are exact, so the same values give the same
 // codes on every path.
@@ -42,7 +43,8 @@ __device__ inline unsigned mx_scale(unsigned bits) {
     s = (bits + 0x200000u) >> 23;
     s = s > 2 ? s - 2 : 0;
   } else {
-    // A subnormal has no leading one of its own: its binade is half as long.
+    // A subnormal has no leading one of its own: its binade is half as long.  254 is the last power of
+    // two; mx_int8_codes cuts off what rounds past 127 of it.
     s = min((bits + (bits < 0x800000u ? 0x8000u : 0x10000u)) >> 23, 254u);
   }
   return bits >= kNotFinite ? 255 : s;

@@ -8,9 +8,10 @@
 // with consecutive outputs of one row of x.
 //
 // Bound by power, then by the copies: from registers the instruction reaches 6.5 PFLOP/s on random
-// codes (10.0 on zeros); 8,192^3 takes 278 us, 3.95 PFLOP/s, and 215 us, 5.1, without the copies into
-// LDS.  118,800 x 2,048 to 8,192 outputs: 1,116 us, 3.57 PFLOP/s, of which a seventh goes to the tiles'
-// starts and stores.  (A library's bf16 product of 8,192^3: 1.2 PFLOP/s.)
+// codes (10.0 on zeros); 8,192^3 takes 256 us on one card and 278 on another, 4.3 and 3.95 PFLOP/s, and
+// on the latter 215 us, 5.1, without the copies into LDS.  118,800 x 2,048 to 8,192 outputs: 1,109-1,137
+// us in a loop, 3.5-3.6 PFLOP/s, up to 1,260 among other calls.  (A library's bf16 product of 8,192^3:
+// 1.2 PFLOP/s.)
 #include <algorithm>
 #include <type_traits>
 
@@ -436,10 +437,10 @@ hipError_t launch(const MxProductArgs& a, hipStream_t s) {
 
 // The largest tile whose rounds over the 256 CUs are worth its size.  A tile of 256 x 256 takes as
 // long as 2.9 of 128 x 128 (two of which a CU holds at once) where it would take four by its work;
-// us at 8 steps, rows x outputs, 256 / 128 / 64 wide: 118,800 x 8,192 1,116 / 1,560 / -;
-// 4,600 x 2,048 (144 tiles of 256) 18.4 / 21.1 / 26.7; 19,200 x 1,024 (300) 35.8 / 33.8 / 45.5;
-// 3,000 x 2,048 (96) 17.0 / 13.6 / 18.1; 1,500 x 2,048 15.9 / 9.3 / 10.1; 256 x 2,048
-// 15.0 / 7.3 / 6.3; 512 x 2,048 at 32 steps 49.7 / 30.2 / 20.7.
+// us at 8 steps, rows x outputs, 256 / 128 / 64 wide: 118,800 x 8,192 1,174 / 1,419 / -;
+// 4,600 x 2,048 (144 tiles of 256) 18.9 / 20.7 / 26.9; 19,200 x 1,024 (300) 35.3 / 31.3 / 46.8;
+// 3,000 x 2,048 (96) 17.1 / 13.4 / 18.5; 1,500 x 2,048 15.7 / 8.6 / 9.7; 256 x 2,048
+// 15.0 / 7.6 / 6.6; 512 x 2,048 at 32 steps 47.4 / 29.5 / 20.8.
 template <class O>
 hipError_t launch_type(const MxProductArgs& a, hipStream_t s) {
   if (few(a)) return launch_few<O, Codes>(a, nullptr, 0, 0, s);
